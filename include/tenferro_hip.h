@@ -77,7 +77,10 @@ typedef enum tfh_dtype {
     TFH_F32 = 0,
     TFH_F64 = 1,
     TFH_C64 = 2,   /* Complex32: interleaved (re, im) f32 */
-    TFH_C128 = 3   /* Complex64: interleaved (re, im) f64 */
+    TFH_C128 = 3,  /* Complex64: interleaved (re, im) f64 */
+    /* 16-bit types: taken by the operations on rows in groups below, by no other */
+    TFH_BF16 = 4,
+    TFH_F16 = 5
 } tfh_dtype;
 size_t tfh_dtype_size(int32_t dtype);
 
@@ -205,6 +208,80 @@ int32_t tfh_conj(int32_t dtype, const tfh_view* in, tfh_view* out, tfh_stream st
 /* Tensor::zeros / ones (tenferro-tensor/src/lib.rs:336-347) on device memory: fill a view with
  * one host scalar of `dtype`. */
 int32_t tfh_fill(int32_t dtype, const void* value, tfh_view* out, tfh_stream stream);
+
+/* ---- rows in groups ------------------------------------------------------------------------------
+ * Additive like the grouped plan above (no counterpart in the reference), for groups that are only known on the device:
+ * which rows belong together is decided by an index per row (a router's choice of experts, a request's adapter, the
+ * sector of a block-sparse tensor's row), so the sizes never reach the host.  All calls enqueue on `stream`, wait for
+ * nothing and allocate nothing; what scratch they need is the caller's (`workspace`), so a captured call keeps to memory
+ * of its own graph.  Scalar types: TFH_BF16, TFH_F16, TFH_F32, TFH_F64.  Sums are held in f32 (f64 for TFH_F64) and
+ * rounded once.  Views may have any strides, negative and zero ones included for inputs; an output may not overlap an
+ * input or itself.  The work runs on the device that is current, on which the memory has to be.
+ *
+ * tfh_row_groups: n_rows rows listed group by group.
+ *   offsets    [n_groups + 1], ascending from 0: group g is p = offsets[g] .. offsets[g + 1]; the rows behind
+ *              offsets[n_groups] belong to no group
+ *   order      [n_rows] or NULL (the rows lie in that order already): place p holds row order[p]
+ *   positions  [n_rows] or NULL: where row i stands, -1 for a row of no group
+ *   fan        rows per source row (a token's choices): row i = t * fan + j is choice j of token t
+ * Entries out of range are treated as absent (offsets are clamped to [0, n_rows]); they never lead out of the views. */
+typedef struct tfh_row_groups {
+    const int32_t* offsets;
+    const int32_t* order;
+    const int32_t* positions;
+    int64_t n_rows;
+    int32_t n_groups;
+    int32_t fan;
+} tfh_row_groups;
+typedef enum tfh_rows_limit { TFH_MAX_ROW_GROUPS = 2048 } tfh_rows_limit;   /* of tfh_group_rows; the products take any number */
+
+/* Stable grouping of rows by an index.  ids: rank 1 [n_rows] or rank 2 [tokens, fan] (row t * fan + j), of 32- or 64-bit
+ * integers (id_bits); an index outside [0, n_groups) puts its row into no group.  Within a group rows keep their order.
+ * Writes offsets [n_groups + 1], order [n_rows] and, unless NULL, positions [n_rows].  workspace: at least
+ * tfh_group_rows_workspace(n_rows, n_groups) bytes (0 for few rows), 16-byte aligned. */
+size_t tfh_group_rows_workspace(int64_t n_rows, int32_t n_groups);
+int32_t tfh_group_rows(int32_t id_bits, const tfh_view* ids, int32_t n_groups, int32_t* offsets, int32_t* order,
+                       int32_t* positions, void* workspace, size_t workspace_bytes, tfh_stream stream);
+
+/* C[p, :] = alpha * A[src(p), :] . B[g(p)] + beta * C[p, :] for every row p in a group g(p): a matrix product for each
+ * group, of as many rows as it happens to have.  A [sources, K], B [n_groups, K, N], C [n_rows, N].
+ * TFH_ROWS_GATHER_A: src(p) = order[p] / fan and sources = n_rows / fan; else src(p) = p and sources = n_rows.
+ * TFH_ROWS_SCATTER_C: the result of p is row order[p] of C.
+ * TFH_ROWS_ZERO_REST: the rows of no group are written as zeros; without it they are left as they are. */
+typedef enum tfh_rows_flag { TFH_ROWS_GATHER_A = 1, TFH_ROWS_SCATTER_C = 2, TFH_ROWS_ZERO_REST = 4 } tfh_rows_flag;
+int32_t tfh_ragged_gemm(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* a,
+                        const tfh_view* b, double beta, const tfh_view* c, tfh_stream stream);
+/* The gradient of that product's B: dB[g] = alpha * sum over p in g of A[src(p), :]^T dC[p, :] + beta * dB[g]; a group
+ * without rows gets beta * dB[g].  (The gradient of A is tfh_ragged_gemm with dC and B transposed.)
+ * A [sources, K], dC [n_rows, N], dB [n_groups, K, N]; of the flags TFH_ROWS_GATHER_A. */
+int32_t tfh_ragged_gemm_grad(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* a,
+                             const tfh_view* dc, double beta, const tfh_view* db, tfh_stream stream);
+
+/* Y[t, :] = sum_j weights[t, j] * X[positions[t * fan + j], :]: the rows of a token joined again.  A choice of no group
+ * adds nothing.  X [n_rows, N], weights [n_rows / fan, fan] of the sums' type (f32; f64 for TFH_F64) or NULL (ones),
+ * Y [n_rows / fan, N].  groups->positions is needed. */
+int32_t tfh_combine_rows(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* weights,
+                         const tfh_view* y, tfh_stream stream);
+/* Its gradients: dX[p, :] = weights[t, j] * dY[t, :] (zeros for rows of no group) and dweights[t, j] = <X[p, :], dY[t, :]>
+ * (0 for a choice of no group).  dx or dweights may be NULL: not wanted; x is read for dweights only. */
+int32_t tfh_combine_rows_grad(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* weights,
+                              const tfh_view* dy, const tfh_view* dx, const tfh_view* dweights, tfh_stream stream);
+
+/* Y[t, :] = X[t, :] . W + scales[g] * (X[t, :] . A[g]) . B[g] for a row t of group g, X[t, :] . W for a row of none: one
+ * matrix for all rows and a low-rank correction of it by group.  X [n_rows, K], W [K, N], A [n_groups, K, R],
+ * B [n_groups, R, N], scales [n_groups] of the sums' type or NULL (ones), Y [n_rows, N]; rows of X and Y in their own
+ * order, not the groups'.  fan must be 1.  workspace: tfh_adapter_workspace(dtype, n_rows, R, 0) bytes, 16-byte aligned. */
+size_t tfh_adapter_workspace(int32_t dtype, int64_t n_rows, int64_t rank, int32_t gradient);
+int32_t tfh_adapter_gemm(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* w, const tfh_view* a,
+                         const tfh_view* b, const tfh_view* scales, const tfh_view* y, void* workspace,
+                         size_t workspace_bytes, tfh_stream stream);
+/* Its gradients for a W that stays as it is: dX = dY . W^T + scales[g] * (dY . B[g]^T) . A[g]^T,
+ * dA[g] = scales[g] * X_g^T . (dY_g . B[g]^T), dB[g] = scales[g] * (X_g . A[g])^T . dY_g with X_g, dY_g the rows of g.
+ * Any of dx, da, db may be NULL: not wanted.  workspace: tfh_adapter_workspace(dtype, n_rows, R, 1) bytes. */
+int32_t tfh_adapter_gemm_grad(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* w,
+                              const tfh_view* a, const tfh_view* b, const tfh_view* scales, const tfh_view* dy,
+                              const tfh_view* dx, const tfh_view* da, const tfh_view* db, void* workspace,
+                              size_t workspace_bytes, tfh_stream stream);
 
 /* ---- einsum front end and executor --------------------------------------------------------- */
 

@@ -27,6 +27,15 @@ pub const TFH_F32: i32 = 0;
 pub const TFH_F64: i32 = 1;
 pub const TFH_C64: i32 = 2;
 pub const TFH_C128: i32 = 3;
+/// 16-bit types: taken by the operations on rows in groups, by no other.
+pub const TFH_BF16: i32 = 4;
+pub const TFH_F16: i32 = 5;
+
+// ---- tfh_rows_limit, tfh_rows_flag: operations on rows in groups
+pub const TFH_MAX_ROW_GROUPS: i32 = 2048;
+pub const TFH_ROWS_GATHER_A: i32 = 1;
+pub const TFH_ROWS_SCATTER_C: i32 = 2;
+pub const TFH_ROWS_ZERO_REST: i32 = 4;
 
 // ---- tfh_op: PrimDescriptor variants (tenferro-prims/src/lib.rs:152-245)
 pub const TFH_OP_BATCHED_GEMM: i32 = 0;
@@ -111,6 +120,18 @@ pub struct tfh_desc {
     pub n_pairs: i32,
 }
 
+/// Rows listed group by group, in device memory: offsets `[n_groups + 1]`, order and positions `[n_rows]` or null.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct tfh_row_groups {
+    pub offsets: *const i32,
+    pub order: *const i32,
+    pub positions: *const i32,
+    pub n_rows: i64,
+    pub n_groups: i32,
+    pub fan: i32,
+}
+
 /// ComputeDevice as (tfh_device_kind, index) (tenferro-device/src/lib.rs:46-62).
 #[repr(C)]
 #[derive(Clone, Copy)]
@@ -166,6 +187,28 @@ extern "C" {
     pub fn tfh_fill(dtype: i32, value: *const c_void, out: *mut tfh_view, stream: tfh_stream) -> i32;
 
     // ---- Subscripts and ContractionTree (tenferro-einsum/src/lib.rs:239-356)
+    // ---- rows in groups
+    pub fn tfh_group_rows_workspace(n_rows: i64, n_groups: i32) -> usize;
+    pub fn tfh_group_rows(id_bits: i32, ids: *const tfh_view, n_groups: i32, offsets: *mut i32, order: *mut i32,
+        positions: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: tfh_stream) -> i32;
+    pub fn tfh_ragged_gemm(dtype: i32, groups: *const tfh_row_groups, flags: i32, alpha: f64, a: *const tfh_view,
+        b: *const tfh_view, beta: f64, c: *const tfh_view, stream: tfh_stream) -> i32;
+    pub fn tfh_ragged_gemm_grad(dtype: i32, groups: *const tfh_row_groups, flags: i32, alpha: f64, a: *const tfh_view,
+        dc: *const tfh_view, beta: f64, db: *const tfh_view, stream: tfh_stream) -> i32;
+    pub fn tfh_combine_rows(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view, weights: *const tfh_view,
+        y: *const tfh_view, stream: tfh_stream) -> i32;
+    pub fn tfh_combine_rows_grad(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view,
+        weights: *const tfh_view, dy: *const tfh_view, dx: *const tfh_view, dweights: *const tfh_view,
+        stream: tfh_stream) -> i32;
+    pub fn tfh_adapter_workspace(dtype: i32, n_rows: i64, rank: i64, gradient: i32) -> usize;
+    pub fn tfh_adapter_gemm(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view, w: *const tfh_view,
+        a: *const tfh_view, b: *const tfh_view, scales: *const tfh_view, y: *const tfh_view, workspace: *mut c_void,
+        workspace_bytes: usize, stream: tfh_stream) -> i32;
+    pub fn tfh_adapter_gemm_grad(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view, w: *const tfh_view,
+        a: *const tfh_view, b: *const tfh_view, scales: *const tfh_view, dy: *const tfh_view, dx: *const tfh_view,
+        da: *const tfh_view, db: *const tfh_view, workspace: *mut c_void, workspace_bytes: usize,
+        stream: tfh_stream) -> i32;
+
     pub fn tfh_subscripts_new(labels: *const u32, ranks: *const i32, n_inputs: i32, output: *const u32,
         n_output: i32, out: *mut *mut tfh_subscripts) -> i32;
     pub fn tfh_subscripts_parse(notation: *const c_char, out: *mut *mut tfh_subscripts) -> i32;

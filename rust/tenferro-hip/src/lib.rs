@@ -8,6 +8,8 @@
 //!   [`HipViewMut`] as the device-side `StridedView` / `StridedViewMut`.
 //! - [`CompletionEvent`] and [`Stream`] (tenferro-tensor/src/lib.rs:301-309, 677-713).
 //! - [`Subscripts`], [`ContractionTree`] and [`einsum_with_plan_into`] (tenferro-einsum/src/lib.rs:239-356, 584-621).
+//! - [`RowGroups`]: products, joins and gradients over rows that an index sorts into groups (an addition of the C
+//!   library, beside its grouped plans).
 //! - [`preferred_compute_devices`] (tenferro-device/src/lib.rs:92-105) and [`check`], which turns a `tfh_status` into
 //!   the matching `tenferro_device::Error` variant (tenferro-device/src/lib.rs:108-159).
 //!
@@ -19,11 +21,13 @@ mod backend;
 mod buffer;
 mod einsum;
 mod event;
+mod rows;
 
 pub use backend::{HipBackend, HipGroupedPlan, HipPlan};
 pub use buffer::{HipBuffer, HipView, HipViewMut, PinnedBuffer};
 pub use einsum::{einsum_with_plan_into, ContractionTree, Subscripts};
 pub use event::{CompletionEvent, Stream};
+pub use rows::{AdapterFactors, RowGroups};
 
 use std::any::TypeId;
 use std::ffi::CStr;

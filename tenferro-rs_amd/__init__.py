@@ -22,7 +22,9 @@ LIB_PATH = os.path.join(_HERE, "libtenferro_hip.so")
 MAX_RANK = 16
 
 F32, F64, C64, C128 = 0, 1, 2, 3
-_NP_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float64): F64, np.dtype(np.complex64): C64, np.dtype(np.complex128): C128}
+BF16, F16 = 4, 5        # taken by the operations on rows in groups only
+_NP_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float64): F64, np.dtype(np.complex64): C64, np.dtype(np.complex128): C128,
+              np.dtype(np.float16): F16}
 _DT_NP = {v: k for k, v in _NP_DTYPES.items()}
 
 
@@ -122,6 +124,17 @@ def lib():
         L.tfh_subscripts_labels.argtypes = [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32]
         L.tfh_subscripts_nesting.argtypes = [C.c_void_p, C.c_char_p, C.c_size_t]
         L.tfh_plan_describe.argtypes = [C.c_void_p, C.c_char_p, C.c_size_t]
+        P, i32, i64, sz, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_double
+        L.tfh_group_rows_workspace.restype = L.tfh_adapter_workspace.restype = C.c_size_t
+        L.tfh_group_rows_workspace.argtypes = [i64, i32]
+        L.tfh_group_rows.argtypes = [i32, P, i32, P, P, P, P, sz, P]
+        L.tfh_ragged_gemm.argtypes = [i32, P, i32, f64, P, P, f64, P, P]
+        L.tfh_ragged_gemm_grad.argtypes = [i32, P, i32, f64, P, P, f64, P, P]
+        L.tfh_combine_rows.argtypes = [i32, P, P, P, P, P]
+        L.tfh_combine_rows_grad.argtypes = [i32, P, P, P, P, P, P, P]
+        L.tfh_adapter_workspace.argtypes = [i32, i64, i64, i32]
+        L.tfh_adapter_gemm.argtypes = [i32, P, P, P, P, P, P, P, P, sz, P]
+        L.tfh_adapter_gemm_grad.argtypes = [i32, P, P, P, P, P, P, P, P, P, P, P, sz, P]
         _lib = L
     return _lib
 
@@ -356,7 +369,8 @@ def dtype_code(dtype):
         return _NP_DTYPES[np.dtype(dtype)]
     except TypeError:
         import torch
-        return {torch.float32: F32, torch.float64: F64, torch.complex64: C64, torch.complex128: C128}[dtype]
+        return {torch.float32: F32, torch.float64: F64, torch.complex64: C64, torch.complex128: C128, torch.bfloat16: BF16,
+                torch.float16: F16}[dtype]
 
 
 def current_stream():
@@ -677,7 +691,8 @@ class Tensor:
             buf = np.zeros(n, _DT_NP[dt]) if fill is None else np.full(n, fill, _DT_NP[dt])
             return cls(buf, dims, _contig_strides(dims, order), 0, space, dt)
         import torch
-        tdt = {F32: torch.float32, F64: torch.float64, C64: torch.complex64, C128: torch.complex128}[dt]
+        tdt = {F32: torch.float32, F64: torch.float64, C64: torch.complex64, C128: torch.complex128, BF16: torch.bfloat16,
+               F16: torch.float16}[dt]
         buf = torch.empty(max(n, 1), dtype=tdt, device=f"cuda:{space.space_id}")
         t = cls(buf, dims, _contig_strides(dims, order), 0, space, dt)
         t._lib_alloc = True
@@ -929,7 +944,8 @@ class Tensor:
             lo = off + sum((d - 1) * s for d, s in zip(self._dims, self._strides) if s < 0 and d > 0)
             hi = off + sum((d - 1) * s for d, s in zip(self._dims, self._strides) if s > 0 and d > 0)
             span = 0 if 0 in self._dims else hi - lo + 1
-            flat = torch.as_strided(self._buf, (span,), (1,), self._buf.storage_offset() + lo).cpu().numpy()
+            flat = torch.as_strided(self._buf, (span,), (1,), self._buf.storage_offset() + lo).cpu()
+            flat = (flat.float() if flat.dtype == torch.bfloat16 else flat).numpy()    # numpy has no bfloat16
             off -= lo
         isz = flat.dtype.itemsize
         out = np.lib.stride_tricks.as_strided(flat[off:], self._dims, [s * isz for s in self._strides]).copy()
@@ -1115,3 +1131,9 @@ def profile_kernels(kind):
         if n.value == 0:
             return out
         out.append((buf.value.decode(), ms.value, n.value))
+
+
+# ---------------------------------------------------------------------------------------------- rows in groups
+from .row_groups import (RowGroups, adapter_gemm, adapter_gemm_backward, adapter_gemm_into, combine_rows,  # noqa: E402,F401
+                         combine_rows_backward, combine_rows_into, ragged_gemm, ragged_gemm_backward, ragged_gemm_grad_into,
+                         ragged_gemm_into)

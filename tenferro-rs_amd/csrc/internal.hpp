@@ -29,6 +29,8 @@ inline size_t dtype_size(int dt) {
         case TFH_F64: return 8;
         case TFH_C64: return 8;
         case TFH_C128: return 16;
+        case TFH_BF16:
+        case TFH_F16: return 2;
         default: return 0;
     }
 }

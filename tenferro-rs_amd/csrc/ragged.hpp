@@ -1,0 +1,456 @@
+// ragged.hpp -- products over rows in groups: the kernel that every type, layout and direction can take, and the
+// pieces it shares with the faster ones (k_ragged_*.hip instantiate it, ragged.cpp checks and dispatches).
+//
+//   rows    C[p, :] = alpha * sum_k A[src(p), k] * B[g(p), k, :] + beta * C[p, :]        for p in group g(p)
+//   outer   C[g, i, :] = alpha * sum_{p in g} A[src(p), i] * B[p, :] + beta * C[g, i, :]
+//   shared  C[t, :] = sum_k A[t, k] * B[k, :] + sum_j V[p, j] * E[g(p), j, :]            t = order[p], p = 0 .. n_rows
+//
+// with the groups' offsets, and the order that src() reads, in device memory: the host knows neither how many rows a
+// group has nor which, so a launch has as many blocks as the rows could need and each block finds its tile in the
+// offsets itself.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "gemm_common.hpp"
+
+namespace tfh {
+namespace ragged {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+
+// E: elements of a 16-byte chunk.  mma() multiplies one chunk of each operand per lane: lane l = 16 q + j holds row j and
+// the k's of its chunk; 16-bit types take the whole chunk in one instruction (k = 8 q + e), f32 and f64 in E of them,
+// instruction e taking the k's E q + e -- any assignment of k's to lanes is right that both operands share.
+// The first operand's row index becomes the accumulator's register index: row() of register r.
+template <class T> struct Num;
+template <> struct Num<__bf16> {
+    static constexpr int E = 8;
+    typedef float acc;   // what sums are held in
+    typedef f32x4 acc4;
+    __device__ static __forceinline__ acc4 mma(u32x4 a, u32x4 b, acc4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    __device__ static __forceinline__ int row(int q, int r) { return 4 * q + r; }
+};
+template <> struct Num<_Float16> {
+    static constexpr int E = 8;
+    typedef float acc;
+    typedef f32x4 acc4;
+    __device__ static __forceinline__ acc4 mma(u32x4 a, u32x4 b, acc4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    __device__ static __forceinline__ int row(int q, int r) { return 4 * q + r; }
+};
+template <> struct Num<float> {
+    static constexpr int E = 4;
+    typedef float acc;
+    typedef f32x4 acc4;
+    __device__ static __forceinline__ acc4 mma(u32x4 a, u32x4 b, acc4 c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+    __device__ static __forceinline__ int row(int q, int r) { return 4 * q + r; }
+};
+template <> struct Num<double> {
+    static constexpr int E = 2;
+    typedef double acc;
+    typedef f64x4 acc4;
+    __device__ static __forceinline__ acc4 mma(u32x4 a, u32x4 b, acc4 c) {
+        const f64x2 x = __builtin_bit_cast(f64x2, a), y = __builtin_bit_cast(f64x2, b);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+    __device__ static __forceinline__ int row(int q, int r) { return q + 4 * r; }
+};
+
+// The kernel's view of a call.  Strides in elements.  K, N: extents of the contracted axis and of C's columns (rows and
+// shared); outer: M and N are C[g]'s extents.
+struct Args {
+    const void* A;
+    const void* B;
+    void* C;
+    const int32_t* offsets;   // n_groups + 1
+    const int32_t* order;     // null: rows lie group by group
+    int64_t a_row, a_col;     // A[row, k] (rows, shared), A[row, i] (outer)
+    int64_t b_group, b_k, b_n;   // B[g, k, n]; outer: B[p, n] with b_k the row stride
+    int64_t b_rows;           // outer: rows that B has
+    int64_t c_group, c_row, c_n;
+    int64_t n_rows;           // rows in the order
+    int64_t a_rows;           // rows that A has: an index beyond them reads as zeros
+    int32_t n_groups, fan;
+    int32_t M, N, K;
+    int32_t gather;           // A's row of p is order[p] / fan, else p
+    int32_t scatter;          // C's row of p is order[p], else p
+    int32_t zero_rest;        // rows: the rows behind the last group are written as zeros, else left alone
+    int32_t use_beta;
+    double alpha, beta;
+    int32_t gather_b;         // outer: B's row of p is order[p], else p
+    // shared: the low-rank part, V[p, 0 .. r) (of the accumulators' type) against E[g, j, n]; rows of no group are without it
+    const void* V;
+    const void* E;
+    int64_t v_row, e_group, e_k, e_n;
+    int32_t r;
+    const void* scales;       // rows: factors of the groups' results (of the accumulators' type) beside alpha, or null
+};
+
+enum Mode { ROWS = 0, OUTER = 1, SHARED = 2 };
+
+// E elements of type C from a row of S that starts at any element: `count` of them are there, the others read as zeros.
+template <class S, class C>
+__device__ __forceinline__ u32x4 load_chunk(const S* p, int64_t stride, int count) {
+    constexpr int E = Num<C>::E;
+    u32x4 v = {0, 0, 0, 0};
+    if (count >= E && stride == 1) {
+        if constexpr (sizeof(S) == sizeof(C)) {
+            __builtin_memcpy(&v, p, 16);
+        } else {
+            S s[E];
+            C c[E];
+            __builtin_memcpy(s, p, E * sizeof(S));
+#pragma unroll
+            for (int i = 0; i < E; ++i) c[i] = (C)s[i];
+            __builtin_memcpy(&v, c, 16);
+        }
+    } else if (count > 0) {
+        C c[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) c[i] = i < count ? (C)p[i * stride] : (C)0;
+        __builtin_memcpy(&v, c, 16);
+    }
+    return v;
+}
+
+// ---- tiles in LDS -------------------------------------------------------------------------------------------------
+// An operand's tile is 128 bytes of k by TM rows.  k-fast: [row][8 chunks], the chunk index XORed with the row so that
+// the 16 rows of a fragment read spread over the banks.  row-fast: [k][TM elements], whose 16-bit fragments are read by
+// the transposing LDS load (four rows of k by 16 columns, 8 bytes a lane); the XOR there moves the 32-byte pieces that
+// the rows of one instruction touch to different banks.
+template <class T> __device__ __forceinline__ uint32_t kfast_at(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+template <class T> __device__ __forceinline__ uint32_t rowfast_swizzle(uint32_t k) {
+    if constexpr (sizeof(T) == 2) return ((k & 3) | (((k >> 3) & 1) << 2)) << 1;
+    else if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+    else return 0;
+}
+template <class T, int TM> __device__ __forceinline__ uint32_t rowfast_at(uint32_t k, uint32_t chunk) {
+    constexpr uint32_t chunks = TM * (uint32_t)sizeof(T) / 16;   // of a row; a narrow tile uses fewer bits of the XOR
+    return k * (TM * (uint32_t)sizeof(T)) + ((chunk ^ (rowfast_swizzle<T>(k) & (chunks - 1))) << 4);
+}
+// The chunk (h = 0, 1: which half of the 128 bytes of k) of 16 rows from `row`, as mma() takes it.
+template <class T, int TM, bool KFAST>
+__device__ __forceinline__ u32x4 fragment(const char* tile, int row, int h, int lane) {
+    const int q = lane >> 4, j = lane & 15;
+    if constexpr (KFAST) {
+        return *(const u32x4*)(tile + kfast_at<T>(row + j, q + 4 * h));
+    } else if constexpr (sizeof(T) == 2) {
+        typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+        const int k = (q + 4 * h) * 8 + (j >> 2), col = row + 4 * (j & 3);
+        const uint32_t within = (col * 2) & 15, chunk = (col * 2) >> 4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + rowfast_at<T, TM>(k, chunk) + within));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + rowfast_at<T, TM>(k + 4, chunk) + within));
+        struct { s16x4 a, b; } both = {lo, hi};
+        return __builtin_bit_cast(u32x4, both);
+    } else {
+        constexpr int E = Num<T>::E;
+        T e[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const uint32_t k = (q + 4 * h) * E + i, at = (row + j) * (uint32_t)sizeof(T);
+            e[i] = *(const T*)(tile + rowfast_at<T, TM>(k, at >> 4) + (at & 15));
+        }
+        u32x4 v;
+        __builtin_memcpy(&v, e, 16);
+        return v;
+    }
+}
+
+// ---- which tile a block works on --------------------------------------------------------------------------------------
+__device__ __forceinline__ int clamp_row(int32_t o, int64_t n_rows) { return o < 0 ? 0 : o > n_rows ? (int)n_rows : o; }
+struct Tile {
+    int group;   // n_groups: the rows behind the last group
+    int first, rows, tile_m, tile_n;
+};
+// Tiles are dealt group by group; inside a group as tile_of() walks a matrix.  Every wave does this for itself: the
+// lanes take 64 groups at a time.  Returns false when the block has none.
+__device__ __forceinline__ bool find_tile(const Args& a, int tm, int tiles_n, uint32_t block, Tile& t) {
+    const int lane = threadIdx.x & 63;
+    const int groups = a.n_groups + (a.zero_rest ? 1 : 0);
+    auto rows_of = [&](int g) {
+        if (g >= groups) return 0;
+        const int from = clamp_row(a.offsets[g], a.n_rows);
+        const int to = g < a.n_groups ? clamp_row(a.offsets[g + 1], a.n_rows) : (int)a.n_rows;
+        return to > from ? to - from : 0;
+    };
+    uint64_t total = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) total += (uint32_t)((rows_of(g0 + lane) + tm - 1) / tm);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
+    total *= tiles_n;
+    if (block >= total) return false;
+    // every XCD walks one contiguous range of the tiles
+    uint64_t want = gemm::logical_block(block, total);
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int rows = rows_of(g0 + lane);
+        const uint64_t mine = (uint64_t)((rows + tm - 1) / tm) * tiles_n;
+        uint64_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+        const uint64_t here = __shfl(upto, 63, 64);
+        if (want < here) {
+            const int at = __builtin_ctzll(__ballot(want < upto));
+            const uint32_t rest = (uint32_t)(want - __shfl(upto - mine, at, 64));
+            t.group = __builtin_amdgcn_readfirstlane(g0 + at);
+            const int rows_g = __builtin_amdgcn_readfirstlane(__shfl(rows, at, 64));
+            gemm::tile_of(__builtin_amdgcn_readfirstlane(rest), (rows_g + tm - 1) / tm, tiles_n, t.tile_m, t.tile_n);
+            t.first = clamp_row(a.offsets[t.group], a.n_rows) + t.tile_m * tm;
+            t.rows = rows_g - t.tile_m * tm < tm ? rows_g - t.tile_m * tm : tm;
+            return true;
+        }
+        want -= here;
+    }
+    return false;
+}
+// The group that holds row p (clamped offsets ascending), n_groups for the rows behind the last one.
+__device__ __forceinline__ int group_of(const Args& a, int p) {
+    int lo = 0, hi = a.n_groups;   // the first group that ends behind p
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.offsets[mid + 1] > p) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+// The row of A that row p of the order reads; -1: none (the order names a row that is not there).
+__device__ __forceinline__ int64_t source_row(const Args& a, int p) {
+    int64_t s = p;
+    if (a.gather && a.order) {
+        const int o = a.order[p];
+        s = o < 0 ? -1 : o / a.fan;
+    }
+    return s < a.a_rows ? s : -1;
+}
+
+// ---- the kernel for every type, layout and direction ------------------------------------------------------------------
+// Tiles of 32 XT x 32 YT, four waves, operands through registers into a double-buffered LDS tile (the loads of the next
+// 128 bytes of k are in flight while the present ones are multiplied).
+constexpr int GENERAL_THREADS = 256;
+
+// One stage (128 bytes of k of type C) of a wave's 16 XT x 16 YT results.  Where not all rows take part, those in
+// [from, to) of the tile take the products and the others keep what they have: a row that is not a group's must not see
+// 0 * infinity from that group's factors.
+template <class C, bool AKFAST, bool BKFAST, int XT, int YT, bool ALL>
+__device__ __forceinline__ void multiply_stage(typename Num<C>::acc4 (&acc)[XT][YT], const char* stage, int wm, int wn, int lane, int from, int to) {
+    constexpr int TM = 32 * XT, TN = 32 * YT;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        u32x4 fa[XT], fb[YT];
+#pragma unroll
+        for (int x = 0; x < XT; ++x) fa[x] = fragment<C, TM, AKFAST>(stage, (wm * XT + x) * 16, h, lane);
+#pragma unroll
+        for (int y = 0; y < YT; ++y) fb[y] = fragment<C, TN, BKFAST>(stage + TM * 128, (wn * YT + y) * 16, h, lane);
+#pragma unroll
+        for (int x = 0; x < XT; ++x) {
+            const int r = (wm * XT + x) * 16 + (lane & 15);
+            const bool mine = ALL || (r >= from && r < to);
+#pragma unroll
+            for (int y = 0; y < YT; ++y) {
+                const typename Num<C>::acc4 v = Num<C>::mma(fb[y], fa[x], acc[x][y]);
+                if constexpr (ALL) acc[x][y] = v;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[x][y][i] = mine ? v[i] : acc[x][y][i];
+            }
+        }
+    }
+}
+// A whole k loop: load(i, k0, ra, rb) fetches a stage's chunks.
+template <class C, bool AKFAST, bool BKFAST, int XT, int YT, bool ALL, class Load>
+__device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], char* lds, int kend, int wm, int wn, int lane, int from, int to, Load load) {
+    constexpr int TM = 32 * XT, TN = 32 * YT, BK = 128 / (int)sizeof(C);
+    constexpr int RA = TM * (int)sizeof(C) / 16, RB = TN * (int)sizeof(C) / 16;   // chunks of a row of k in a row-fast tile
+    const int tid = threadIdx.x, cc = tid & 7, cr = tid >> 3;
+    u32x4 ra[XT], rb[YT];
+    auto store_stage = [&](char* stage) {
+#pragma unroll
+        for (int i = 0; i < XT; ++i) {
+            const int id = tid + GENERAL_THREADS * i;
+            if constexpr (AKFAST) *(u32x4*)(stage + kfast_at<C>(cr + 32 * i, cc)) = ra[i];
+            else *(u32x4*)(stage + rowfast_at<C, TM>(id / RA, id % RA)) = ra[i];
+        }
+#pragma unroll
+        for (int i = 0; i < YT; ++i) {
+            const int id = tid + GENERAL_THREADS * i;
+            if constexpr (BKFAST) *(u32x4*)(stage + TM * 128 + kfast_at<C>(cr + 32 * i, cc)) = rb[i];
+            else *(u32x4*)(stage + TM * 128 + rowfast_at<C, TN>(id / RB, id % RB)) = rb[i];
+        }
+    };
+    if (kend <= 0) return;
+    __syncthreads();
+    load(0, ra, rb);
+    store_stage(lds);
+    __syncthreads();
+    int at = 0;
+    for (int k0 = 0; k0 < kend; k0 += BK) {
+        const bool more = k0 + BK < kend;
+        if (more) load(k0 + BK, ra, rb);
+        multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds + at, wm, wn, lane, from, to);
+        at ^= (TM + TN) * 128;
+        if (more) store_stage(lds + at);
+        __syncthreads();
+    }
+}
+
+// TA, TB: the operands' types; C: the type multiplied in (theirs, or that of the sums); TO: the result's.
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, int XT, int YT>
+__global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(const Args a) {
+    typedef Num<C> NT;
+    typedef typename NT::acc W;
+    constexpr int E = NT::E, TM = 32 * XT, TN = 32 * YT;
+    constexpr bool AKFAST = MODE != OUTER;
+    __shared__ __align__(16) char lds[2 * (TM + TN) * 128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1, q = lane >> 4, j = lane & 15;
+    const int tiles_n = (a.N + TN - 1) / TN;
+    Tile t;
+    if constexpr (MODE == ROWS) {
+        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+    } else if constexpr (MODE == OUTER) {
+        const int tiles_m = (a.M + TM - 1) / TM;
+        const uint64_t id = gemm::logical_block(blockIdx.x, gridDim.x);
+        t.group = (int)(id / ((uint64_t)tiles_m * tiles_n));
+        gemm::tile_of((uint32_t)(id % ((uint64_t)tiles_m * tiles_n)), tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.first = clamp_row(a.offsets[t.group], a.n_rows);
+        const int to = clamp_row(a.offsets[t.group + 1], a.n_rows);
+        t.rows = to > t.first ? to - t.first : 0;
+    } else {
+        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
+        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.group = 0;
+        t.first = t.tile_m * TM;
+        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
+    }
+    const bool real = MODE != ROWS || t.group < a.n_groups;   // the rows behind the last group have nothing to multiply
+    const int n0 = t.tile_n * TN, m0 = t.tile_m * TM;
+    typename NT::acc4 acc[XT][YT];
+#pragma unroll
+    for (int x = 0; x < XT; ++x)
+#pragma unroll
+        for (int y = 0; y < YT; ++y) acc[x][y] = (typename NT::acc4){0, 0, 0, 0};
+
+    // This thread's chunks of a stage.  k-fast: chunk tid % 8 of rows tid / 8 + 32 i; row-fast: chunks tid + 256 i of [k][row].
+    const int cc = tid & 7, cr = tid >> 3;
+
+    if constexpr (MODE == SHARED) {
+        constexpr int EW = Num<W>::E, RW = TN * (int)sizeof(W) / 16;
+        const int last = t.first + t.rows - 1;
+        for (int g = group_of(a, t.first); g < a.n_groups; ++g) {
+            const int from = clamp_row(a.offsets[g], a.n_rows), to = clamp_row(a.offsets[g + 1], a.n_rows);
+            if (from > last) break;
+            if (to <= from) continue;
+            const TB* const Eg = (const TB*)a.E + g * a.e_group;
+            auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+#pragma unroll
+                for (int i = 0; i < XT; ++i) {
+                    const int k = k0 + cc * EW, r = cr + 32 * i;
+                    ra[i] = load_chunk<W, W>((const W*)a.V + (int64_t)(t.first + r) * a.v_row + k, 1, r < t.rows ? a.r - k : 0);
+                }
+#pragma unroll
+                for (int i = 0; i < YT; ++i) {
+                    const int id = tid + GENERAL_THREADS * i;
+                    if constexpr (BKFAST) {
+                        const int k = k0 + cc * EW, n = n0 + cr + 32 * i;
+                        rb[i] = load_chunk<TB, W>(Eg + n * a.e_n + k * a.e_k, a.e_k, n < a.N ? a.r - k : 0);
+                    } else {
+                        const int k = k0 + id / RW, n = n0 + (id % RW) * EW;
+                        rb[i] = load_chunk<TB, W>(Eg + k * a.e_k + n * a.e_n, a.e_n, k < a.r ? a.N - n : 0);
+                    }
+                }
+            };
+            k_loop<W, true, BKFAST, XT, YT, false>(acc, lds, a.r, wm, wn, lane, from - t.first, to - t.first, load);
+        }
+    }
+
+    const TA* const A = (const TA*)a.A;
+    int64_t arow[XT];   // k-fast A: the source rows of this thread's chunks (-1: none)
+    if constexpr (AKFAST) {
+#pragma unroll
+        for (int i = 0; i < XT; ++i) arow[i] = cr + 32 * i < t.rows && real ? source_row(a, t.first + cr + 32 * i) : -1;
+    }
+    const TB* const B = (const TB*)a.B + (MODE == ROWS && real ? t.group * a.b_group : 0);
+    const int kend = MODE == OUTER ? t.rows : real ? a.K : 0;
+    constexpr int RA = TM * (int)sizeof(C) / 16, RB = TN * (int)sizeof(C) / 16;
+    auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+#pragma unroll
+        for (int i = 0; i < XT; ++i) {
+            const int id = tid + GENERAL_THREADS * i;
+            if constexpr (AKFAST) {
+                const int k = k0 + cc * E;
+                ra[i] = load_chunk<TA, C>(A + arow[i] * a.a_row + k * a.a_col, a.a_col, arow[i] >= 0 ? kend - k : 0);
+            } else {
+                const int k = k0 + id / RA, m = m0 + (id % RA) * E;
+                const int64_t s = k < kend ? source_row(a, t.first + k) : -1;
+                ra[i] = load_chunk<TA, C>(A + s * a.a_row + m * a.a_col, a.a_col, s >= 0 ? a.M - m : 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < YT; ++i) {
+            const int id = tid + GENERAL_THREADS * i;
+            if constexpr (BKFAST) {
+                const int k = k0 + cc * E, n = n0 + cr + 32 * i;
+                rb[i] = load_chunk<TB, C>(B + n * a.b_n + k * a.b_k, a.b_k, n < a.N ? kend - k : 0);
+            } else {
+                const int k = k0 + id / RB, n = n0 + (id % RB) * E;
+                int64_t s = k;
+                if constexpr (MODE == OUTER) {
+                    s = -1;
+                    if (k < kend) s = a.gather_b && a.order ? a.order[t.first + k] : t.first + k;
+                    if (s >= a.b_rows) s = -1;
+                }
+                rb[i] = load_chunk<TB, C>(B + s * a.b_k + n * a.b_n, a.b_n, k < kend && s >= 0 ? a.N - n : 0);
+            }
+        }
+    };
+    k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load);
+
+    W alpha = (W)a.alpha;
+    const W beta = (W)a.beta;
+    if constexpr (MODE == ROWS)
+        if (a.scales && real) alpha *= ((const W*)a.scales)[t.group];
+#pragma unroll
+    for (int x = 0; x < XT; ++x) {
+        const int r = (wm * XT + x) * 16 + j;
+        if (MODE == OUTER ? m0 + r >= a.M : r >= t.rows) continue;
+        int64_t row = MODE == OUTER ? m0 + r : t.first + r;
+        if constexpr (MODE != OUTER)
+            if (a.scatter && a.order) {
+                row = a.order[row];
+                if (row < 0 || row >= a.n_rows) continue;
+            }
+        TO* const c = (TO*)a.C + (MODE == OUTER ? t.group * a.c_group : 0) + row * a.c_row;
+#pragma unroll
+        for (int y = 0; y < YT; ++y)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = n0 + (wn * YT + y) * 16 + NT::row(q, i);
+                if (n >= a.N) continue;
+                W v = real ? alpha * acc[x][y][i] : (W)0;
+                if (a.use_beta && real) v += beta * (W)c[n * a.c_n];
+                c[n * a.c_n] = (TO)v;
+            }
+    }
+}
+
+}  // namespace ragged
+}  // namespace tfh

@@ -1,0 +1,62 @@
+// ragged_api.hpp -- what ragged.cpp (argument checks, dispatch) and the kernels on rows in groups agree on.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#include "internal.hpp"
+
+namespace tfh {
+namespace ragged {
+
+// Rows by group (k_row_groups.hip).
+struct GroupArgs {
+    const void* ids;          // element of row i: (i / inner) * s_outer + (i % inner) * s_inner
+    int64_t s_outer, s_inner;
+    int32_t inner, id64;
+    int32_t n_rows, n_groups;
+    int32_t* offsets;
+    int32_t* order;
+    int32_t* positions;       // may be null
+    int32_t* counts;          // [n_groups + 1][blocks] in the workspace (more than one block)
+    int32_t blocks;
+};
+size_t group_rows_workspace(int64_t n_rows, int32_t n_groups);
+int32_t launch_group_rows(GroupArgs a, void* stream);
+
+// A token's rows joined (k_combine.hip).  Strides in elements.
+struct CombineArgs {
+    const void* x;            // [n_rows, n] rows in order
+    int64_t x_row, x_n;
+    const void* w;            // [tokens, fan], of the sums' type, or null (ones)
+    int64_t w_token, w_fan;
+    void* y;                  // [tokens, n]; the gradient's: dy
+    int64_t y_row, y_n;
+    void* dx;                 // the gradient's [n_rows, n], may be null
+    int64_t dx_row, dx_n;
+    void* dw;                 // the gradient's [tokens, fan], may be null
+    int64_t dw_token, dw_fan;
+    const int32_t* positions;
+    const int32_t* offsets;
+    int64_t n_rows, tokens;
+    int32_t n_groups, fan, n;
+};
+int32_t launch_combine(int dtype, const CombineArgs& a, void* stream);
+int32_t launch_combine_grad(int dtype, const CombineArgs& a, void* stream);
+
+// Products (k_ragged_*.hip): one entry per operand type, which chooses among its kernels.
+struct Args;
+enum Kind {
+    PRODUCT_ROWS,      // rows in, rows out, all of the type
+    PRODUCT_OUTER,     // a group's rows summed over, all of the type
+    PRODUCT_SHARED,    // one matrix for all rows and a low-rank part by group
+    PRODUCT_MIDDLE,    // rows in, rows out in the sums' type
+    PRODUCT_OUTER_V,   // A of the type, B of the sums' type
+    PRODUCT_V_OUTER    // A of the sums' type, B of the type
+};
+int32_t launch_bf16(int kind, const Args& a, void* stream);
+int32_t launch_f16(int kind, const Args& a, void* stream);
+int32_t launch_f32(int kind, const Args& a, void* stream);
+int32_t launch_f64(int kind, const Args& a, void* stream);
+
+}  // namespace ragged
+}  // namespace tfh

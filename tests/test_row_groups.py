@@ -1,0 +1,736 @@
+"""Rows in groups (tfh_group_rows, tfh_ragged_gemm*, tfh_combine_rows*, tfh_adapter_gemm*): against plain loops in 64 bits
+on the CPU, at the sizes, layouts and groups where such kernels go wrong, and what the entry points refuse.
+
+Tolerances, element by element, from arithmetic alone: a result is rounded once (half a step of its type relative to it, or
+half the smallest step of f16 where that is larger), and a sum of k products held in f32 (f64) is off by at most
+2 (k + 4) u times the sum of the products' absolute values, u = 2^-24 (2^-53).  The adapters' middle X A is kept to at
+least 16 bits (half a step 2^-17) beside 16-bit operands."""
+import ctypes as C
+import itertools
+import os
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def tf():
+    import tenferro_rs_amd as tf
+    tf.lib()
+    return tf
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    return torch
+
+
+TYPES = ["bfloat16", "float16", "float32", "float64"]
+HALF_STEP = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11, "float32": 2.0 ** -24, "float64": 2.0 ** -53}
+U = {"bfloat16": 2.0 ** -24, "float16": 2.0 ** -24, "float32": 2.0 ** -24, "float64": 2.0 ** -53}
+SMALLEST = {"bfloat16": 2.0 ** -134, "float16": 2.0 ** -25, "float32": 2.0 ** -150, "float64": 0.0}
+MIDDLE = {"bfloat16": 2.0 ** -17, "float16": 2.0 ** -17, "float32": 0.0, "float64": 0.0}
+
+
+def close(got, want, size, k, name, extra=0.0):
+    """`size`: the sum of the products' absolute values; `extra`: further absolute slack, derived by the caller."""
+    got, want = got.double().cpu(), want.double().cpu()
+    assert got.shape == want.shape
+    bound = HALF_STEP[name] * (1 + 2 ** -6) * want.abs() + SMALLEST[name] + 2 * (k + 4) * U[name] * size.double().cpu() + extra
+    off = (got - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), (name, int(bad.sum()), off[bad][:4].tolist(), bound[bad][:4].tolist(), bad.nonzero()[:4].tolist())
+
+
+def grouping(ids, n):
+    """offsets, order, positions of a flat list of indices, in plain Python."""
+    ids = [int(i) for i in ids]
+    order = [i for g in range(n) for i, x in enumerate(ids) if x == g]
+    grouped = len(order)
+    order += [i for i, x in enumerate(ids) if not 0 <= x < n]
+    offsets = [0]
+    for g in range(n):
+        offsets.append(offsets[-1] + sum(1 for x in ids if x == g))
+    positions = [-1] * len(ids)
+    for p in range(grouped):
+        positions[order[p]] = p
+    return offsets, order, positions
+
+
+def choices(rng, tokens, fan, groups, none=0.15, only=None):
+    """Distinct choices for each token; `only`: groups that are chosen at all (the others stay empty)."""
+    pool = np.arange(groups) if only is None else np.asarray(only)
+    ids = np.stack([rng.permutation(pool)[:fan] if len(pool) >= fan else rng.choice(pool, fan) for _ in range(tokens)]) if tokens else np.zeros((0, fan), int)
+    ids = np.where(rng.random(ids.shape) < none, rng.choice([-1, groups, groups + 7, -5], ids.shape), ids)
+    return ids
+
+
+def made(tf, torch, ids, groups):
+    return tf.RowGroups.from_ids(torch.from_numpy(np.ascontiguousarray(ids)).cuda(), groups)
+
+
+def tensor(torch, rng, shape, name, scale=1.0):
+    return torch.from_numpy(rng.standard_normal(shape) * scale).to(getattr(torch, name))
+
+
+def layout(torch, t, how):
+    """The same values on the GPU with other strides."""
+    t = t.cuda()
+    if how == "columns":        # the last axis contiguous
+        return t.contiguous()
+    if how == "rows":           # the last but one contiguous
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    if how == "pitch":          # rows further apart than they are long, and an odd start
+        big = torch.zeros(*t.shape[:-2], t.shape[-2] + 1, t.shape[-1] + 3, dtype=t.dtype, device="cuda")
+        view = big[..., 1:, 1:t.shape[-1] + 1]
+        view.copy_(t)
+        return view
+    if how == "steps":          # every second element of both axes
+        big = torch.zeros(*t.shape[:-2], 2 * t.shape[-2], 2 * t.shape[-1], dtype=t.dtype, device="cuda")
+        view = big[..., ::2, ::2]
+        view.copy_(t)
+        return view
+    raise ValueError(how)
+
+
+# ------------------------------------------------------------------------------------------------------ grouping
+GROUPINGS = [(0, 1, 3), (1, 1, 1), (1, 8, 9), (5, 1, 2048), (63, 1, 2), (64, 3, 3), (257, 4, 65), (1000, 2, 7), (1024, 8, 128),
+             (2731, 3, 512), (8192, 1, 2), (8193, 1, 2), (5000, 8, 64), (70001, 2, 2047)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,fan,groups", GROUPINGS)
+@pytest.mark.parametrize("bits", [32, 64])
+def test_grouping_is_the_stable_one(tf, torch, tokens, fan, groups, bits):
+    rng = np.random.default_rng(tokens + groups)
+    ids = rng.integers(-1, groups + 1, (tokens, fan)).astype(np.int32 if bits == 32 else np.int64)
+    g = made(tf, torch, ids, groups)
+    key = np.where((ids >= 0) & (ids < groups), ids, groups).reshape(-1)
+    order = np.argsort(key, kind="stable")
+    offsets = np.searchsorted(key[order], np.arange(groups + 1))
+    positions = np.empty(len(key), int)
+    positions[order] = np.arange(len(key))
+    positions[key == groups] = -1
+    assert g.n_rows == tokens * fan and g.n_groups == groups and (g.fan == fan)
+    assert g.offsets.cpu().numpy().tolist() == offsets.tolist()
+    assert np.array_equal(g.order.cpu().numpy(), order)
+    assert np.array_equal(g.positions.cpu().numpy(), positions)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["all one", "all none", "last only", "huge 64-bit"])
+def test_grouping_of_extreme_indices(tf, torch, how):
+    n, groups = 9000, 33
+    ids = np.zeros(n, np.int64)
+    if how == "all none":
+        ids[:] = -1
+    elif how == "last only":
+        ids[:] = groups - 1
+    elif how == "huge 64-bit":       # their low halves are valid indices
+        ids[:] = np.where(np.arange(n) % 2 == 0, (1 << 32) + 5, -(1 << 40) + 3)
+    g = made(tf, torch, ids, groups)
+    offsets, order, positions = grouping(ids, groups)
+    assert g.offsets.tolist() == offsets and g.order.tolist() == order and g.positions.tolist() == positions
+
+
+@pytest.mark.gpu
+def test_grouping_reads_strided_indices(tf, torch):
+    rng = np.random.default_rng(3)
+    base = torch.from_numpy(rng.integers(0, 6, (40, 10))).cuda()
+    for view in (base[:, 2:5], base.t()[1:4].t(), base[::3, ::4], base[:, 7], base[5], base[3:4, 1:8:2], base[:, 1:2], base[:1, 4:5].expand(9, 3)):
+        g = tf.RowGroups.from_ids(view, 6)
+        offsets, order, positions = grouping(view.reshape(-1).cpu().numpy(), 6)
+        assert g.offsets.tolist() == offsets and g.order.tolist() == order and g.positions.tolist() == positions
+
+
+# ------------------------------------------------------------------------------------------------------ products
+def ragged_reference(torch, a, b, offsets, order, fan, gather):
+    """c and the sums of absolute values, zeros for rows of no group."""
+    n = len(order)
+    a, b = a.double(), b.double()
+    c, size = torch.zeros(n, b.shape[2], dtype=torch.float64), torch.zeros(n, b.shape[2], dtype=torch.float64)
+    for g in range(len(offsets) - 1):
+        for p in range(offsets[g], offsets[g + 1]):
+            row = a[order[p] // fan if gather else p]
+            c[p], size[p] = row @ b[g], row.abs() @ b[g].abs()
+    return c, size
+
+
+SHAPES = [  # tokens, fan, groups, K, N
+    (1, 1, 1, 1, 1), (1, 2, 3, 8, 16), (7, 1, 5, 33, 5), (16, 4, 8, 64, 64), (40, 2, 3, 129, 65), (130, 3, 4, 72, 200), (300, 1, 2, 256, 136),
+    (65, 2, 70, 40, 24), (3, 2, 2, 520, 264), (200, 2, 3, 1000, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("how", ["columns", "rows"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_ragged_product(tf, torch, name, shape, how, gather):
+    tokens, fan, groups, K, N = shape
+    rng = np.random.default_rng(tokens * 7 + K)
+    ids = choices(rng, tokens, min(fan, groups), groups)
+    fan = ids.shape[1]
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    a = tensor(torch, rng, (tokens if gather else tokens * fan, K), name)
+    b = tensor(torch, rng, (groups, K, N), name, K ** -0.5)
+    want, size = ragged_reference(torch, a, b, offsets, order, fan, gather)
+    got = tf.ragged_gemm(a.cuda(), layout(torch, b, how), made(tf, torch, ids, groups), gather=gather)
+    close(got, want, size, K, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16", "float64"])
+@pytest.mark.parametrize("how_a,how_b,how_c", [("pitch", "pitch", "pitch"), ("rows", "steps", "columns"), ("steps", "columns", "rows"), ("columns", "rows", "steps")])
+def test_ragged_product_into_strided_views(tf, torch, name, how_a, how_b, how_c):
+    rng = np.random.default_rng(11)
+    tokens, fan, groups, K, N = 90, 2, 5, 88, 72
+    ids = choices(rng, tokens, fan, groups, only=[0, 3])           # three groups are empty
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    a, b, c = (tensor(torch, rng, s, name) for s in ((tokens, K), (groups, K, N), (tokens * fan, N)))
+    want, size = ragged_reference(torch, a, b, offsets, order, fan, True)
+    grouped = offsets[-1]
+    want = 0.5 * want - 1.5 * c.double()
+    want[grouped:] = c.double()[grouped:]
+    size = 0.5 * size + 1.5 * c.double().abs()
+    out = layout(torch, c, how_c)
+    tf.ragged_gemm_into(layout(torch, a, how_a), layout(torch, b, how_b), made(tf, torch, ids, groups), 0.5, -1.5, out, gather=True)
+    close(out, want, size, K, name)
+    assert torch.equal(out.cpu()[grouped:], c[grouped:])           # rows of no group stay as they were
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+def test_ragged_product_scatters_and_overwrites_what_is_no_number(tf, torch, name):
+    rng = np.random.default_rng(5)
+    tokens, fan, groups, K, N = 50, 3, 4, 64, 40
+    ids = choices(rng, tokens, fan, groups)
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    a, b = tensor(torch, rng, (tokens * fan, K), name), tensor(torch, rng, (groups, K, N), name)
+    want, size = ragged_reference(torch, a, b, offsets, order, fan, False)
+    out = torch.full((tokens * fan, N), float("nan"), dtype=a.dtype, device="cuda")
+    tf.ragged_gemm_into(a.cuda(), b.cuda(), made(tf, torch, ids, groups), 1.0, 0.0, out, scatter=True)
+    kept = torch.tensor(order[:offsets[-1]])
+    close(out.cpu()[kept], want[:offsets[-1]], size[:offsets[-1]], K, name)
+    assert out.cpu()[torch.tensor(order[offsets[-1]:], dtype=torch.long)].isnan().all()
+
+
+@pytest.mark.gpu
+def test_ragged_product_without_rows_groups_or_k(tf, torch):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    g = tf.RowGroups.from_ids(torch.zeros(0, dtype=torch.int32, device="cuda"), 4)
+    assert g.offsets.tolist() == [0] * 5
+    assert tf.ragged_gemm(z(0, 8), z(4, 8, 6), g).shape == (0, 6)
+    da, db = tf.ragged_gemm_backward(z(0, 8), torch.ones(4, 8, 6, dtype=torch.bfloat16, device="cuda"), z(0, 6), g)
+    assert da.shape == (0, 8) and db.shape == (4, 8, 6) and not db.any()
+    g = tf.RowGroups.from_ids(torch.tensor([1, -1, 0], device="cuda"), 2)
+    out = tf.ragged_gemm(z(3, 0), z(2, 0, 5), g)                    # nothing to sum: zeros
+    assert out.shape == (3, 5) and not out.any()
+    assert tf.ragged_gemm(z(3, 4), z(2, 4, 0), g).shape == (3, 0)
+    none = tf.RowGroups.from_ids(torch.full((3,), -1, device="cuda"), 2)
+    out = tf.ragged_gemm(torch.ones(3, 4, dtype=torch.bfloat16, device="cuda"), torch.ones(2, 4, 5, dtype=torch.bfloat16, device="cuda"), none)
+    assert not out.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float32"])
+def test_ragged_product_keeps_infinities_to_their_groups_and_rows(tf, torch, name):
+    rng = np.random.default_rng(8)
+    ids = np.array([0, 1, 1, 2, 2, 2, -1, 0])
+    a, b = tensor(torch, rng, (8, 48), name), tensor(torch, rng, (3, 48, 32), name)
+    clean = tf.ragged_gemm(a.cuda(), b.cuda(), made(tf, torch, ids, 3), gather=True).cpu()
+    b[1] = float("inf")
+    a[6] = float("nan")                                           # the row of no group
+    a[0, 3] = float("nan")
+    got = tf.ragged_gemm(a.cuda(), b.cuda(), made(tf, torch, ids, 3), gather=True).cpu()
+    assert got[0].isnan().all() and torch.equal(got[1], clean[1]) and torch.equal(got[4:7], clean[4:7])
+    assert not got[2:4].isfinite().any() and not got[7].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("how", ["columns", "rows"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_ragged_gradients(tf, torch, name, shape, how, gather):
+    tokens, fan, groups, K, N = shape
+    rng = np.random.default_rng(tokens * 5 + N)
+    ids = choices(rng, tokens, min(fan, groups), groups)
+    fan = ids.shape[1]
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    a = tensor(torch, rng, (tokens if gather else tokens * fan, K), name)
+    b, dc = tensor(torch, rng, (groups, K, N), name, K ** -0.5), tensor(torch, rng, (tokens * fan, N), name)
+    da, db = tf.ragged_gemm_backward(a.cuda(), layout(torch, b, how), dc.cuda(), made(tf, torch, ids, groups), gather=gather)
+    A, B, D = a.double(), b.double(), dc.double()
+    want_a, size_a = torch.zeros(A.shape, dtype=torch.float64), torch.zeros(A.shape, dtype=torch.float64)
+    parts = torch.zeros(A.shape, dtype=torch.float64)               # the parts that are rounded before they are added up
+    want_b, size_b = torch.zeros(B.shape, dtype=torch.float64), torch.zeros(B.shape, dtype=torch.float64)
+    for g in range(groups):
+        for p in range(offsets[g], offsets[g + 1]):
+            s = order[p] // fan if gather else p
+            part = D[p] @ B[g].t()
+            want_a[s] += part
+            parts[s] += part.abs()
+            size_a[s] += D[p].abs() @ B[g].abs().t()
+            want_b[g] += torch.outer(A[s], D[p])
+            size_b[g] += torch.outer(A[s], D[p]).abs()
+    extra = HALF_STEP[name] * (1 + 2 ** -6) * parts + fan * SMALLEST[name] if gather and fan > 1 else 0.0
+    close(da, want_a, size_a, N + fan, name, extra)
+    close(db, want_b, size_b, max(offsets[g + 1] - offsets[g] for g in range(groups)), name)
+
+
+@pytest.mark.gpu
+def test_ragged_weight_gradient_adds_to_what_is_there(tf, torch):
+    rng = np.random.default_rng(2)
+    ids = choices(rng, 60, 1, 4, only=[0, 2])[:, 0]
+    offsets, order, _ = grouping(ids, 4)
+    a, dc, db = tensor(torch, rng, (60, 24), "float32"), tensor(torch, rng, (60, 36), "float32"), tensor(torch, rng, (4, 24, 36), "float32")
+    want, size = 2.0 * db.double(), 2.0 * db.double().abs()
+    for g in range(4):
+        rows = torch.tensor(order[offsets[g]:offsets[g + 1]], dtype=torch.long)
+        want[g] += 0.25 * a[rows].double().t() @ dc[offsets[g]:offsets[g + 1]].double()
+        size[g] += 0.25 * a[rows].double().abs().t() @ dc[offsets[g]:offsets[g + 1]].double().abs()
+    out = db.cuda()
+    tf.ragged_gemm_grad_into(a.cuda(), dc.cuda(), made(tf, torch, ids, 4), 0.25, 2.0, out, gather=True)
+    close(out, want, size, 60, "float32")
+
+
+@pytest.mark.gpu
+def test_ragged_gradients_against_differences(tf, torch):
+    rng = np.random.default_rng(4)
+    ids = choices(rng, 12, 2, 3)
+    g = made(tf, torch, ids, 3)
+    a, b, dc = (tensor(torch, rng, s, "float64").cuda() for s in ((12, 9), (3, 9, 7), (24, 7)))
+    da, db = tf.ragged_gemm_backward(a, b, dc, g, gather=True)
+    for t, grad in ((a, da), (b, db)):
+        for _ in range(6):
+            d = torch.randn_like(t)
+            h = 1e-5      # the product is linear in each operand: the difference has no error but rounding, < 1e-8 here
+            value = lambda s: (tf.ragged_gemm(*((t + s * d, b) if t is a else (a, t + s * d)), g, gather=True) * dc).sum()
+            assert abs((value(h) - value(-h)) / (2 * h) - (grad * d).sum()) < 1e-8
+
+
+@pytest.mark.gpu
+def test_ragged_product_beyond_32_bit_offsets(tf, torch):
+    # the weights, the result and the rows' source each span more than 2^32 bytes
+    rng = np.random.default_rng(6)
+    groups, K, N = 70, 64, 700000
+    b = torch.zeros(groups, K, N, dtype=torch.bfloat16, device="cuda")
+    some = tensor(torch, rng, (K, 40), "bfloat16")
+    b[69, :, -40:] = some.cuda()
+    a = tensor(torch, rng, (3200, K), "bfloat16")
+    ids = np.full(3200, 69)
+    ids[:5] = 0
+    c = tf.ragged_gemm(a.cuda(), b, made(tf, torch, ids, groups), gather=True)
+    want, size = a[-6:].double() @ some.double(), a[-6:].double().abs() @ some.double().abs()
+    close(c[-6:, -40:], want, size, K, "bfloat16")
+    assert not c[:5].any() and not c[-1, :-40].any()
+    del b, c
+    wide = torch.zeros(3200, 700000, dtype=torch.bfloat16, device="cuda")
+    wide[:, -K:] = a.cuda()
+    small = tensor(torch, rng, (2, K, 24), "bfloat16")
+    c = tf.ragged_gemm(wide[:, -K:], small.cuda(), made(tf, torch, np.ones(3200, int), 2), gather=True)
+    close(c, a.double() @ small[1].double(), a.double().abs() @ small[1].double().abs(), K, "bfloat16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+def test_ragged_product_of_uneven_groups_of_many_rows(tf, torch, name):
+    # groups of 0, 1, 1023 ... rows across many tiles; the reference in blocks
+    rng = np.random.default_rng(9)
+    counts = [0, 1, 1023, 0, 257, 256, 5, 128, 600, 0, 31]
+    ids = np.repeat(np.arange(len(counts)), counts)
+    K, N = 320, 288
+    offsets = np.cumsum([0] + counts)
+    a, b = tensor(torch, rng, (len(ids), K), name), tensor(torch, rng, (len(counts), K, N), name, K ** -0.5)
+    for how in ("columns", "rows"):
+        g = tf.RowGroups(torch.tensor(offsets, dtype=torch.int32, device="cuda"), n_rows=len(ids))
+        got = tf.ragged_gemm(a.cuda(), layout(torch, b, how), g)
+        want = torch.cat([a[offsets[i]:offsets[i + 1]].double() @ b[i].double() for i in range(len(counts))])
+        size = torch.cat([a[offsets[i]:offsets[i + 1]].double().abs() @ b[i].double().abs() for i in range(len(counts))])
+        close(got, want, size, K, name)
+        dc = tensor(torch, rng, (len(ids), N), name)
+        da, db = tf.ragged_gemm_backward(a.cuda(), layout(torch, b, how), dc.cuda(), g)
+        D, A, B = dc.double(), a.double(), b.double()
+        cut = [slice(offsets[i], offsets[i + 1]) for i in range(len(counts))]
+        close(da, torch.cat([D[s] @ B[i].t() for i, s in enumerate(cut)]), torch.cat([D[s].abs() @ B[i].abs().t() for i, s in enumerate(cut)]), N, name)
+        close(db, torch.stack([A[s].t() @ D[s] for s in cut]), torch.stack([A[s].abs().t() @ D[s].abs() for s in cut]), 1023, name)
+
+
+# ------------------------------------------------------------------------------------------------------ joining
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("tokens,fan,groups,N", [(1, 1, 1, 1), (1, 8, 8, 40), (33, 2, 5, 7), (70, 3, 4, 513), (9, 11, 12, 64), (600, 4, 16, 128)])
+@pytest.mark.parametrize("how", ["columns", "pitch", "steps"])
+def test_combine_and_its_gradients(tf, torch, name, tokens, fan, groups, N, how):
+    rng = np.random.default_rng(tokens + N)
+    ids = choices(rng, tokens, fan, groups)
+    offsets, order, positions = grouping(ids.reshape(-1), groups)
+    wide = torch.float64 if name == "float64" else torch.float32
+    x, dy = tensor(torch, rng, (tokens * fan, N), name), tensor(torch, rng, (tokens, N), name)
+    w = torch.from_numpy(rng.standard_normal((tokens, fan))).to(wide)
+    grouped = np.asarray(positions).reshape(tokens, fan) >= 0
+    w[~torch.from_numpy(grouped)] = float("nan")                   # the weight of a choice of no group is never used
+    g = made(tf, torch, ids, groups)
+    y = tf.combine_rows(layout(torch, x, how), g, w.cuda())
+    dx, dw = tf.combine_rows_backward(layout(torch, x, how), layout(torch, w, "steps"), layout(torch, dy, how), g)
+    plain = tf.combine_rows(x.cuda(), g)
+    X, D, W = x.double(), dy.double(), w.double()
+    want, size, ones, ones_size = (torch.zeros(tokens, N, dtype=torch.float64) for _ in range(4))
+    want_x = torch.zeros(tokens * fan, N, dtype=torch.float64)
+    want_w, size_w = torch.zeros(tokens, fan, dtype=torch.float64), torch.zeros(tokens, fan, dtype=torch.float64)
+    for t, j in itertools.product(range(tokens), range(fan)):
+        p = positions[t * fan + j]
+        if p < 0:
+            continue
+        want[t] += W[t, j] * X[p]
+        size[t] += (W[t, j] * X[p]).abs()
+        ones[t] += X[p]
+        ones_size[t] += X[p].abs()
+        want_x[p] = W[t, j] * D[t]
+        want_w[t, j], size_w[t, j] = X[p] @ D[t], X[p].abs() @ D[t].abs()
+    close(y, want, size, fan, name)
+    close(plain, ones, ones_size, fan, name)
+    close(dx, want_x, want_x.abs(), 1, name)
+    close(dw, want_w, size_w, N, "float64" if name == "float64" else "float32")
+    only_x, none = tf.combine_rows_backward(x.cuda(), None, dy.cuda(), g)
+    assert none is None
+    close(only_x, torch.where(torch.tensor([p in set(positions) for p in range(tokens * fan)])[:, None], D[torch.tensor(order) // fan], 0.0), D.abs().max() * torch.ones(1), 1, name)
+
+
+# ------------------------------------------------------------------------------------------------------ adapters
+def adapter_reference(torch, x, w, a, b, scales, ids):
+    X, W, A, B = x.double(), w.double(), a.double(), b.double()
+    y, size, low = X @ W, X.abs() @ W.abs(), torch.zeros(X.shape[0], W.shape[1], dtype=torch.float64)
+    for t, g in enumerate(ids):
+        if 0 <= g < A.shape[0]:
+            s = 1.0 if scales is None else float(scales[g])
+            y[t] += s * (X[t] @ A[g] @ B[g])
+            low[t] = abs(s) * (X[t].abs() @ A[g].abs() @ B[g].abs())
+    return y, size + low, low
+
+
+ADAPTERS = [(1, 1, 1, 1, 1), (1, 3, 64, 40, 4), (5, 2, 33, 17, 7), (64, 32, 136, 200, 16), (100, 3, 72, 65, 24), (200, 4, 256, 130, 50), (130, 64, 96, 128, 100), (20, 2, 64, 64, 200)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("tokens,groups,K,N,R", ADAPTERS)
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_adapters_and_their_gradients(tf, torch, name, tokens, groups, K, N, R, how):
+    rng = np.random.default_rng(tokens + K + R)
+    ids = choices(rng, tokens, 1, groups, none=0.25)[:, 0]
+    wide = torch.float64 if name == "float64" else torch.float32
+    x, w = tensor(torch, rng, (tokens, K), name), tensor(torch, rng, (K, N), name, K ** -0.5)
+    a, b = tensor(torch, rng, (groups, K, R), name, K ** -0.5), tensor(torch, rng, (groups, R, N), name, R ** -0.5)
+    scales = torch.from_numpy(0.2 + rng.random(groups)).to(wide)
+    dy = tensor(torch, rng, (tokens, N), name)
+    g = made(tf, torch, ids, groups)
+    on = [layout(torch, t, how) for t in (w, a, b)]
+    want, size, low = adapter_reference(torch, x, w, a, b, scales, ids)
+    close(tf.adapter_gemm(x.cuda(), *on, g, scales.cuda()), want, size, K + R, name, MIDDLE[name] * low)
+    want, size, low = adapter_reference(torch, x, w, a, b, None, ids)
+    close(tf.adapter_gemm(x.cuda(), *on, g), want, size, K + R, name, MIDDLE[name] * low)
+    dx, da, db = tf.adapter_gemm_backward(x.cuda(), *on, dy.cuda(), g, scales.cuda())
+    want, size, low = adapter_reference(torch, dy, w.t(), b.transpose(1, 2), a.transpose(1, 2), scales, ids)
+    close(dx, want, size, N + R, name, MIDDLE[name] * low)
+    X, D, A, B, S = x.double(), dy.double(), a.double(), b.double(), scales.double()
+    for i in range(groups):
+        rows = torch.tensor(np.nonzero(ids == i)[0])
+        xg, dg = X[rows], D[rows]
+        u, ua = dg @ B[i].t(), dg.abs() @ B[i].abs().t()
+        v, va = xg @ A[i], xg.abs() @ A[i].abs()
+        size = S[i] * xg.abs().t() @ ua
+        close(da[i], S[i] * xg.t() @ u, size, len(rows) + N, name, MIDDLE[name] * size)
+        size = S[i] * va.t() @ dg.abs()
+        close(db[i], S[i] * v.t() @ dg, size, len(rows) + K, name, MIDDLE[name] * size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16", "float32"])
+def test_an_adapter_that_is_no_number_stays_with_its_rows(tf, torch, name):
+    rng = np.random.default_rng(1)
+    ids = np.array([0, 1, 2, -1, 1, 0, 2, 9])
+    x, w = tensor(torch, rng, (8, 64), name), tensor(torch, rng, (64, 48), name, 0.125)
+    a, b = tensor(torch, rng, (3, 64, 8), name, 0.125), tensor(torch, rng, (3, 8, 48), name)
+    g = made(tf, torch, ids, 3)
+    clean = tf.adapter_gemm(x.cuda(), w.cuda(), a.cuda(), b.cuda(), g).cpu()
+    b[1], a[2, 5, 3] = float("inf"), float("nan")
+    got = tf.adapter_gemm(x.cuda(), w.cuda(), a.cuda(), b.cuda(), g).cpu()
+    for t in (0, 3, 5, 7):
+        assert torch.equal(got[t], clean[t])
+    for t in (1, 2, 4, 6):
+        assert not got[t].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,big", [("float16", 3.0e4), ("bfloat16", 1.0e30), ("float32", 1.0e30)])
+def test_an_adapters_middle_may_exceed_the_operands_range(tf, torch, name, big):
+    # x a is 64 * big (beyond f16's largest 65504), x a b again in range
+    x = torch.full((6, 64), 1.0, dtype=getattr(torch, name))
+    a, b = torch.full((2, 64, 4), big, dtype=x.dtype), torch.full((2, 4, 24), 2.0 ** -13 if name == "float16" else 2.0 ** -60, dtype=x.dtype)
+    w = torch.zeros(64, 24, dtype=x.dtype)
+    ids = np.array([0, 1, 0, 1, -1, 0])
+    want, size, low = adapter_reference(torch, x, w, a, b, None, ids)
+    assert want.abs().max() < 6e4 or name != "float16"
+    close(tf.adapter_gemm(x.cuda(), w.cuda(), a.cuda(), b.cuda(), made(tf, torch, ids, 2)), want, size, 68, name, MIDDLE[name] * low)
+
+
+# ------------------------------------------------------------------------------------------------------ together, streams, graphs
+def expert_layer(tf, x, up, down, ids, gates):
+    groups = tf.RowGroups.from_ids(ids, up.shape[0])
+    h = tf.ragged_gemm(x, up, groups, gather=True)
+    return tf.combine_rows(tf.ragged_gemm(h, down, groups), groups, gates), groups, h
+
+
+def expert_gradients(tf, x, up, down, gates, dy, groups, h):
+    z = tf.ragged_gemm(h, down, groups)
+    dz, dgates = tf.combine_rows_backward(z, gates, dy, groups)
+    dh, ddown = tf.ragged_gemm_backward(h, down, dz, groups)
+    dx, dup = tf.ragged_gemm_backward(x, up, dh, groups, gather=True)
+    return dx, dup, ddown, dgates
+
+
+def layer_inputs(torch, seed, name="float32", tokens=48, fan=2, groups=6, K=40, N=56):
+    rng = np.random.default_rng(seed)
+    x, up, down = tensor(torch, rng, (tokens, K), name), tensor(torch, rng, (groups, K, N), name, K ** -0.5), tensor(torch, rng, (groups, N, K), name, N ** -0.5)
+    ids = torch.from_numpy(choices(rng, tokens, fan, groups))
+    gates = torch.softmax(torch.from_numpy(rng.standard_normal((tokens, fan))), 1).to(torch.float64 if name == "float64" else torch.float32)
+    return [t.cuda() for t in (x, up, down, ids, gates, tensor(torch, rng, (tokens, K), name))]
+
+
+@pytest.mark.gpu
+def test_a_layer_of_experts_and_its_gradients_together(tf, torch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 0, "float64")
+    y, groups, h = expert_layer(tf, x, up, down, ids, gates)
+    got = expert_gradients(tf, x, up, down, gates, dy, groups, h)
+    leaves = [t.cpu().clone().requires_grad_() for t in (x, up, down, gates)]
+    X, UP, DOWN, GATES = leaves
+    rows = []
+    for t in range(X.shape[0]):
+        total = torch.zeros(X.shape[1], dtype=torch.float64)
+        for j, e in enumerate(ids[t].tolist()):
+            if 0 <= e < UP.shape[0]:
+                total = total + GATES[t, j] * (X[t] @ UP[e] @ DOWN[e])
+        rows.append(total)
+    Y = torch.stack(rows)
+    want = torch.autograd.grad((Y * dy.cpu()).sum(), leaves)
+    assert (y.cpu() - Y).abs().max() < 1e-12          # sums of 40, 56 and 2 products of order one in 64 bits
+    for a, b in zip((got[0], got[1], got[2], got[3]), want):
+        assert (a.cpu() - b).abs().max() < 1e-11
+
+
+@pytest.mark.gpu
+def test_calls_on_another_stream_and_on_tensors(tf, torch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 1)
+    want, _, _ = expert_layer(tf, x, up, down, ids, gates)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    st = side.cuda_stream
+    groups = tf.RowGroups.from_ids(ids, up.shape[0], stream=st)
+    h = tf.ragged_gemm(x, up, groups, gather=True, stream=st)
+    y = tf.combine_rows(tf.ragged_gemm(h, down, groups, stream=st), groups, gates, stream=st)
+    del h
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, want)
+    T = tf.Tensor.from_torch
+    groups = tf.RowGroups.from_ids(ids, up.shape[0], stream=st)      # its event orders the current stream's calls behind it
+    out = tf.combine_rows(tf.ragged_gemm(tf.ragged_gemm(T(x), T(up), groups, gather=True), T(down), groups), groups, T(gates))
+    assert isinstance(out, tf.Tensor) and out.event is not None
+    assert np.array_equal(out.to_numpy(), want.cpu().numpy())
+    assert tf.Tensor.from_torch(x.bfloat16()).to_numpy().dtype == np.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float32"])
+def test_captured_calls_replay_on_new_choices(tf, torch, name):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 2, name)
+    others = [layer_inputs(torch, s, name) for s in (3, 4, 5)]
+    low_a, low_b = up[:, :, :8].contiguous(), up[:, :8, :].contiguous()
+    weights = up[0].contiguous()
+
+    def everything():
+        y, groups, h = expert_layer(tf, x, up, down, ids, gates)
+        flat = tf.RowGroups.from_ids(ids[:, 0], up.shape[0])
+        z = tf.adapter_gemm(x, weights, low_a, low_b, flat)
+        return (y, z) + expert_gradients(tf, x, up, down, gates, dy, groups, h) + tf.adapter_gemm_backward(x, weights, low_a, low_b, z, flat)
+
+    everything()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                       # two graphs, each with buffers of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = everything()
+        graphs.append((graph, out))
+    for new in others:
+        for t, n in zip((x, ids, gates, dy), (new[0], new[3], new[4], new[5])):
+            t.copy_(n)
+        want = [t.clone() for t in everything()]
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_the_same_call_gives_the_same_bits(tf, torch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 7, "bfloat16", tokens=300, fan=3, groups=5, K=136, N=264)
+    first = None
+    for _ in range(3):
+        y, groups, h = expert_layer(tf, x, up, down, ids, gates)
+        out = (y,) + expert_gradients(tf, x, up, down, gates, dy, groups, h)
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+@pytest.mark.gpu
+def test_lists_that_lead_nowhere_stay_inside_the_views(tf, torch):
+    # offsets, orders and positions beyond the rows are treated as absent
+    a = torch.ones(8, 16, dtype=torch.bfloat16, device="cuda")
+    b = torch.ones(3, 16, 8, dtype=torch.bfloat16, device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    g = tf.RowGroups(i32([0, 3, 900, 1000]), i32([0, 1, 77, -3, 4, 5, 2000000000, 7]), i32([0, 900, -7, 3, 4, 5, 6, 7]))
+    c = tf.ragged_gemm(a, b, g, gather=True).cpu()
+    assert [float(v) for v in c[:, 0]] == [16, 16, 0, 0, 16, 16, 0, 16]
+    y = tf.combine_rows(a, g).cpu()
+    assert [float(v) for v in y[:, 0]] == [1, 0, 0, 1, 1, 1, 1, 1]
+    g = tf.RowGroups(i32([-5, 6, 2, 8]), n_rows=8)                 # not ascending: the middle group has no rows
+    tf.ragged_gemm(a, b, g)
+    tf.adapter_gemm(a, b[0], b, torch.ones(3, 8, 8, dtype=torch.bfloat16, device="cuda"), g)
+    tf.ragged_gemm_backward(a, b, torch.ones(8, 8, dtype=torch.bfloat16, device="cuda"), g)
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------------ refusals (no GPU)
+def view(tf, dims, strides=None, base=4096, flags=0):
+    v = tf.tfh_view()
+    v.base, v.rank, v.flags, v.offset = base, len(dims), flags, 0
+    if strides is None:
+        strides = [int(np.prod(dims[i + 1:])) for i in range(len(dims))]
+    for i, (d, s) in enumerate(zip(dims, strides)):
+        v.dims[i], v.strides[i] = d, s
+    return C.byref(v)
+
+
+def row_groups(tf, n_rows=8, n_groups=3, fan=1, offsets=4096, order=4096, positions=4096):
+    from tenferro_rs_amd.row_groups import tfh_row_groups
+    return C.byref(tfh_row_groups(offsets, order, positions, n_rows, n_groups, fan))
+
+
+def refused(tf, call, error):
+    with pytest.raises(error) as e:
+        tf._check(call)
+    return e.value
+
+
+def test_products_refuse_what_does_not_fit(tf):
+    L, V, G = tf.lib(), lambda *d, **k: view(tf, d, **k), lambda **k: row_groups(tf, **k)
+    run = lambda dt=4, g=None, fl=0, a=None, b=None, c=None: L.tfh_ragged_gemm(dt, g or G(), fl, 1.0, a or V(8, 16), b or V(3, 16, 24), 0.0, c or V(8, 24), None)
+    for dt in (2, 3, -1, 6):
+        refused(tf, run(dt=dt), tf.InvalidArgument)
+    e = refused(tf, run(a=V(7, 16)), tf.ShapeMismatch)
+    assert e.expected == [8, 16] and e.got == [7, 16]
+    refused(tf, run(a=V(8, 16, 1)), tf.RankMismatch)
+    refused(tf, run(b=V(16, 24)), tf.RankMismatch)
+    assert refused(tf, run(b=V(3, 17, 24)), tf.ShapeMismatch).expected == [3, 16, 24]
+    refused(tf, run(b=V(4, 16, 24)), tf.ShapeMismatch)
+    refused(tf, run(c=V(8, 25)), tf.ShapeMismatch)
+    refused(tf, run(c=V(8, 24, strides=[0, 1])), tf.InvalidArgument)
+    refused(tf, run(a=V(8, 16, base=0)), tf.InvalidArgument)
+    refused(tf, run(a=V(8, 16, flags=1)), tf.InvalidArgument)
+    refused(tf, run(fl=8), tf.InvalidArgument)
+    refused(tf, run(fl=1, g=G(order=None)), tf.InvalidArgument)
+    refused(tf, run(fl=2, g=G(order=None)), tf.InvalidArgument)
+    refused(tf, run(fl=1, g=G(fan=2)), tf.ShapeMismatch)               # gathered: A has n_rows / fan rows
+    for bad in (dict(n_groups=0), dict(n_rows=-1), dict(fan=0), dict(fan=3), dict(offsets=None), dict(n_rows=1 << 40)):
+        refused(tf, run(g=G(**bad)), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm(4, None, 0, 1.0, V(8, 16), V(3, 16, 24), 0.0, V(8, 24), None), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm(4, G(), 0, 1.0, None, V(3, 16, 24), 0.0, V(8, 24), None), tf.InvalidArgument)
+    grad = lambda fl=0, a=None, dc=None, db=None: L.tfh_ragged_gemm_grad(4, G(), fl, 1.0, a or V(8, 16), dc or V(8, 24), 0.0, db or V(3, 16, 24), None)
+    refused(tf, grad(fl=4), tf.InvalidArgument)
+    refused(tf, grad(dc=V(9, 24)), tf.ShapeMismatch)
+    refused(tf, grad(db=V(3, 24, 16)), tf.ShapeMismatch)
+
+
+def test_grouping_refuses_what_does_not_fit(tf):
+    L = tf.lib()
+    run = lambda bits=32, ids=None, n=4, off=4096, order=4096, ws=4096, b=1 << 20: L.tfh_group_rows(bits, ids or view(tf, [8]), n, off, order, None, ws, b, None)
+    refused(tf, run(bits=16), tf.InvalidArgument)
+    refused(tf, run(n=0), tf.InvalidArgument)
+    refused(tf, run(n=2049), tf.InvalidArgument)
+    refused(tf, run(ids=view(tf, [2, 2, 2])), tf.RankMismatch)
+    refused(tf, run(ids=view(tf, [8], base=0)), tf.InvalidArgument)
+    refused(tf, run(ids=view(tf, [1 << 20, 1 << 20])), tf.InvalidArgument)
+    refused(tf, run(off=None), tf.InvalidArgument)
+    refused(tf, run(order=None), tf.InvalidArgument)
+    refused(tf, run(ids=view(tf, [100000]), b=16), tf.InvalidArgument)
+    refused(tf, run(ids=view(tf, [100000]), ws=4100), tf.InvalidArgument)
+    assert L.tfh_group_rows_workspace(100, 4) == 0 and L.tfh_group_rows_workspace(1 << 20, 4) > 0
+
+
+def test_joining_refuses_what_does_not_fit(tf):
+    L, V, G = tf.lib(), lambda *d, **k: view(tf, d, **k), lambda **k: row_groups(tf, **dict(dict(fan=2), **k))
+    run = lambda g=None, x=None, w=None, y=None: L.tfh_combine_rows(4, g or G(), x or V(8, 6), w, y or V(4, 6), None)
+    refused(tf, run(g=G(positions=None)), tf.InvalidArgument)
+    refused(tf, run(x=V(8, 7)), tf.ShapeMismatch)
+    refused(tf, run(y=V(8, 6)), tf.ShapeMismatch)
+    refused(tf, run(w=V(2, 4)), tf.ShapeMismatch)
+    refused(tf, run(y=V(4)), tf.RankMismatch)
+    refused(tf, L.tfh_combine_rows_grad(4, G(), V(8, 6), None, V(4, 6), V(8, 5), None, None), tf.ShapeMismatch)
+    refused(tf, L.tfh_combine_rows_grad(4, G(), None, None, V(4, 6), V(8, 6), V(4, 2), None), tf.InvalidArgument)
+
+
+def test_adapters_refuse_what_does_not_fit(tf):
+    L, V, G = tf.lib(), lambda *d, **k: view(tf, d, **k), lambda **k: row_groups(tf, **k)
+    ok = dict(x=V(8, 16), w=V(16, 24), a=V(3, 16, 4), b=V(3, 4, 24), s=None, y=V(8, 24))
+
+    def run(g=None, ws=4096, nb=1 << 20, **k):
+        v = dict(ok, **k)
+        return L.tfh_adapter_gemm(4, g or G(), v["x"], v["w"], v["a"], v["b"], v["s"], v["y"], ws, nb, None)
+
+    refused(tf, run(g=G(fan=2)), tf.InvalidArgument)
+    refused(tf, run(x=V(8, 15)), tf.ShapeMismatch)
+    refused(tf, run(a=V(3, 16)), tf.RankMismatch)
+    refused(tf, run(b=V(3, 5, 24)), tf.ShapeMismatch)
+    refused(tf, run(b=V(2, 4, 24)), tf.ShapeMismatch)
+    refused(tf, run(y=V(8, 16)), tf.ShapeMismatch)
+    refused(tf, run(s=V(4)), tf.ShapeMismatch)
+    refused(tf, run(s=V(3, strides=[2])), tf.Strided)
+    refused(tf, run(ws=None), tf.InvalidArgument)
+    refused(tf, run(nb=8 * 4 * 4 - 1), tf.InvalidArgument)
+    refused(tf, run(ws=4104), tf.InvalidArgument)
+    assert L.tfh_adapter_workspace(4, 8, 4, 0) == 8 * 4 * 4
+    refused(tf, L.tfh_adapter_gemm_grad(4, G(), ok["x"], ok["w"], ok["a"], ok["b"], None, V(8, 24), None, V(3, 16, 5), None, 4096, 1 << 20, None), tf.ShapeMismatch)
+
+
+def test_what_has_no_place_on_the_gpu_is_refused_by_name(tf):
+    import torch
+    with pytest.raises(tf.NoCompatibleComputeDevice):
+        tf.RowGroups.from_ids(torch.zeros(4, dtype=torch.int64), 2)
+    with pytest.raises(tf.NoCompatibleComputeDevice):
+        tf.RowGroups(torch.zeros(3, dtype=torch.int32), n_rows=4)
+    with pytest.raises(tf.InvalidArgument):
+        tf.ragged_gemm(torch.zeros(4, 4), torch.zeros(1, 4, 4), None)
+
+
+@pytest.mark.parametrize("call", ["plan", "fill", "conj"])
+def test_16_bit_types_are_refused_elsewhere(tf, call):
+    L = tf.lib()
+    for dt in (tf.BF16, tf.F16):
+        assert L.tfh_dtype_size(dt) == 2
+        if call == "plan":
+            with pytest.raises(tf.InvalidArgument):
+                tf.HipBackend.plan(dt, tf.PrimDescriptor.Contract([0, 1], [1, 2], [0, 2]), [[2, 3], [3, 4], [2, 4]])
+            assert not tf.HipBackend.has_extension_for(dt, tf.Extension.Contract)
+        elif call == "fill":
+            refused(tf, L.tfh_fill(dt, (C.c_double * 2)(), view(tf, [4]), None), tf.InvalidArgument)
+        else:
+            refused(tf, L.tfh_conj(dt, view(tf, [4]), view(tf, [4]), None), tf.InvalidArgument)
