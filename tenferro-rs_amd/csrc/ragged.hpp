@@ -191,31 +191,32 @@ __device__ __forceinline__ bool find_tile(const Args& a, int tm, int tiles_n, ui
         const int to = g < a.n_groups ? clamp_row(a.offsets[g + 1], a.n_rows) : (int)a.n_rows;
         return to > from ? to - from : 0;
     };
-    uint64_t total = 0;
+    // (a launch has fewer blocks than 2^31, and so there are fewer tiles; the scalars tell the compiler that they are)
+    uint32_t total = 0;
     for (int g0 = 0; g0 < groups; g0 += 64) total += (uint32_t)((rows_of(g0 + lane) + tm - 1) / tm);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
-    total *= tiles_n;
+    total = __builtin_amdgcn_readfirstlane(total) * (uint32_t)tiles_n;
     if (block >= total) return false;
     // every XCD walks one contiguous range of the tiles
-    uint64_t want = gemm::logical_block(block, total);
+    uint32_t want = __builtin_amdgcn_readfirstlane((uint32_t)gemm::logical_block(block, total));
     for (int g0 = 0; g0 < groups; g0 += 64) {
         const int rows = rows_of(g0 + lane);
-        const uint64_t mine = (uint64_t)((rows + tm - 1) / tm) * tiles_n;
-        uint64_t upto = mine;
+        const uint32_t mine = (uint32_t)((rows + tm - 1) / tm) * (uint32_t)tiles_n;
+        uint32_t upto = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t o = __shfl_up(upto, d, 64);
+            const uint32_t o = __shfl_up(upto, d, 64);
             if (lane >= d) upto += o;
         }
-        const uint64_t here = __shfl(upto, 63, 64);
+        const uint32_t here = __builtin_amdgcn_readlane(upto, 63);
         if (want < here) {
             const int at = __builtin_ctzll(__ballot(want < upto));
-            const uint32_t rest = (uint32_t)(want - __shfl(upto - mine, at, 64));
-            t.group = __builtin_amdgcn_readfirstlane(g0 + at);
-            const int rows_g = __builtin_amdgcn_readfirstlane(__shfl(rows, at, 64));
-            gemm::tile_of(__builtin_amdgcn_readfirstlane(rest), (rows_g + tm - 1) / tm, tiles_n, t.tile_m, t.tile_n);
-            t.first = clamp_row(a.offsets[t.group], a.n_rows) + t.tile_m * tm;
+            const uint32_t rest = want - __builtin_amdgcn_readlane(upto - mine, at);
+            const int rows_g = __builtin_amdgcn_readlane(rows, at);
+            t.group = g0 + at;
+            gemm::tile_of(rest, (rows_g + tm - 1) / tm, tiles_n, t.tile_m, t.tile_n);
+            t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows)) + t.tile_m * tm;
             t.rows = rows_g - t.tile_m * tm < tm ? rows_g - t.tile_m * tm : tm;
             return true;
         }

@@ -1,0 +1,282 @@
+// ragged_fast.hpp -- products over rows in groups for 16-bit operands whose rows start 16-byte aligned: the same tiles in
+// LDS as ragged.hpp, but written there by the memory system itself (buffer loads with LDS as their destination, 16 bytes a
+// lane, no registers in between), double-buffered, and a register pipeline in front of the matrix cores.
+//
+// Per stage (128 bytes of k of every row, two halves of 64) and wave:
+//   first half's products   while the second half's fragments are read from LDS
+//   wait: the fragments are here, the next stage's loads have landed; barrier: so they have for every wave, and this
+//         stage's buffer has been read by all
+//   second half's products  while the loads of the stage after the next are issued into this stage's buffer and the next
+//                           stage's first fragments are read
+// so a load has most of a stage's products to arrive in, a fragment half a stage, and there is one barrier per stage.
+#pragma once
+#include "ragged.hpp"
+
+namespace tfh {
+namespace ragged {
+
+// A buffer of `bytes` bytes from `base`: a load whose offset lies beyond reads zeros.
+__device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
+    const uint64_t p = (uint64_t)base;
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((uint32_t)p);
+    r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32) & 0xffff);
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = 0x00020000;
+    return r;
+}
+constexpr uint32_t NOWHERE = 0xfffffff0u;   // an offset beyond every buffer (spans are under MOST_SPAN)
+constexpr int64_t MOST_SPAN = 0xffff0000ll;
+
+// 16 bytes a lane from buffer + offset + scalar into LDS at `to` + 16 * lane.  The compiler does not count these loads:
+// wait_loads() does, before anything they write is read.
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t scalar, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(buffer), "s"(scalar) : "memory");
+}
+template <int LEFT> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void wait_fragments_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// 32 x 32 x 16 products: lane l = 32 p + j holds row j and k = 8 p .. 8 p + 7 of either operand; register r of the result
+// is row 8 (r / 4) + 4 p + r % 4 of the first operand and column j, a row of the second.  (The 16 x 16 form needs twice
+// the instructions, and its 256 accumulators in pieces of 4 made the compiler move a third of them in every stage.)
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <class T> __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The 16 k's h = 0 .. 3 of a stage for 32 rows from `row`.
+template <class T, int TM, bool KFAST>
+__device__ __forceinline__ u32x4 fragment32(const char* tile, int row, int h, int lane) {
+    if constexpr (KFAST) {
+        return *(const u32x4*)(tile + kfast_at<T>(row + (lane & 31), 2 * h + (lane >> 5)));
+    } else {
+        typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+        const int j = lane & 15, k = 16 * h + 8 * (lane >> 5) + (j >> 2), col = row + (lane & 16) + 4 * (j & 3);
+        const uint32_t within = (col * 2) & 15, chunk = (col * 2) >> 4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + rowfast_at<T, TM>(k, chunk) + within));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + rowfast_at<T, TM>(k + 4, chunk) + within));
+        struct { s16x4 a, b; } both = {lo, hi};
+        return __builtin_bit_cast(u32x4, both);
+    }
+}
+
+// The shape of a block: WM x WN = 4 waves of 32 XT x 32 YT results.
+template <int WM_, int WN_, int XT_, int YT_> struct Shape {
+    static_assert(WM_ * WN_ == 4, "four waves");
+    static constexpr int WM = WM_, WN = WN_, XT = XT_, YT = YT_, TM = 32 * WM * XT, TN = 32 * WN * YT;
+    static constexpr int STAGE = (TM + TN) * 128, LDS = 2 * STAGE;
+    static constexpr int BLOCKS = XT * YT > 8 ? 1 : 2;   // of a CU: registers and LDS leave room for so many
+};
+
+template <class T, int MODE, bool BKFAST, class S>
+__global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args a) {
+    static_assert(sizeof(T) == 2, "16-bit operands");
+    constexpr int XT = S::XT, YT = S::YT, TM = S::TM, TN = S::TN, BK = 64, STAGE = S::STAGE;
+    constexpr int CA = TM / 32, CB = TN / 32;      // chunks of each operand per thread and stage
+    constexpr bool AKFAST = MODE != OUTER;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    char* const lds = (char*)smem_raw;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % S::WM, wn = wave / S::WM;
+    const int tiles_n = (a.N + TN - 1) / TN;
+    Tile t;
+    if constexpr (MODE == ROWS) {
+        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+    } else if constexpr (MODE == OUTER) {
+        const int tiles_m = (a.M + TM - 1) / TM;
+        const uint32_t id = (uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), each = (uint32_t)tiles_m * tiles_n;
+        t.group = (int)(id / each);
+        gemm::tile_of(id % each, tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows));
+        const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group + 1], a.n_rows));
+        t.rows = to > t.first ? to - t.first : 0;
+    } else {
+        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
+        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.group = 0;
+        t.first = t.tile_m * TM;
+        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
+    }
+    const bool real = MODE != ROWS || t.group < a.n_groups;
+    const int n0 = t.tile_n * TN, m0 = t.tile_m * TM;
+    f32x16 acc[XT][YT];
+#pragma unroll
+    for (int x = 0; x < XT; ++x)
+#pragma unroll
+        for (int y = 0; y < YT; ++y)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[x][y][r] = 0;
+
+    // This thread's chunks.  k-fast: the chunk (tid ^ row) % 8 of rows tid / 8 + 32 i; row-fast: chunk (tid + 256 i) % RX of
+    // k = (tid + 256 i) / RX, its place swizzled; either way a wave's 64 lanes fill 1024 consecutive bytes of LDS.
+    const int cr = tid >> 3, kc = ((tid ^ cr) & 7) * 8;
+    constexpr int RA = TM / 8, RB = TN / 8;        // chunks of a row of k in a row-fast tile
+    const int kend = MODE == OUTER ? t.rows : real ? a.K : 0;
+    uint32_t va[CA], vb[CB];
+    u32x4 A, B;
+    uint32_t step_a = BK * 2, step_b = BK * 2;     // bytes from a stage to the next
+    int32_t next_row = -1;                         // outer, gathered: lane l holds the row of A for the next stage's l-th k
+    auto look_up = [&](int k0) {
+        if constexpr (!AKFAST)
+            if (a.gather && a.order) next_row = k0 + lane < kend ? (int)source_row(a, t.first + k0 + lane) : -1;
+    };
+    if constexpr (AKFAST) {
+        A = buffer_of(a.A, (uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2));
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            const int64_t s = cr + 32 * i < t.rows && real ? source_row(a, t.first + cr + 32 * i) : -1;
+            va[i] = s >= 0 ? (uint32_t)(s * a.a_row * 2) + kc * 2 : NOWHERE;
+        }
+    } else {
+        // rows of k are rows of the group; a gathered A's are looked up stage by stage
+        const bool gather = a.gather && a.order;
+        const int64_t first = gather ? 0 : t.first, rows = gather ? a.a_rows : kend;
+        A = buffer_of((const char*)a.A + first * a.a_row * 2, rows > 0 ? (uint32_t)((rows - 1) * a.a_row * 2 + a.M * 2) : 0);
+        step_a = gather ? 0 : BK * (uint32_t)a.a_row * 2;
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            const int id = tid + 256 * i, k = id / RA, m = m0 + ((id % RA) ^ (rowfast_swizzle<T>(k) & (RA - 1))) * 8;
+            va[i] = m < a.M ? (gather ? 0 : (uint32_t)(k * a.a_row * 2)) + m * 2 : NOWHERE;
+        }
+        look_up(0);
+    }
+    if constexpr (BKFAST) {
+        B = buffer_of((const char*)a.B + (MODE == ROWS && real ? t.group * a.b_group * 2 : 0), (uint32_t)((a.N - 1) * a.b_n * 2 + a.K * 2));
+#pragma unroll
+        for (int i = 0; i < CB; ++i) vb[i] = n0 + cr + 32 * i < a.N ? (uint32_t)((n0 + cr + 32 * i) * a.b_n * 2) + kc * 2 : NOWHERE;
+    } else {
+        const int64_t first = MODE == OUTER ? t.first * a.b_k : MODE == ROWS && real ? t.group * a.b_group : 0;
+        B = buffer_of((const char*)a.B + first * 2, kend > 0 ? (uint32_t)((kend - 1) * a.b_k * 2 + a.N * 2) : 0);
+        step_b = BK * (uint32_t)a.b_k * 2;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int id = tid + 256 * i, k = id / RB, n = n0 + ((id % RB) ^ (rowfast_swizzle<T>(k) & (RB - 1))) * 8;
+            vb[i] = n < a.N ? (uint32_t)(k * a.b_k * 2) + n * 2 : NOWHERE;
+        }
+    }
+    // chunk i of the two operands for the stage at k0, into buffer `to`
+    auto issue_a = [&](int i, int k0, uint32_t soff, uint32_t to) {
+        uint32_t v = va[i];
+        if constexpr (AKFAST) {
+            v = k0 + kc < kend ? v : NOWHERE;
+        } else {
+            const int k = (tid + 256 * i) / RA;
+            if (a.gather && a.order) {
+                const int s = __shfl(next_row, k, 64);   // (-1 behind the group's last row)
+                v = s >= 0 && v != NOWHERE ? v + (uint32_t)s * (uint32_t)(a.a_row * 2) : NOWHERE;
+            } else
+                v = k0 + k < kend ? v : NOWHERE;
+        }
+        load_to_lds(A, v, soff, to + i * 4096 + wave * 1024);
+    };
+    auto issue_b = [&](int i, int k0, uint32_t soff, uint32_t to) {
+        uint32_t v = vb[i];
+        if constexpr (BKFAST) v = k0 + kc < kend ? v : NOWHERE;
+        else v = k0 + (tid + 256 * i) / RB < kend ? v : NOWHERE;
+        load_to_lds(B, v, soff, to + TM * 128 + i * 4096 + wave * 1024);
+    };
+    u32x4 fa[2][XT], fb[2][YT];
+    auto read = [&](int set, int i, const char* stage, int h) {
+        if (i < XT) fa[set][i] = fragment32<T, TM, AKFAST>(stage, (wm * XT + i) * 32, h, lane);
+        else fb[set][i - XT] = fragment32<T, TN, BKFAST>(stage + TM * 128, (wn * YT + i - XT) * 32, h, lane);
+    };
+    constexpr int FRAGS = XT + YT, CHUNKS = CA + CB;
+    const int stages = (kend + BK - 1) / BK;
+    if (stages > 0) {
+        uint32_t sa = 0, sb = 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint32_t oa = s < stages ? sa : 0, ob = s < stages ? sb : 0;
+#pragma unroll
+            for (int i = 0; i < CA; ++i) issue_a(i, s * BK, oa, lds0 + s * STAGE);
+#pragma unroll
+            for (int i = 0; i < CB; ++i) issue_b(i, s * BK, ob, lds0 + s * STAGE);
+            look_up((s + 1) * BK);
+            sa += step_a, sb += step_b;
+        }
+        wait_loads<CHUNKS>();
+        wait_fragments_and_barrier();
+#pragma unroll
+        for (int i = 0; i < FRAGS; ++i) read(0, i, lds, 0);
+        int at = 0;
+        for (int s = 0; s < stages; ++s) {
+            // (behind the last stage the loads go nowhere and the fragments that are read are not used: no branch in the loop)
+            const int k0 = (s + 2) * BK;
+            const uint32_t to = lds0 + at, oa = s + 2 < stages ? sa : 0, ob = s + 2 < stages ? sb : 0;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                if (h == 3) {
+                    wait_loads<0>();
+                    wait_fragments_and_barrier();
+                }
+                constexpr int EACH = (FRAGS + XT - 1) / XT, LOADS = (CHUNKS + XT - 1) / XT;
+#pragma unroll
+                for (int x = 0; x < XT; ++x) {
+                    if (h == 3)
+#pragma unroll
+                        for (int i = x * LOADS; i < (x + 1) * LOADS && i < CHUNKS; ++i) {
+                            if (i < CA) issue_a(i, k0, oa, to);
+                            else issue_b(i - CA, k0, ob, to);
+                        }
+#pragma unroll
+                    for (int i = x * EACH; i < (x + 1) * EACH && i < FRAGS; ++i) read((h + 1) & 1, i, lds + (h == 3 ? at ^ STAGE : at), (h + 1) & 3);
+#pragma unroll
+                    for (int y = 0; y < YT; ++y) acc[x][y] = mma32<T>(fb[h & 1][y], fa[h & 1][x], acc[x][y]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            look_up(k0 + BK);
+            sa += step_a, sb += step_b;
+            at ^= STAGE;
+        }
+        wait_loads<0>();
+    }
+
+    const float alpha = (float)a.alpha * (MODE == ROWS && a.scales && real ? ((const float*)a.scales)[t.group] : 1.0f), beta = (float)a.beta;
+#pragma unroll
+    for (int x = 0; x < XT; ++x) {
+        const int r = (wm * XT + x) * 32 + (lane & 31);
+        if (MODE == OUTER ? m0 + r >= a.M : r >= t.rows) continue;
+        int64_t row = MODE == OUTER ? m0 + r : t.first + r;
+        if constexpr (MODE != OUTER)
+            if (a.scatter && a.order) {
+                row = a.order[row];
+                if (row < 0 || row >= a.n_rows) continue;
+            }
+        T* const c = (T*)a.C + (MODE == OUTER ? t.group * a.c_group : 0) + row * a.c_row;
+#pragma unroll
+        for (int y = 0; y < YT; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int n = n0 + (wn * YT + y) * 32 + 8 * g + 4 * (lane >> 5);
+                if (n >= a.N) continue;
+                T out[4];
+                if (a.use_beta && real) __builtin_memcpy(out, c + n, 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = real ? alpha * acc[x][y][4 * g + i] : 0.0f;
+                    if (a.use_beta && real) v += beta * (float)out[i];
+                    out[i] = (T)v;
+                }
+                __builtin_memcpy(c + n, out, 8);
+            }
+    }
+}
+
+// Whether the kernel can take a call: rows that start 16-byte aligned and end with a chunk, spans that 32 bits address.
+inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+inline bool fast_rows(const void* p, int64_t rows, int64_t stride, int64_t inner_stride, int64_t inner) {
+    return aligned(p, 16) && inner_stride == 1 && inner % 8 == 0 && stride % 8 == 0 && stride > 0 && (rows - 1) * stride * 2 + inner * 2 < MOST_SPAN;
+}
+template <int MODE> inline bool fast_takes(const Args& a, bool bkfast) {
+    if (a.c_n != 1 || a.c_row % 4 || a.N % 4 || !aligned(a.C, 8)) return false;
+    if (MODE == OUTER) {
+        if (a.c_group % 4) return false;
+        return fast_rows(a.A, a.a_rows, a.a_row, a.a_col, a.M) && fast_rows(a.B, a.b_rows, a.b_k, a.b_n, a.N) && !a.gather_b;
+    }
+    if (a.b_group % 8) return false;
+    return fast_rows(a.A, a.a_rows, a.a_row, a.a_col, a.K) && (bkfast ? fast_rows(a.B, a.N, a.b_n, a.b_k, a.K) : fast_rows(a.B, a.K, a.b_k, a.b_n, a.N));
+}
+
+}  // namespace ragged
+}  // namespace tfh
