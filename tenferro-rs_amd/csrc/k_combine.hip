@@ -131,16 +131,21 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, 
     }
 }
 
+template <class T> constexpr const char* name_of(const char* bf16, const char* f16, const char* f32, const char* f64) {
+    return __is_same(T, __bf16) ? bf16 : __is_same(T, _Float16) ? f16 : __is_same(T, float) ? f32 : f64;
+}
+
 template <class T> int32_t combine_of(const CombineArgs& a, hipStream_t st) {
     const int64_t blocks = (a.tokens + 3) / 4, pieces = (a.n + 64 * Num<T>::E - 1) / (64 * Num<T>::E);
     // few tokens: their columns are dealt to several blocks, so that more waves wait for memory
     const int64_t split = blocks >= 512 ? 1 : pieces < 512 / blocks ? pieces : 512 / blocks;
-    TFH_LAUNCH_TIMED(combine_kernel<T>, dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
+    TFH_LAUNCH_NAMED(name_of<T>("(combine_kernel<bf16>)", "(combine_kernel<f16>)", "(combine_kernel<float>)", "(combine_kernel<double>)"), combine_kernel<T>, dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
     return hip_check(hipGetLastError(), "combine launch");
 }
 template <class T> int32_t combine_grad_of(const CombineArgs& a, hipStream_t st) {
     const int64_t blocks = (a.tokens + 3) / 4, rest = a.n_rows < 256 ? (a.n_rows + 3) / 4 : 64;
-    TFH_LAUNCH_TIMED(combine_grad_kernel<T>, dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
+    TFH_LAUNCH_NAMED(name_of<T>("(combine_grad_kernel<bf16>)", "(combine_grad_kernel<f16>)", "(combine_grad_kernel<float>)", "(combine_grad_kernel<double>)"),
+                     combine_grad_kernel<T>, dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
     return hip_check(hipGetLastError(), "combine gradient launch");
 }
 

@@ -58,9 +58,12 @@ __device__ __forceinline__ void prefetch_kernel_arguments() {
     }
 }
 
-#define TFH_LAUNCH_TIMED(kernel, grid, block, lds, st, ...)                                                          \
+#define TFH_LAUNCH_TIMED(kernel, grid, block, lds, st, ...) TFH_LAUNCH_NAMED(tfh::kernel_label<&kernel>(), kernel, grid, block, lds, st, __VA_ARGS__)
+// The same with a label of the caller's (a string that lives as long as the library), for kernels whose template arguments
+// the demangler does not know: the 16-bit floating types.
+#define TFH_LAUNCH_NAMED(label, kernel, grid, block, lds, st, ...)                                                   \
     do {                                                                                                             \
-        const char* label_ = tfh::kernel_label<&kernel>();                                                           \
+        const char* label_ = label;                                                                                  \
         tfh::note_kernel(label_);                                                                                    \
         const tfh::ProfEvents pe_ = tfh::prof_take(label_);                                                          \
         if (pe_.start)                                                                                               \

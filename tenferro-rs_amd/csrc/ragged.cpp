@@ -4,8 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
-#include "ragged.hpp"
 #include "ragged_api.hpp"
+#include "ragged_thin.hpp"
 
 namespace tfh {
 namespace ragged {
@@ -190,8 +190,16 @@ int32_t combine(int32_t dtype, const tfh_row_groups* g, const tfh_view* x, const
     return e;
 }
 
-int64_t middle_row(int64_t rank) { return (rank + 3) & ~(int64_t)3; }   // rows of the middle product start 16-byte aligned
-size_t middle_bytes(int32_t dtype, int64_t n_rows, int64_t rank) { return (size_t)n_rows * middle_row(rank) * sums_size(dtype); }
+// The middle product X . A of the adapters, in scratch: rows in the sums' type, 16-byte aligned, or a pair of the operands'
+// type with a power of two per row (f16).
+int64_t wide_row(int64_t rank) { return (rank + 3) & ~(int64_t)3; }
+int64_t pair_pad(int64_t rank) { return (rank + 31) & ~(int64_t)31; }
+size_t middle_bytes(int32_t dtype, int64_t n_rows, int64_t rank) {
+    if (rank == 0) return 0;
+    if (dtype == TFH_F32 || dtype == TFH_F64) return (size_t)n_rows * wide_row(rank) * sums_size(dtype);
+    return (size_t)n_rows * pair_pad(rank) * 4 + (((size_t)n_rows * 4 + 15) & ~(size_t)15);
+}
+int middle_count(int32_t dtype, bool gradient) { return !gradient ? 1 : dtype == TFH_F32 || dtype == TFH_F64 ? 2 : 3; }
 
 struct Adapter {
     int32_t dtype;
@@ -220,21 +228,23 @@ int32_t check_adapter(Adapter& d) {
     return TFH_OK;
 }
 // V[p, :] = scales[g] * X[order[p], :] . F[g], F [K, R] by strides.
-int32_t middle(const Adapter& d, const tfh_view& x, int64_t K, const tfh_view& f, int k_axis, int r_axis, void* v, void* stream) {
+Args middle_args(const Adapter& d, const tfh_view& x, int64_t K, const tfh_view& f, int k_axis, int r_axis, void* v, bool pair) {
     Args p = base_args(*d.g);
     set_a(p, d.dtype, x);
     p.B = view_ptr(f, d.dtype);
     p.b_group = f.strides[0], p.b_k = f.strides[k_axis], p.b_n = f.strides[r_axis];
     p.C = v;
-    p.c_row = middle_row(d.R), p.c_n = 1;
+    p.pad = pair ? (int32_t)pair_pad(d.R) : 0;
+    p.c_row = pair ? 2 * p.pad : wide_row(d.R), p.c_n = 1;
+    if (pair && d.dtype == TFH_F16) p.up = (float*)((char*)v + (size_t)d.g->n_rows * p.pad * 4);
     p.N = (int32_t)d.R, p.K = (int32_t)K;
     p.gather = d.g->order != nullptr;
     if (d.scales) p.scales = view_ptr(*d.scales, d.dtype == TFH_F64 ? TFH_F64 : TFH_F32);
-    return product(d.dtype, PRODUCT_MIDDLE, p, stream);
+    return p;
 }
 // Y = X . W + V . E[g]: X [n_rows, K], W [K, N] by (w_k, w_n), E [R, N] of f by (r_axis, n_axis).
-int32_t shared(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int64_t w_k, int64_t w_n, const tfh_view& f, int r_axis,
-               int n_axis, const void* v, const tfh_view& y, void* stream) {
+Args shared_args(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int64_t w_k, int64_t w_n, const tfh_view& f, int r_axis,
+                 int n_axis, void* v, const tfh_view& y, bool pair) {
     Args p = base_args(*d.g);
     set_a(p, d.dtype, x);
     p.B = view_ptr(*d.w, d.dtype);
@@ -243,11 +253,31 @@ int32_t shared(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int64_
     p.c_row = y.strides[0], p.c_n = y.strides[1];
     p.N = (int32_t)N, p.K = (int32_t)K;
     p.gather = p.scatter = d.g->order != nullptr;
-    p.V = v, p.v_row = middle_row(d.R);
+    p.V = v;
+    p.pad = pair ? (int32_t)pair_pad(d.R) : 0;
+    p.v_row = pair ? 2 * p.pad : wide_row(d.R);
+    if (pair && d.dtype == TFH_F16) p.up = (float*)((char*)v + (size_t)d.g->n_rows * p.pad * 4);
     p.E = view_ptr(f, d.dtype);
     p.e_group = f.strides[0], p.e_k = f.strides[r_axis], p.e_n = f.strides[n_axis];
     p.r = (int32_t)d.R;
-    return product(d.dtype, PRODUCT_SHARED, p, stream);
+    return p;
+}
+// Whether the two are done by the kernels that keep the middle as a pair.
+bool by_pair(int32_t dtype, const Args& middle, const Args& shared) {
+    if (dtype != TFH_BF16 && dtype != TFH_F16) return false;
+    return thin_takes(middle, !(middle.b_n == 1 && middle.b_k != 1)) && fast_takes<SHARED>(shared, !(shared.b_n == 1 && shared.b_k != 1));
+}
+// Y = X . W + scales (X . F[g]) . E[g]; `v`: scratch, left as a pair or as sums (`*pair`).
+int32_t both(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int64_t w_k, int64_t w_n, const tfh_view& f, int f_k, int f_r, const tfh_view& e,
+             int e_r, int e_n, void* v, const tfh_view& y, bool* pair, void* stream) {
+    *pair = false;
+    if (d.R > 0) {
+        Args m = middle_args(d, x, K, f, f_k, f_r, v, true), s = shared_args(d, x, K, N, w_k, w_n, e, e_r, e_n, v, y, true);
+        *pair = by_pair(d.dtype, m, s);
+    }
+    if (d.R > 0)
+        if (int32_t err = product(d.dtype, PRODUCT_MIDDLE, middle_args(d, x, K, f, f_k, f_r, v, *pair), stream)) return err;
+    return product(d.dtype, PRODUCT_SHARED, shared_args(d, x, K, N, w_k, w_n, e, e_r, e_n, v, y, *pair), stream);
 }
 
 int32_t adapter_gemm(Adapter d, const tfh_view* y, void* workspace, size_t workspace_bytes, void* stream) {
@@ -255,9 +285,33 @@ int32_t adapter_gemm(Adapter d, const tfh_view* y, void* workspace, size_t works
     if (int32_t e = check_view("Y", y, {d.g->n_rows, d.N}, true)) return e;
     if (int32_t e = check_workspace(workspace, workspace_bytes, middle_bytes(d.dtype, d.g->n_rows, d.R))) return e;
     if (d.g->n_rows == 0 || d.N == 0) return TFH_OK;
-    if (d.R)
-        if (int32_t e = middle(d, *d.x, d.K, *d.a, 1, 2, workspace, stream)) return e;
-    return shared(d, *d.x, d.K, d.N, d.w->strides[0], d.w->strides[1], *d.b, 1, 2, workspace, *y, stream);
+    bool pair;
+    return both(d, *d.x, d.K, d.N, d.w->strides[0], d.w->strides[1], *d.a, 1, 2, *d.b, 1, 2, workspace, *y, &pair, stream);
+}
+
+// A factor's gradient: G[g] = sum over the group's rows of X[order[p], :]^T . V[p, :] with V = scales Z[order[p], :] . F[g], in
+// the view `grad` by (x_axis, r_axis).  `have`: V from before, as a pair or as sums; null or of the other form: it is made
+// again, in `spare`.  A pair in bf16; f16's pairs carry a factor for each row, for which a sum over rows has no place.
+int32_t factor_gradient(const Adapter& d, const tfh_view& x, int64_t K, const tfh_view& z, int64_t KZ, const tfh_view& f, int f_k, int f_r,
+                        const tfh_view& grad, int x_axis, int r_axis, void* have, bool have_pair, void* spare, void* stream) {
+    Args p = base_args(*d.g);
+    set_a(p, d.dtype, x);
+    p.gather = d.g->order != nullptr;
+    p.b_rows = d.g->n_rows;
+    p.C = view_ptr(grad, d.dtype), p.c_group = grad.strides[0], p.c_row = grad.strides[x_axis], p.c_n = grad.strides[r_axis];
+    p.M = (int32_t)K, p.r = (int32_t)d.R;
+    p.b_n = 1;
+    Args q = p;
+    q.pad = (int32_t)pair_pad(d.R), q.N = 2 * q.pad, q.b_k = 2 * q.pad, q.B = spare;
+    p.N = (int32_t)d.R, p.b_k = wide_row(d.R);
+    const Args as_pair = middle_args(d, z, KZ, f, f_k, f_r, spare, true);
+    const bool pair = d.dtype == TFH_BF16 && fast_takes<PAIR>(q, false) && thin_takes(as_pair, !(as_pair.b_n == 1 && as_pair.b_k != 1));
+    void* v = have && have_pair == pair ? have : spare;
+    if (v == spare && d.g->n_rows)
+        if (int32_t e = product(d.dtype, PRODUCT_MIDDLE, pair ? as_pair : middle_args(d, z, KZ, f, f_k, f_r, spare, false), stream)) return e;
+    Args& out = pair ? q : p;
+    out.B = v;
+    return product(d.dtype, PRODUCT_OUTER_V, out, stream);
 }
 
 int32_t adapter_gemm_grad(Adapter d, const tfh_view* dy, const tfh_view* dx, const tfh_view* da, const tfh_view* db, void* workspace,
@@ -272,33 +326,18 @@ int32_t adapter_gemm_grad(Adapter d, const tfh_view* dy, const tfh_view* dx, con
     if (db)
         if (int32_t e = check_view("dB", db, {d.g->n_groups, d.R, d.N}, true)) return e;
     const size_t each = middle_bytes(d.dtype, rows, d.R);
-    if (int32_t e = check_workspace(workspace, workspace_bytes, 2 * each)) return e;
-    char* const v = (char*)workspace;
-    char* const u = v + each;   // (rows of 16 bytes: aligned)
-    if (rows && d.R && (dx || da))
-        if (int32_t e = middle(d, *dy, d.N, *d.b, 2, 1, u, stream)) return e;
-    if (rows && dx && d.K)
-        if (int32_t e = shared(d, *dy, d.N, d.K, d.w->strides[1], d.w->strides[0], *d.a, 2, 1, u, *dx, stream)) return e;
-    if (da && d.K && d.R) {   // X_g^T . U_g
-        Args p = base_args(*d.g);
-        set_a(p, d.dtype, *d.x);
-        p.gather = d.g->order != nullptr;
-        p.B = u, p.b_rows = rows, p.b_k = middle_row(d.R), p.b_n = 1;
-        p.C = view_ptr(*da, d.dtype), p.c_group = da->strides[0], p.c_row = da->strides[1], p.c_n = da->strides[2];
-        p.M = (int32_t)d.K, p.N = (int32_t)d.R;
-        if (int32_t e = product(d.dtype, PRODUCT_OUTER_V, p, stream)) return e;
+    if (int32_t e = check_workspace(workspace, workspace_bytes, each * middle_count(d.dtype, true))) return e;
+    char* const u = (char*)workspace;
+    bool pair = false, made = false;
+    if (rows && dx && d.K) {
+        if (int32_t e = both(d, *dy, d.N, d.K, d.w->strides[1], d.w->strides[0], *d.b, 2, 1, *d.a, 2, 1, u, *dx, &pair, stream)) return e;
+        made = true;
     }
-    if (db && d.N && d.R) {   // V_g^T . dY_g
-        if (rows)
-            if (int32_t e = middle(d, *d.x, d.K, *d.a, 1, 2, v, stream)) return e;
-        Args p = base_args(*d.g);
-        p.A = v, p.a_rows = rows, p.a_row = middle_row(d.R), p.a_col = 1;
-        p.B = view_ptr(*dy, d.dtype), p.b_rows = rows, p.b_k = dy->strides[0], p.b_n = dy->strides[1];
-        p.gather_b = d.g->order != nullptr;
-        p.C = view_ptr(*db, d.dtype), p.c_group = db->strides[0], p.c_row = db->strides[1], p.c_n = db->strides[2];
-        p.M = (int32_t)d.R, p.N = (int32_t)d.N;
-        if (int32_t e = product(d.dtype, PRODUCT_V_OUTER, p, stream)) return e;
-    }
+    if (d.R == 0) return TFH_OK;
+    if (da && d.K)
+        if (int32_t e = factor_gradient(d, *d.x, d.K, *dy, d.N, *d.b, 2, 1, *da, 1, 2, made ? u : nullptr, pair, u + each, stream)) return e;
+    if (db && d.N)
+        if (int32_t e = factor_gradient(d, *dy, d.N, *d.x, d.K, *d.a, 1, 2, *db, 2, 1, nullptr, false, u + (middle_count(d.dtype, true) - 1) * each, stream)) return e;
     return TFH_OK;
 }
 
@@ -379,7 +418,7 @@ int32_t tfh_combine_rows_grad(int32_t dtype, const tfh_row_groups* groups, const
 }
 size_t tfh_adapter_workspace(int32_t dtype, int64_t n_rows, int64_t rank, int32_t gradient) {
     return !ragged::known(dtype) || n_rows < 0 || rank < 0 || n_rows > ragged::MOST || rank > ragged::MOST ? 0
-           : ragged::middle_bytes(dtype, n_rows, rank) * (gradient ? 2 : 1);
+           : ragged::middle_bytes(dtype, n_rows, rank) * ragged::middle_count(dtype, gradient != 0);
 }
 int32_t tfh_adapter_gemm(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* w, const tfh_view* a,
                          const tfh_view* b, const tfh_view* scales, const tfh_view* y, void* workspace, size_t workspace_bytes,

@@ -95,16 +95,17 @@ struct Args {
     int32_t zero_rest;        // rows: the rows behind the last group are written as zeros, else left alone
     int32_t use_beta;
     double alpha, beta;
-    int32_t gather_b;         // outer: B's row of p is order[p], else p
-    // shared: the low-rank part, V[p, 0 .. r) (of the accumulators' type) against E[g, j, n]; rows of no group are without it
+    // shared: the low-rank part, V[p, 0 .. r) against E[g, j, n]; rows of no group are without it.  V is of the sums' type, or
+    // (pad > 0) a pair of the operands' type: row p is hi[0 .. pad), lo[0 .. pad), V = up[p] (hi + lo), zeros from r on
     const void* V;
     const void* E;
     int64_t v_row, e_group, e_k, e_n;
-    int32_t r;
+    int32_t r, pad;
+    float* up;                // f16: the power of two by which row p was scaled down; null: 1 (written with V, read with it)
     const void* scales;       // rows: factors of the groups' results (of the accumulators' type) beside alpha, or null
 };
 
-enum Mode { ROWS = 0, OUTER = 1, SHARED = 2 };
+enum Mode { ROWS = 0, OUTER = 1, SHARED = 2, PAIR = 3 };   // PAIR: outer with a pair of V's form for B (ragged_fast.hpp)
 
 // E elements of type C from a row of S that starts at any element: `count` of them are there, the others read as zeros.
 template <class S, class C>
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                 int64_t s = k;
                 if constexpr (MODE == OUTER) {
                     s = -1;
-                    if (k < kend) s = a.gather_b && a.order ? a.order[t.first + k] : t.first + k;
+                    if (k < kend) s = t.first + k;
                     if (s >= a.b_rows) s = -1;
                 }
                 rb[i] = load_chunk<TB, C>(B + s * a.b_k + n * a.b_n, a.b_n, k < kend && s >= 0 ? a.N - n : 0);

@@ -49,9 +49,8 @@ enum Kind {
     PRODUCT_ROWS,      // rows in, rows out, all of the type
     PRODUCT_OUTER,     // a group's rows summed over, all of the type
     PRODUCT_SHARED,    // one matrix for all rows and a low-rank part by group
-    PRODUCT_MIDDLE,    // rows in, rows out in the sums' type
-    PRODUCT_OUTER_V,   // A of the type, B of the sums' type
-    PRODUCT_V_OUTER    // A of the sums' type, B of the type
+    PRODUCT_MIDDLE,    // rows in, rows out in the sums' type or as a pair (Args::pad)
+    PRODUCT_OUTER_V    // a group's rows summed over, B what PRODUCT_MIDDLE has written
 };
 int32_t launch_bf16(int kind, const Args& a, void* stream);
 int32_t launch_f16(int kind, const Args& a, void* stream);

@@ -3,6 +3,7 @@
 #include "launch.hpp"
 #include "ragged.hpp"
 #include "ragged_fast.hpp"
+#include "ragged_thin.hpp"
 #include "ragged_api.hpp"
 
 namespace tfh {
@@ -15,6 +16,15 @@ inline int64_t row_tiles(const Args& a, int tm) {
     return a.n_rows / tm + (groups < a.n_rows ? groups : a.n_rows);
 }
 
+// "(kernel<arguments>)" as tfh_last_kernel spells them.
+template <class T> constexpr const char* type_name() {
+    if constexpr (__is_same(T, __bf16)) return "bf16";
+    else if constexpr (__is_same(T, _Float16)) return "f16";
+    else if constexpr (__is_same(T, float)) return "float";
+    else return "double";
+}
+constexpr const char* mode_name(int mode) { return mode == ROWS ? "rows" : mode == OUTER ? "outer" : mode == SHARED ? "shared" : "pair"; }
+
 template <class TA, class TB, class C, class TO, int MODE, bool BKFAST>
 int32_t launch_general(const Args& a, void* stream) {
     constexpr int XT = 2, YT = 2;
@@ -23,15 +33,17 @@ int32_t launch_general(const Args& a, void* stream) {
                            : MODE == OUTER ? a.n_groups * tiles(a.M, 32 * XT) * tn : tiles(a.n_rows, 32 * XT) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
-    TFH_LAUNCH_TIMED((ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, XT, YT>), dim3((unsigned)blocks), dim3(GENERAL_THREADS), 0, (hipStream_t)stream, a);
+    static const std::string label = std::string("(ragged_general_kernel<") + type_name<TA>() + ", " + type_name<TB>() + ", " + type_name<C>() + ", " +
+                                     type_name<TO>() + ", " + mode_name(MODE) + (BKFAST ? ", k>)" : ", n>)");
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, XT, YT>), dim3((unsigned)blocks), dim3(GENERAL_THREADS), 0, (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 
 template <class T, int MODE, bool BKFAST, class S>
 int32_t launch_fast(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, S::TN);
-    const int64_t blocks = MODE == ROWS ? row_tiles(a, S::TM) * tn
-                           : MODE == OUTER ? a.n_groups * tiles(a.M, S::TM) * tn : tiles(a.n_rows, S::TM) * tn;
+    const int64_t blocks = MODE == ROWS || (MODE == SHARED && S::BY_GROUP) ? row_tiles(a, S::TM) * tn
+                           : MODE == OUTER || MODE == PAIR ? a.n_groups * tiles(a.M, S::TM) * tn : tiles(a.n_rows, S::TM) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
     static const bool once = [] {
@@ -39,7 +51,9 @@ int32_t launch_fast(const Args& a, void* stream) {
         return true;
     }();
     (void)once;
-    TFH_LAUNCH_TIMED((ragged_fast_kernel<T, MODE, BKFAST, S>), dim3((unsigned)blocks), dim3(256), S::LDS, (hipStream_t)stream, a);
+    static const std::string label = std::string("(ragged_fast_kernel<") + type_name<T>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") +
+                                     std::to_string(S::TM) + "x" + std::to_string(S::TN) + ">)";
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_fast_kernel<T, MODE, BKFAST, S>), dim3((unsigned)blocks), dim3(256), S::LDS, (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 typedef Shape<2, 2, 4, 4> Large;    // 256 x 256
@@ -52,6 +66,31 @@ int32_t launch_shape(const Args& a, void* stream) {
     if (rows > 48) return launch_fast<T, MODE, BKFAST, Middle>(a, stream);
     return launch_fast<T, MODE, BKFAST, Small>(a, stream);
 }
+template <class T, bool BKFAST>
+int32_t launch_shared(const Args& a, void* stream) {
+    // tiles by group read W once for each group's rows; worth it where they fill most of a tile.  (f16 scales its rows'
+    // low-rank part back before the rest is added, which the large tile's one loop has no place for.)
+    if constexpr (__is_same(T, __bf16))
+        if (a.n_rows / (a.n_groups + 1) > 192) {
+            Args g = a;
+            g.zero_rest = 1;
+            return launch_fast<T, SHARED, BKFAST, Large>(g, stream);
+        }
+    return launch_fast<T, SHARED, BKFAST, Middle>(a, stream);
+}
+template <class T, bool BKFAST, int YT>
+int32_t launch_thin(const Args& a, void* stream) {
+    const int64_t blocks = row_tiles(a, THIN_ROWS);
+    if (blocks <= 0) return TFH_OK;
+    static const bool once = [] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT>), hipFuncAttributeMaxDynamicSharedMemorySize, thin_lds<T, BKFAST, YT>());
+        return true;
+    }();
+    (void)once;
+    static const std::string label = std::string("(ragged_thin_kernel<") + type_name<T>() + (BKFAST ? ", k, " : ", n, ") + std::to_string(32 * YT) + ">)";
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT>), dim3((unsigned)blocks), dim3(64 * THIN_WAVES), (thin_lds<T, BKFAST, YT>()), (hipStream_t)stream, a);
+    return hip_check(hipGetLastError(), "product over groups of rows");
+}
 
 template <class T> int32_t launch_product(int kind, const Args& a, void* stream) {
     typedef typename Num<T>::acc W;
@@ -61,14 +100,19 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         if (kind == PRODUCT_ROWS && fast_takes<ROWS>(a, !columns))
             return columns ? launch_shape<T, ROWS, false>(a, stream) : launch_shape<T, ROWS, true>(a, stream);
         if (kind == PRODUCT_OUTER && fast_takes<OUTER>(a, false)) return launch_shape<T, OUTER, false>(a, stream);
+        if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_shared<T, false>(a, stream) : launch_shared<T, true>(a, stream);
+        if (kind == PRODUCT_OUTER_V && a.pad > 0) return launch_fast<T, PAIR, false, Middle>(a, stream);
+        if (kind == PRODUCT_MIDDLE && thin_takes(a, !columns)) {
+            if (columns) return a.N <= 32 ? launch_thin<T, false, 1>(a, stream) : a.N <= 64 ? launch_thin<T, false, 2>(a, stream) : launch_thin<T, false, 4>(a, stream);
+            return a.N <= 32 ? launch_thin<T, true, 1>(a, stream) : a.N <= 64 ? launch_thin<T, true, 2>(a, stream) : launch_thin<T, true, 4>(a, stream);
+        }
     }
     switch (kind) {
         case PRODUCT_ROWS: return columns ? launch_general<T, T, T, T, ROWS, false>(a, stream) : launch_general<T, T, T, T, ROWS, true>(a, stream);
         case PRODUCT_MIDDLE: return columns ? launch_general<T, T, T, W, ROWS, false>(a, stream) : launch_general<T, T, T, W, ROWS, true>(a, stream);
         case PRODUCT_SHARED: return columns ? launch_general<T, T, T, T, SHARED, false>(a, stream) : launch_general<T, T, T, T, SHARED, true>(a, stream);
         case PRODUCT_OUTER: return launch_general<T, T, T, T, OUTER, false>(a, stream);
-        case PRODUCT_OUTER_V: return launch_general<T, W, W, T, OUTER, false>(a, stream);
-        default: return launch_general<W, T, W, T, OUTER, false>(a, stream);
+        default: return launch_general<T, W, W, T, OUTER, false>(a, stream);
     }
 }
 

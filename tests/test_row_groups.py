@@ -414,7 +414,8 @@ def adapter_reference(torch, x, w, a, b, scales, ids):
     return y, size + low, low
 
 
-ADAPTERS = [(1, 1, 1, 1, 1), (1, 3, 64, 40, 4), (5, 2, 33, 17, 7), (64, 32, 136, 200, 16), (100, 3, 72, 65, 24), (200, 4, 256, 130, 50), (130, 64, 96, 128, 100), (20, 2, 64, 64, 200)]
+ADAPTERS = [(1, 1, 1, 1, 1), (1, 3, 64, 40, 4), (5, 2, 33, 17, 7), (64, 32, 136, 200, 16), (100, 3, 72, 65, 24), (200, 4, 256, 130, 50), (130, 64, 96, 128, 100), (20, 2, 64, 64, 200),
+            (900, 3, 128, 320, 32), (700, 2, 192, 264, 64), (300, 5, 72, 136, 128), (450, 1, 64, 256, 8)]
 
 
 @pytest.mark.gpu
@@ -705,9 +706,9 @@ def test_adapters_refuse_what_does_not_fit(tf):
     refused(tf, run(s=V(4)), tf.ShapeMismatch)
     refused(tf, run(s=V(3, strides=[2])), tf.Strided)
     refused(tf, run(ws=None), tf.InvalidArgument)
-    refused(tf, run(nb=8 * 4 * 4 - 1), tf.InvalidArgument)
+    refused(tf, run(nb=L.tfh_adapter_workspace(4, 8, 4, 0) - 1), tf.InvalidArgument)
     refused(tf, run(ws=4104), tf.InvalidArgument)
-    assert L.tfh_adapter_workspace(4, 8, 4, 0) == 8 * 4 * 4
+    assert L.tfh_adapter_workspace(4, 8, 4, 1) > L.tfh_adapter_workspace(4, 8, 4, 0) >= 8 * 4 * 4 and L.tfh_adapter_workspace(4, 8, 0, 1) == 0
     refused(tf, L.tfh_adapter_gemm_grad(4, G(), ok["x"], ok["w"], ok["a"], ok["b"], None, V(8, 24), None, V(3, 16, 5), None, 4096, 1 << 20, None), tf.ShapeMismatch)
 
 
