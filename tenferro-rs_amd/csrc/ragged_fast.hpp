@@ -69,38 +69,15 @@ template <int WM_, int WN_, int XT_, int YT_> struct Shape {
     static constexpr int BLOCKS = XT * YT > 8 ? 1 : 2;   // of a CU: registers and LDS leave room for so many
 };
 
-template <class T, int MODE, bool BKFAST, class S>
-__global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args a) {
+// One tile: its k loop and its results.  BY_GROUP: its rows are of one group (of none: t.group == a.n_groups).
+template <class T, int MODE, bool BKFAST, class S, bool BY_GROUP>
+__device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* lds) {
     static_assert(sizeof(T) == 2, "16-bit operands");
     constexpr int XT = S::XT, YT = S::YT, TM = S::TM, TN = S::TN, BK = 64, STAGE = S::STAGE;
     constexpr int CA = TM / 32, CB = TN / 32;      // chunks of each operand per thread and stage
     constexpr bool OUT = MODE == OUTER || MODE == PAIR, AKFAST = !OUT;
-    // shared mode: large tiles belong to one group each (the host sets zero_rest: the rows of no group are one more), small
-    // ones span as many as their rows are of, so that few rows of many groups do not read W once for each
-    constexpr bool BY_GROUP = MODE == ROWS || (MODE == SHARED && S::BY_GROUP);
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    char* const lds = (char*)smem_raw;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % S::WM, wn = wave / S::WM;
-    const int tiles_n = (a.N + TN - 1) / TN;
-    Tile t;
-    if constexpr (BY_GROUP) {
-        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
-    } else if constexpr (OUT) {
-        const int tiles_m = (a.M + TM - 1) / TM;
-        const uint32_t id = (uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), each = (uint32_t)tiles_m * tiles_n;
-        t.group = (int)(id / each);
-        gemm::tile_of(id % each, tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows));
-        const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group + 1], a.n_rows));
-        t.rows = to > t.first ? to - t.first : 0;
-    } else {
-        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
-        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.group = 0;
-        t.first = t.tile_m * TM;
-        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
-    }
     const bool real = MODE != ROWS || t.group < a.n_groups;
     const int n0 = t.tile_n * TN, m0 = t.tile_m * TM;
     f32x16 acc[XT][YT];
@@ -440,6 +417,50 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
         if (most_n - n >= 8) __builtin_memcpy(c, &v, 16);
         else __builtin_memcpy(c, &v, 8);
     }
+}
+
+template <class T, int MODE, bool BKFAST, class S>
+__global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args a) {
+    // shared mode: large tiles belong to one group each (the host sets zero_rest: the rows of no group are one more), small
+    // ones span as many as their rows are of, so that few rows of many groups do not read W once for each
+    constexpr bool BY_GROUP = MODE == ROWS || (MODE == SHARED && S::BY_GROUP);
+    constexpr int TM = S::TM, TN = S::TN;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    char* const lds = (char*)smem_raw;
+    const int tiles_n = (a.N + TN - 1) / TN;
+    Tile t;
+    if constexpr (BY_GROUP) {
+        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+        if constexpr (TM == 256) {
+            // a group's last tile is seldom full: half or a quarter of the rows in half or 0.4 of the time
+            typedef Shape<1, 4, 2, 2> Quarter;
+            typedef Shape<2, 2, 2, 4> Half;
+            static_assert(Quarter::TN == TN && Half::TN == TN && Half::LDS <= S::LDS, "the same columns");
+            if (t.rows <= 64) {
+                fast_tile<T, MODE, BKFAST, Quarter, true>(a, t, lds);
+                return;
+            }
+            if (t.rows <= 128) {
+                fast_tile<T, MODE, BKFAST, Half, true>(a, t, lds);
+                return;
+            }
+        }
+    } else if constexpr (MODE == OUTER || MODE == PAIR) {
+        const int tiles_m = (a.M + TM - 1) / TM;
+        const uint32_t id = (uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), each = (uint32_t)tiles_m * tiles_n;
+        t.group = (int)(id / each);
+        gemm::tile_of(id % each, tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows));
+        const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group + 1], a.n_rows));
+        t.rows = to > t.first ? to - t.first : 0;
+    } else {
+        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
+        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
+        t.group = 0;
+        t.first = t.tile_m * TM;
+        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
+    }
+    fast_tile<T, MODE, BKFAST, S, BY_GROUP>(a, t, lds);
 }
 
 // Whether the kernel can take a call: rows that start 16-byte aligned and end with a chunk, spans that 32 bits address.

@@ -3,6 +3,7 @@
 #include "launch.hpp"
 #include "ragged.hpp"
 #include "ragged_fast.hpp"
+#include "ragged_few.hpp"
 #include "ragged_thin.hpp"
 #include "ragged_api.hpp"
 
@@ -78,6 +79,19 @@ int32_t launch_shared(const Args& a, void* stream) {
         }
     return launch_fast<T, SHARED, BKFAST, Middle>(a, stream);
 }
+template <class T, int MODE, int TR, int STEPS>
+int32_t launch_few_steps(const Args& a, void* stream) {
+    const int64_t blocks = (MODE == ROWS ? row_tiles(a, 16 * TR) : tiles(a.n_rows, 16 * TR)) * tiles(a.N, 16);
+    if (blocks <= 0) return TFH_OK;
+    if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
+    static const std::string label = std::string("(ragged_few_kernel<") + type_name<T>() + ", " + mode_name(MODE) + ", " + std::to_string(16 * TR) + ">)";
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR, STEPS>), dim3((unsigned)blocks), dim3(64 * FEW_WAVES), 0, (hipStream_t)stream, a);
+    return hip_check(hipGetLastError(), "product over groups of rows");
+}
+template <class T, int MODE, int TR>
+int32_t launch_few(const Args& a, void* stream) {
+    return a.K <= 4 * 32 * FEW_WAVES ? launch_few_steps<T, MODE, TR, 4>(a, stream) : launch_few_steps<T, MODE, TR, 16>(a, stream);
+}
 template <class T, bool BKFAST, int YT>
 int32_t launch_thin(const Args& a, void* stream) {
     const int64_t blocks = row_tiles(a, THIN_ROWS);
@@ -100,6 +114,9 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         if (kind == PRODUCT_ROWS && fast_takes<ROWS>(a, !columns))
             return columns ? launch_shape<T, ROWS, false>(a, stream) : launch_shape<T, ROWS, true>(a, stream);
         if (kind == PRODUCT_OUTER && fast_takes<OUTER>(a, false)) return launch_shape<T, OUTER, false>(a, stream);
+        if (kind == PRODUCT_SHARED && a.pad > 0 && a.n_rows <= 128 && !columns && few_takes<SHARED>(a))
+            return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream)
+                   : a.n_rows <= 64 ? launch_few<T, SHARED, 4>(a, stream) : launch_few<T, SHARED, 8>(a, stream);
         if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_shared<T, false>(a, stream) : launch_shared<T, true>(a, stream);
         if (kind == PRODUCT_OUTER_V && a.pad > 0) return launch_fast<T, PAIR, false, Middle>(a, stream);
         if (kind == PRODUCT_MIDDLE && thin_takes(a, !columns)) {

@@ -51,7 +51,7 @@ __device__ __forceinline__ void store_pair(const Args& a, int64_t p, const float
 template <class T, bool BKFAST, int YT> constexpr int thin_lds() { return THIN_WAVES * THIN_ROWS * 32 * YT * 4; }
 
 template <class T, bool BKFAST, int YT>
-__global__ __launch_bounds__(64 * THIN_WAVES, 2) void ragged_thin_kernel(const Args a) {
+__global__ __launch_bounds__(64 * THIN_WAVES, 1) void ragged_thin_kernel(const Args a) {
     constexpr int TN = 32 * YT, RB = TN / 8;   // RB: chunks of a row of k of F
     extern __shared__ __align__(16) unsigned char smem_raw[];
     char* const lds = (char*)smem_raw;
@@ -73,12 +73,13 @@ __global__ __launch_bounds__(64 * THIN_WAVES, 2) void ragged_thin_kernel(const A
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[y][r] = 0;
     // a step: 64 k's, 16 for each h; lane (row, half) has chunk 2 h + half of its row
-    u32x4 na[4], nb[4 * YT];
-    auto load = [&](int k0) {
+    constexpr int AHEAD = YT == 1 ? 4 : YT == 2 ? 2 : 1;   // steps whose loads are in flight, by the registers they take
+    u32x4 na[AHEAD][4], nb[AHEAD][4 * YT];
+    auto load = [&](int k0, u32x4 (&la)[4], u32x4 (&lb)[4 * YT]) {
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
             const int k = k0 + 16 * h + 8 * half;
-            na[h] = __builtin_amdgcn_raw_buffer_load_b128(A, k < a.K && va != NOWHERE ? va + k * 2 : NOWHERE, 0, 0);
+            la[h] = __builtin_amdgcn_raw_buffer_load_b128(A, k < a.K && va != NOWHERE ? va + k * 2 : NOWHERE, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 4 * YT; ++i) {
@@ -90,34 +91,38 @@ __global__ __launch_bounds__(64 * THIN_WAVES, 2) void ragged_thin_kernel(const A
                 const int id = lane + 64 * i, k = k0 + id / RB, n = (id % RB) * 8;
                 v = k < a.K && n < a.N ? (uint32_t)(k * a.b_k * 2) + n * 2 : NOWHERE;
             }
-            nb[i] = __builtin_amdgcn_raw_buffer_load_b128(B, v, 0, 0);
+            lb[i] = __builtin_amdgcn_raw_buffer_load_b128(B, v, 0, 0);
         }
     };
     char* const mine = lds + wave * (64 * TN * 2);   // row-fast F: this wave's own tile, to be read across
-    int k0 = wave * 64;
-    if (k0 < a.K) load(k0);
-    for (; k0 < a.K; k0 += 64 * THIN_WAVES) {
-        u32x4 fa[4], fb[4 * YT];
+    constexpr int STRIDE = 64 * THIN_WAVES;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) fa[h] = na[h];
+    for (int d = 0; d < AHEAD; ++d) load(wave * 64 + d * STRIDE, na[d], nb[d]);   // (beyond K: zeros)
+    for (int k0 = wave * 64; k0 < a.K; k0 += AHEAD * STRIDE) {
 #pragma unroll
-        for (int i = 0; i < 4 * YT; ++i) fb[i] = nb[i];
-        if (k0 + 64 * THIN_WAVES < a.K) load(k0 + 64 * THIN_WAVES);
-        if constexpr (!BKFAST) {
+        for (int d = 0; d < AHEAD; ++d) {
+            u32x4 fa[4], fb[4 * YT];
 #pragma unroll
-            for (int i = 0; i < 4 * YT; ++i) {
-                const int id = lane + 64 * i;
-                *(u32x4*)(mine + rowfast_at<T, TN>(id / RB, id % RB)) = fb[i];
+            for (int h = 0; h < 4; ++h) fa[h] = na[d][h];
+#pragma unroll
+            for (int i = 0; i < 4 * YT; ++i) fb[i] = nb[d][i];
+            load(k0 + (d + AHEAD) * STRIDE, na[d], nb[d]);
+            if constexpr (!BKFAST) {
+#pragma unroll
+                for (int i = 0; i < 4 * YT; ++i) {
+                    const int id = lane + 64 * i;
+                    *(u32x4*)(mine + rowfast_at<T, TN>(id / RB, id % RB)) = fb[i];
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < 4 * YT; ++i) fb[i] = fragment32<T, TN, false>(mine, (i % YT) * 32, i / YT, lane);
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < 4 * YT; ++i) fb[i] = fragment32<T, TN, false>(mine, (i % YT) * 32, i / YT, lane);
-            __builtin_amdgcn_wave_barrier();
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int y = 0; y < YT; ++y) acc[y] = mma32<T>(fb[h * YT + y], fa[h], acc[y]);
         }
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int y = 0; y < YT; ++y) acc[y] = mma32<T>(fb[h * YT + y], fa[h], acc[y]);
     }
     // the waves' sums, in the order of the waves
     __syncthreads();
