@@ -2,26 +2,37 @@
 // LDS as ragged.hpp, but written there by the memory system itself (buffer loads with LDS as their destination, 16 bytes a
 // lane, no registers in between), double-buffered, and a register pipeline in front of the matrix cores.
 //
-// Per stage (128 bytes of k of every row, two halves of 64) and wave:
-//   first half's products   while the second half's fragments are read from LDS
-//   wait: the fragments are here, the next stage's loads have landed; barrier: so they have for every wave, and this
-//         stage's buffer has been read by all
-//   second half's products  while the loads of the stage after the next are issued into this stage's buffer and the next
-//                           stage's first fragments are read
-// so a load has most of a stage's products to arrive in, a fragment half a stage, and there is one barrier per stage.
+// Per stage (64 or 128 bytes of k of every row) and wave, 16 k's at a time:
+//   their products          while the fragments of the next 16 are read from LDS
+//   before the last 16:     wait until those fragments are here and the next stage's loads have landed; barrier: so they
+//                           have for every wave, and this stage's slot has been read by all
+//   the last 16's products  while a later stage's loads are issued into this stage's slot and the next stage's first
+//                           fragments are read
+// so a fragment has 16 k's products to arrive in, a load those of all slots but one, and there is one barrier per stage.
 #pragma once
+#include <utility>
+
 #include "ragged.hpp"
 
 namespace tfh {
 namespace ragged {
 
+// A scalar operand of the loads below.  A vector instruction's write of a scalar register (readfirstlane is one) must lie
+// five wait states before a load that reads it; the compiler sees to that for its own loads, not for those in asm.  Moved
+// here by the scalar unit, which waits for it, the value is one that a load may read at once.  (A spilled scalar register
+// would come back through a vector instruction: the kernels that use these loads have to be built without scalar spills.)
+__device__ __forceinline__ uint32_t scalar_of(uint32_t v) {
+    uint32_t s;
+    asm("s_mov_b32 %0, %1" : "=s"(s) : "s"(__builtin_amdgcn_readfirstlane(v)));
+    return s;
+}
 // A buffer of `bytes` bytes from `base`: a load whose offset lies beyond reads zeros.
 __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
     const uint64_t p = (uint64_t)base;
     u32x4 r;
-    r[0] = __builtin_amdgcn_readfirstlane((uint32_t)p);
-    r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32) & 0xffff);
-    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[0] = scalar_of((uint32_t)p);
+    r[1] = scalar_of((uint32_t)(p >> 32) & 0xffff);
+    r[2] = scalar_of(bytes);
     r[3] = 0x00020000;
     return r;
 }
@@ -31,8 +42,15 @@ constexpr int64_t MOST_SPAN = 0xffff0000ll;
 // 16 bytes a lane from buffer + offset + scalar into LDS at `to` + 16 * lane.  The compiler does not count these loads:
 // wait_loads() does, before anything they write is read.
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t scalar, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(buffer), "s"(scalar) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(buffer), "s"(scalar) : "memory");
 }
+// The same in two parts, with one instruction at least in between: where the chunk goes, and the load.
+template <int AT> __device__ __forceinline__ void load_goes_to(uint32_t base) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(base), "n"(AT) : "memory", "scc"); }
+__device__ __forceinline__ void load_there(u32x4 buffer, uint32_t offset, uint32_t scalar) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(offset), "s"(buffer), "s"(scalar) : "memory");
+}
+template <class F, int... I> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F> __device__ __forceinline__ void unrolled(F f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 template <int LEFT> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void wait_fragments_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -44,11 +62,15 @@ template <class T> __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32
     if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// The 16 k's h = 0 .. 3 of a stage for 32 rows from `row`.
-template <class T, int TM, bool KFAST>
+// A k-fast tile with KB = 64 or 128 bytes of k for each row: where a chunk lies, so that any eight consecutive rows' same
+// chunk fills the banks once.
+template <int KB> __device__ __forceinline__ uint32_t turn(uint32_t row) { return KB == 128 ? row & 7 : (row >> 1) & 3; }
+template <int KB> __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t chunk) { return row * KB + ((chunk ^ turn<KB>(row)) << 4); }
+// The 16 k's h of a stage for 32 rows from `row`.
+template <class T, int TM, bool KFAST, int KB = 128>
 __device__ __forceinline__ u32x4 fragment32(const char* tile, int row, int h, int lane) {
     if constexpr (KFAST) {
-        return *(const u32x4*)(tile + kfast_at<T>(row + (lane & 31), 2 * h + (lane >> 5)));
+        return *(const u32x4*)(tile + chunk_at<KB>(row + (lane & 31), 2 * h + (lane >> 5)));
     } else {
         typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
         const int j = lane & 15, k = 16 * h + 8 * (lane >> 5) + (j >> 2), col = row + (lane & 16) + 4 * (j & 3);
@@ -60,11 +82,17 @@ __device__ __forceinline__ u32x4 fragment32(const char* tile, int row, int h, in
     }
 }
 
-// The shape of a block: WM x WN = 4 waves of 32 XT x 32 YT results.
-template <int WM_, int WN_, int XT_, int YT_> struct Shape {
+// The shape of a block: WM x WN = 4 waves of 32 XT x 32 YT results; KB bytes of k of each row are a stage, SA stages of the
+// first operand and SB of the second are in LDS or on their way to it.
+//
+// A k-fast tile wants KB = 128: its loads then ask for whole lines, and 64-byte pieces cost L2 as much each (256 x 256 tiles
+// need 13 TB/s of it).  That leaves room in LDS for five tiles, three of one operand and two of the other; the other's loads
+// go first after the barrier.  Row-fast tiles ask for whole rows of columns anyway and take KB = 64, five stages of both.
+template <int WM_, int WN_, int XT_, int YT_, int KB_ = 128, int SA_ = 2, int SB_ = 2> struct Shape {
     static_assert(WM_ * WN_ == 4, "four waves");
-    static constexpr int WM = WM_, WN = WN_, XT = XT_, YT = YT_, TM = 32 * WM * XT, TN = 32 * WN * YT;
-    static constexpr int STAGE = (TM + TN) * 128, LDS = 2 * STAGE;
+    static_assert(SB_ >= 2 && (SA_ == SB_ || SA_ == SB_ + 1), "the waits below count on it");
+    static constexpr int WM = WM_, WN = WN_, XT = XT_, YT = YT_, TM = 32 * WM * XT, TN = 32 * WN * YT, KB = KB_, SA = SA_, SB = SB_;
+    static constexpr int TILE_A = TM * KB, TILE_B = TN * KB, LDS = SA * TILE_A + SB * TILE_B;
     static constexpr bool BY_GROUP = TM > 128;
     static constexpr int BLOCKS = XT * YT > 8 ? 1 : 2;   // of a CU: registers and LDS leave room for so many
 };
@@ -73,8 +101,10 @@ template <int WM_, int WN_, int XT_, int YT_> struct Shape {
 template <class T, int MODE, bool BKFAST, class S, bool BY_GROUP>
 __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* lds) {
     static_assert(sizeof(T) == 2, "16-bit operands");
-    constexpr int XT = S::XT, YT = S::YT, TM = S::TM, TN = S::TN, BK = 64, STAGE = S::STAGE;
-    constexpr int CA = TM / 32, CB = TN / 32;      // chunks of each operand per thread and stage
+    constexpr int XT = S::XT, YT = S::YT, TM = S::TM, TN = S::TN, KB = S::KB, BK = KB / 2, SA = S::SA, SB = S::SB;
+    constexpr int TILE_A = S::TILE_A, TILE_B = S::TILE_B, BASE_B = SA * TILE_A;   // LDS: the first operand's slots, then the second's
+    constexpr int CPR = KB / 16, RPI = 256 / CPR;            // k-fast: chunks of a row, rows that 256 threads fetch at once
+    constexpr int CA = TM / RPI, CB = TN / RPI, H = BK / 16;   // chunks of each operand per thread and stage; 16 k's of a stage
     constexpr bool OUT = MODE == OUTER || MODE == PAIR, AKFAST = !OUT;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % S::WM, wn = wave / S::WM;
@@ -88,10 +118,9 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0;
 
-    // (shared mode's low-rank part comes first, see below)
-    // This thread's chunks.  k-fast: the chunk (tid ^ row) % 8 of rows tid / 8 + 32 i; row-fast: chunk (tid + 256 i) % RX of
-    // k = (tid + 256 i) / RX, its place swizzled; either way a wave's 64 lanes fill 1024 consecutive bytes of LDS.
-    const int cr = tid >> 3, kc = ((tid ^ cr) & 7) * 8;
+    // This thread's chunks.  k-fast: of rows tid / CPR + RPI i, its place in the row turned; row-fast: chunk (tid + 256 i) % RX
+    // of k = (tid + 256 i) / RX, turned as well; either way a wave's 64 lanes fill 1024 consecutive bytes of LDS.
+    const int cr = tid / CPR, kc = (int)((tid ^ turn<KB>(cr)) & (CPR - 1)) * 8;
     constexpr int RA = TM / 8, RB = TN / 8;        // chunks of a row of k in a row-fast tile
     const int kend = OUT ? t.rows : real ? a.K : 0;
     uint32_t va[CA], vb[CB];
@@ -106,7 +135,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         A = buffer_of(a.A, (uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2));
 #pragma unroll
         for (int i = 0; i < CA; ++i) {
-            const int64_t s = cr + 32 * i < t.rows && real ? source_row(a, t.first + cr + 32 * i) : -1;
+            const int64_t s = cr + RPI * i < t.rows && real ? source_row(a, t.first + cr + RPI * i) : -1;
             va[i] = s >= 0 ? (uint32_t)(s * a.a_row * 2) + kc * 2 : NOWHERE;
         }
     } else {
@@ -125,7 +154,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     if constexpr (BKFAST) {
         B = buffer_of((const char*)a.B + (MODE == ROWS && real ? t.group * a.b_group * 2 : 0), (uint32_t)((a.N - 1) * a.b_n * 2 + a.K * 2));
 #pragma unroll
-        for (int i = 0; i < CB; ++i) vb[i] = n0 + cr + 32 * i < a.N ? (uint32_t)((n0 + cr + 32 * i) * a.b_n * 2) + kc * 2 : NOWHERE;
+        for (int i = 0; i < CB; ++i) vb[i] = n0 + cr + RPI * i < a.N ? (uint32_t)((n0 + cr + RPI * i) * a.b_n * 2) + kc * 2 : NOWHERE;
     } else {
         const int64_t first = OUT ? t.first * a.b_k : MODE == ROWS && real ? t.group * a.b_group : 0;
         B = buffer_of((const char*)a.B + first * 2, kend > 0 ? (uint32_t)((kend - 1) * a.b_k * 2 + a.N * 2) : 0);
@@ -138,77 +167,89 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     }
     // Large shared tiles: the low-rank part is the first stages of the loop, V[p, :] as A's and E[g] as B's.
     constexpr bool EXT = MODE == SHARED && BY_GROUP;
-    u32x4 V = A, F = B;
-    uint32_t ve = 0, fe = 0;
     int ext = 0;
-    if constexpr (EXT) {
-        if (t.group < a.n_groups) {
-            ext = 2 * a.pad / BK;
-            V = buffer_of((const char*)a.V + (int64_t)t.first * a.v_row * 2, (uint32_t)((t.rows - 1) * a.v_row * 2 + 2 * a.pad * 2));
-            F = buffer_of((const char*)a.E + t.group * a.e_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.e_n * 2 + a.r * 2 : (a.r - 1) * a.e_k * 2 + a.N * 2));
-            ve = (uint32_t)(cr * a.v_row * 2) + kc * 2;
-            fe = BKFAST ? (uint32_t)((n0 + cr) * a.e_n * 2) : 0;
-        }
-    }
-    const int stages = ext + (kend + BK - 1) / BK;
-    struct Stage {
-        bool low;              // of the low-rank part
-        int k0;                // first k in its part
-        uint32_t oa, ob;       // scalar offsets
-    };
-    auto stage_of = [&](int s) {   // (behind the last one every chunk is beyond kend)
-        Stage g;
-        g.low = EXT && s < ext;
-        g.k0 = (g.low ? s : s - ext) * BK;
-        const bool there = s < stages;
-        g.oa = !there ? 0 : g.low ? g.k0 * 2 : (uint32_t)(s - ext) * step_a;
-        g.ob = !there || g.low ? 0 : (uint32_t)(s - ext) * step_b;
-        return g;
-    };
-    auto pick = [](bool first, u32x4 x, u32x4 y) { return (u32x4){first ? x[0] : y[0], first ? x[1] : y[1], first ? x[2] : y[2], y[3]}; };
-    // chunk i of the two operands for a stage, into buffer `to`
-    auto issue_a = [&](int i, const Stage& g, uint32_t to) {
-        uint32_t v = va[i];
-        if constexpr (AKFAST) {
-            v = g.k0 + kc < kend ? v : NOWHERE;
-            if constexpr (EXT) {
-                const uint32_t low = cr + 32 * i < t.rows ? ve + i * 32 * (uint32_t)(a.v_row * 2) : NOWHERE;
-                v = g.low ? low : v;
-            }
-        } else {
-            const int k = (tid + 256 * i) / RA;
-            if (a.gather && a.order) {
-                const int s = __shfl(next_row, k, 64);   // (-1 behind the group's last row)
-                v = s >= 0 && v != NOWHERE ? v + (uint32_t)s * (uint32_t)(a.a_row * 2) : NOWHERE;
-            } else
-                v = g.k0 + k < kend ? v : NOWHERE;
-        }
-        load_to_lds(EXT ? pick(g.low, V, A) : A, v, g.oa, to + i * 4096 + wave * 1024);
-    };
-    auto issue_b = [&](int i, const Stage& g, uint32_t to) {
-        uint32_t v = vb[i];
-        if constexpr (BKFAST) v = g.k0 + kc < kend ? v : NOWHERE;
-        else v = g.k0 + (tid + 256 * i) / RB < kend ? v : NOWHERE;
+    if constexpr (EXT) ext = t.group < a.n_groups ? 2 * a.pad / BK : 0;
+    const int main_stages = (kend + BK - 1) / BK, stages = ext + main_stages;
+
+    // What the loads of a stage are: buffers, the chunks' offsets in them, and scalar offsets that go on from stage to stage.
+    // Offsets change at the ends of the parts only, by a branch that is seldom taken, and the loop's loads take them as they are.
+    struct {
+        u32x4 A, B;
+        uint32_t va[CA], vb[CB], oa, ob;
+    } now;
+    auto stage_a = [&](int s) {   // s one more than before
+        now.oa += step_a;
         if constexpr (EXT) {
-            uint32_t low;
-            if constexpr (BKFAST) {
-                int rank = g.k0 + kc;
-                rank = rank >= a.pad ? rank - a.pad : rank;
-                low = rank < a.r && vb[i] != NOWHERE ? fe + i * 32 * (uint32_t)(a.e_n * 2) + rank * 2 : NOWHERE;
-            } else {
-                const int id = tid + 256 * i, kk = id / RB;
-                int rank = g.k0 + kk;
-                rank = rank >= a.pad ? rank - a.pad : rank;
-                low = rank < a.r && vb[i] != NOWHERE ? (uint32_t)rank * (uint32_t)(a.e_k * 2) + vb[i] - (uint32_t)(kk * a.b_k * 2) : NOWHERE;
+            if (s < ext) {   // the halves of the pair, one after the other
+                now.A = buffer_of((const char*)a.V + (int64_t)t.first * a.v_row * 2, (uint32_t)((t.rows - 1) * a.v_row * 2 + 2 * a.pad * 2));
+                now.oa = 0;
+#pragma unroll
+                for (int i = 0; i < CA; ++i) now.va[i] = cr + RPI * i < t.rows ? (uint32_t)((cr + RPI * i) * a.v_row * 2) + (s * BK + kc) * 2 : NOWHERE;
             }
-            v = g.low ? low : v;
         }
-        load_to_lds(EXT ? pick(g.low, F, B) : B, v, g.ob, to + TM * 128 + i * 4096 + wave * 1024);
+        if (s == ext) {
+            now.A = A, now.oa = 0;
+#pragma unroll
+            for (int i = 0; i < CA; ++i) now.va[i] = va[i];
+        }
+        if constexpr (!AKFAST) {
+            if (a.gather && a.order && s < stages) {
+#pragma unroll
+                for (int i = 0; i < CA; ++i) {
+                    const int row = __shfl(next_row, (tid + 256 * i) / RA, 64);   // (-1 behind the group's last row)
+                    now.va[i] = row >= 0 && va[i] != NOWHERE ? va[i] + (uint32_t)row * (uint32_t)(a.a_row * 2) : NOWHERE;
+                }
+                look_up((s + 1) * BK);
+            }
+        }
+        if (s >= stages - 1) {
+            const bool gone = s >= stages;   // behind the last stage: nothing; in it: nothing beyond the last k
+            const int k0 = (s - ext) * BK;
+            if (gone) now.oa = 0;
+#pragma unroll
+            for (int i = 0; i < CA; ++i) {
+                const int k = k0 + (AKFAST ? kc : (tid + 256 * i) / RA);
+                now.va[i] = gone || (main_stages > 0 && k >= kend) ? NOWHERE : now.va[i];
+            }
+        }
+        now.oa = scalar_of(now.oa);
+    };
+    auto stage_b = [&](int s) {
+        now.ob += step_b;
+        if constexpr (EXT) {
+            if (s < ext) {   // ranks beyond r read as zeros on both sides
+                const int k0 = s * BK;
+                now.B = buffer_of((const char*)a.E + t.group * a.e_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.e_n * 2 + a.r * 2 : (a.r - 1) * a.e_k * 2 + a.N * 2));
+                now.ob = 0;
+#pragma unroll
+                for (int i = 0; i < CB; ++i) {
+                    const int id = tid + 256 * i, kk = BKFAST ? kc : id / RB, k = k0 + kk, rank = k >= a.pad ? k - a.pad : k;
+                    const int n = BKFAST ? n0 + cr + RPI * i : n0 + ((id % RB) ^ (rowfast_swizzle<T>(kk) & (RB - 1))) * 8;
+                    now.vb[i] = n < a.N && rank < a.r ? (uint32_t)(n * a.e_n * 2) + (uint32_t)(rank * a.e_k * 2) : NOWHERE;
+                }
+            }
+        }
+        if (s == ext) {
+            now.B = B, now.ob = 0;
+#pragma unroll
+            for (int i = 0; i < CB; ++i) now.vb[i] = vb[i];
+        }
+        if (s >= stages - 1) {
+            const bool gone = s >= stages;
+            const int k0 = (s - ext) * BK;
+            if (gone) now.ob = 0;
+#pragma unroll
+            for (int i = 0; i < CB; ++i) {
+                const int k = k0 + (BKFAST ? kc : (tid + 256 * i) / RB);
+                now.vb[i] = gone || (main_stages > 0 && k >= kend) ? NOWHERE : now.vb[i];
+            }
+        }
+        now.ob = scalar_of(now.ob);
     };
     u32x4 fa[2][XT], fb[2][YT];
-    auto read = [&](int set, int i, const char* stage, int h) {
-        if (i < XT) fa[set][i] = fragment32<T, TM, AKFAST>(stage, (wm * XT + i) * 32, h, lane);
-        else fb[set][i - XT] = fragment32<T, TN, BKFAST>(stage + TM * 128, (wn * YT + i - XT) * 32, h, lane);
+    auto read = [&](int set, int i, int slot_a, int slot_b, int h) {   // in the order in which the products ask for them
+        if (i >= YT) fa[set][i - YT] = fragment32<T, TM, AKFAST, KB>(lds + slot_a, (wm * XT + i - YT) * 32, h, lane);
+        else fb[set][i] = fragment32<T, TN, BKFAST, KB>(lds + slot_b, (wn * YT + i) * 32, h, lane);
     };
     constexpr int FRAGS = XT + YT, CHUNKS = CA + CB;
     if constexpr (MODE == SHARED && !BY_GROUP) {
@@ -227,32 +268,32 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
                 __syncthreads();   // the last stage has been read
 #pragma unroll
                 for (int i = 0; i < CA; ++i)
-                    load_to_lds(V, cr + 32 * i < t.rows ? (uint32_t)((cr + 32 * i) * a.v_row * 2) + (k0 + kc) * 2 : NOWHERE, 0, lds0 + i * 4096 + wave * 1024);
+                    load_to_lds(V, cr + RPI * i < t.rows ? (uint32_t)((cr + RPI * i) * a.v_row * 2) + (k0 + kc) * 2 : NOWHERE, 0, lds0 + i * 4096 + wave * 1024);
 #pragma unroll
                 for (int i = 0; i < CB; ++i) {
                     uint32_t v;
                     if constexpr (BKFAST) {
-                        const int k = k0 + kc, rank = k >= a.pad ? k - a.pad : k, n = n0 + cr + 32 * i;
+                        const int k = k0 + kc, rank = k >= a.pad ? k - a.pad : k, n = n0 + cr + RPI * i;
                         v = n < a.N && rank < a.r ? (uint32_t)(n * a.e_n * 2) + rank * 2 : NOWHERE;
                     } else {
                         const int id = tid + 256 * i, kk = id / RB, k = k0 + kk, rank = k >= a.pad ? k - a.pad : k;
                         const int n = n0 + ((id % RB) ^ (rowfast_swizzle<T>(kk) & (RB - 1))) * 8;
                         v = n < a.N && rank < a.r ? (uint32_t)(rank * a.e_k * 2) + n * 2 : NOWHERE;
                     }
-                    load_to_lds(E, v, 0, lds0 + TM * 128 + i * 4096 + wave * 1024);
+                    load_to_lds(E, v, 0, lds0 + BASE_B + i * 4096 + wave * 1024);
                 }
                 wait_loads<0>();
                 wait_fragments_and_barrier();
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
+                for (int h = 0; h < H; ++h) {
                     u32x4 eb[YT];
 #pragma unroll
-                    for (int y = 0; y < YT; ++y) eb[y] = fragment32<T, TN, BKFAST>(lds + TM * 128, (wn * YT + y) * 32, h, lane);
+                    for (int y = 0; y < YT; ++y) eb[y] = fragment32<T, TN, BKFAST, KB>(lds + BASE_B, (wn * YT + y) * 32, h, lane);
 #pragma unroll
                     for (int x = 0; x < XT; ++x) {
                         const int r0 = (wm * XT + x) * 32, r = r0 + (lane & 31);
                         if (to <= r0 || from >= r0 + 32) continue;
-                        const u32x4 ea = fragment32<T, TM, true>(lds, r0, h, lane);
+                        const u32x4 ea = fragment32<T, TM, true, KB>(lds, r0, h, lane);
                         const bool all = from <= r0 && to >= r0 + 32, mine = r >= from && r < to;
 #pragma unroll
                         for (int y = 0; y < YT; ++y) {
@@ -281,48 +322,79 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         }
     }
     if (stages > 0) {
+        // Between two barriers lie H M products, and the loads of a stage of each operand into the slots that the first of them
+        // frees: item c, chunk item_i of operand item_a, beside product place(c).  Evenly, because loads in a row wait for one
+        // another and hold the products up; with a slot less for the second operand, that one's first.
+        constexpr int M = XT * YT;
+        constexpr bool SKEW = SA > SB;
+        auto item_a = [](int c) { return SKEW ? c >= CB : c < CA; };
+        auto item_i = [](int c) { return SKEW ? (c >= CB ? c - CB : c) : c < CA ? c : c - CA; };
+        auto place = [](int c) { return !SKEW ? c * H * M / CHUNKS : c < CB ? c * M / CB : M + (c - CB) * 2 * M / CA; };
+        constexpr int FIRST = SKEW ? CB : (CHUNKS + H - 1) / H;   // items before the stage's end
+        now.oa = now.ob = 0;
+        const uint32_t mine = scalar_of(lds0 + wave * 1024);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const Stage g = stage_of(s);
+        for (int s = 0; s < SA; ++s) {
+            stage_a(s);
+            if (s < SB) stage_b(s);
 #pragma unroll
-            for (int i = 0; i < CA; ++i) issue_a(i, g, lds0 + s * STAGE);
+            for (int i = 0; i < CA; ++i)                           // (the loop goes on with what is left out here)
+                if (s < SA - 1 || (!SKEW && i < FIRST)) load_to_lds(now.A, now.va[i], now.oa, mine + s * TILE_A + i * 4096);
 #pragma unroll
-            for (int i = 0; i < CB; ++i) issue_b(i, g, lds0 + s * STAGE);
-            look_up((s + 1) * BK);
+            for (int i = 0; i < CB; ++i)
+                if (s < SB - 1 || (SKEW && s < SB) || (!SKEW && CA + i < FIRST)) load_to_lds(now.B, now.vb[i], now.ob, mine + BASE_B + s * TILE_B + i * 4096);
         }
-        wait_loads<CHUNKS>();
+        wait_loads<SKEW ? (SB - 1) * CHUNKS : (SA - 2) * CHUNKS + FIRST>();
         wait_fragments_and_barrier();
+        int at_a = 0, at_b = BASE_B;
 #pragma unroll
-        for (int i = 0; i < FRAGS; ++i) read(0, i, lds, 0);
-        int at = 0;
+        for (int i = 0; i < FRAGS; ++i) read(0, i, at_a, at_b, 0);
+        uint32_t before_a = scalar_of(mine + (SA - 1) * TILE_A), before_b = scalar_of(mine + BASE_B + (SB - 1) * TILE_B);
         for (int s = 0; s < stages; ++s) {
-            // (behind the last stage the loads go nowhere and the fragments that are read are not used: no branch in the loop)
-            const Stage g = stage_of(s + 2);
-            const uint32_t to = lds0 + at;
+            // (behind the last stage the loads go nowhere and the fragments that are read are not used)
+            const int next_a = at_a + TILE_A < BASE_B ? at_a + TILE_A : 0, next_b = at_b + TILE_B < S::LDS ? at_b + TILE_B : BASE_B;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                if (h == 3) {
-                    wait_loads<0>();
+            for (int h = 0; h < H; ++h) {
+                constexpr int LAST = H - 1;
+                if (h == LAST) {
+                    stage_b(s + SB);
+                    stage_a(s + SA);
+                    before_a = scalar_of(mine + at_a), before_b = scalar_of(mine + at_b);
+                    wait_loads<(SB - 2) * CHUNKS + (SA - SB) * CA>();
                     wait_fragments_and_barrier();
                 }
-                constexpr int EACH = (FRAGS + XT - 1) / XT, LOADS = (CHUNKS + XT - 1) / XT;
+                // One wave has a SIMD to itself and issues one instruction in four cycles or more, a few beside each product of
+                // 32: the reads and loads are dealt out between the products, in this order and no other.
+                const int from = h == LAST ? 0 : (h + 1) * M;   // products since the barrier
 #pragma unroll
-                for (int x = 0; x < XT; ++x) {
-                    if (h == 3)
+                for (int m = 0; m < M; ++m) {
 #pragma unroll
-                        for (int i = x * LOADS; i < (x + 1) * LOADS && i < CHUNKS; ++i) {
-                            if (i < CA) issue_a(i, g, to);
-                            else issue_b(i - CA, g, to);
+                    for (int i = m * FRAGS / M; i < (m + 1) * FRAGS / M; ++i)
+                        read((h + 1) & 1, i, h == LAST ? next_a : at_a, h == LAST ? next_b : at_b, (h + 1) % H);
+                    bool first = true;
+                    unrolled<CHUNKS>([&](auto item) {
+                        constexpr int c = decltype(item)::value, to = (SKEW ? c >= CB ? c - CB : c : c < CA ? c : c - CA) * 4096;
+                        if (place(c) != from + m || !first) return;
+                        load_goes_to<to>(item_a(c) ? before_a : before_b);
+                        first = false;
+                    });
+                    acc[m / YT][m % YT] = mma32<T>(fb[h & 1][m % YT], fa[h & 1][m / YT], acc[m / YT][m % YT]);
+                    first = true;
+                    unrolled<CHUNKS>([&](auto item) {
+                        constexpr int c = decltype(item)::value, to = (SKEW ? c >= CB ? c - CB : c : c < CA ? c : c - CA) * 4096;
+                        if (place(c) != from + m) return;
+                        if (!first) {   // (more than one beside a product, in small tiles)
+                            load_goes_to<to>(item_a(c) ? before_a : before_b);
+                            asm volatile("s_nop 0" ::: "memory");
                         }
-#pragma unroll
-                    for (int i = x * EACH; i < (x + 1) * EACH && i < FRAGS; ++i) read((h + 1) & 1, i, lds + (h == 3 ? at ^ STAGE : at), (h + 1) & 3);
-#pragma unroll
-                    for (int y = 0; y < YT; ++y) acc[x][y] = mma32<T>(fb[h & 1][y], fa[h & 1][x], acc[x][y]);
+                        first = false;
+                        if (item_a(c)) load_there(now.A, now.va[item_i(c)], now.oa);
+                        else load_there(now.B, now.vb[item_i(c)], now.ob);
+                    });
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            look_up((s + 3) * BK);
-            at ^= STAGE;
+            at_a = next_a, at_b = next_b;
         }
         wait_loads<0>();
     }
@@ -433,8 +505,8 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
         if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
         if constexpr (TM == 256) {
             // a group's last tile is seldom full: half or a quarter of the rows in half or 0.4 of the time
-            typedef Shape<1, 4, 2, 2> Quarter;
-            typedef Shape<2, 2, 2, 4> Half;
+            typedef Shape<1, 4, 2, 2, S::KB, S::SA, S::SB> Quarter;
+            typedef Shape<2, 2, 2, 4, S::KB, S::SA, S::SB> Half;
             static_assert(Quarter::TN == TN && Half::TN == TN && Half::LDS <= S::LDS, "the same columns");
             if (t.rows <= 64) {
                 fast_tile<T, MODE, BKFAST, Quarter, true>(a, t, lds);
@@ -466,7 +538,7 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
 // Whether the kernel can take a call: rows that start 16-byte aligned and end with a chunk, spans that 32 bits address.
 inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 inline bool fast_rows(const void* p, int64_t rows, int64_t stride, int64_t inner_stride, int64_t inner) {
-    return aligned(p, 16) && inner_stride == 1 && inner % 8 == 0 && stride % 8 == 0 && stride > 0 && (rows - 1) * stride * 2 + inner * 2 < MOST_SPAN;
+    return aligned(p, 16) && inner_stride == 1 && inner % 8 == 0 && stride % 8 == 0 && stride >= inner && (rows - 1) * stride * 2 + inner * 2 < MOST_SPAN;
 }
 template <int MODE> inline bool fast_takes(const Args& a, bool bkfast) {
     if (MODE == PAIR) return a.pad > 0 && a.pad <= 64 && !a.use_beta && fast_rows(a.A, a.a_rows, a.a_row, a.a_col, a.M) && fast_rows(a.B, a.b_rows, a.b_k, a.b_n, 2 * a.pad);

@@ -1,5 +1,7 @@
 // ragged_launch.hpp -- chooses and launches a kernel on rows in groups; one translation unit per operand type includes it.
 #pragma once
+#include <type_traits>
+
 #include "launch.hpp"
 #include "ragged.hpp"
 #include "ragged_fast.hpp"
@@ -57,13 +59,14 @@ int32_t launch_fast(const Args& a, void* stream) {
     TFH_LAUNCH_NAMED(label.c_str(), (ragged_fast_kernel<T, MODE, BKFAST, S>), dim3((unsigned)blocks), dim3(256), S::LDS, (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
-typedef Shape<2, 2, 4, 4> Large;    // 256 x 256
+typedef Shape<2, 2, 4, 4, 128, 3, 2> Large;     // 256 x 256
+typedef Shape<2, 2, 4, 4, 64, 5, 5> LargeOuter;
 typedef Shape<2, 2, 2, 2> Middle;   // 128 x 128
 typedef Shape<1, 4, 1, 1> Small;    // 32 x 128
 template <class T, int MODE, bool BKFAST>
 int32_t launch_shape(const Args& a, void* stream) {
     const int64_t rows = MODE == OUTER ? a.M : a.n_rows / a.n_groups;
-    if (rows > 192) return launch_fast<T, MODE, BKFAST, Large>(a, stream);
+    if (rows > 192) return launch_fast<T, MODE, BKFAST, std::conditional_t<MODE == OUTER, LargeOuter, Large>>(a, stream);
     if (rows > 48) return launch_fast<T, MODE, BKFAST, Middle>(a, stream);
     return launch_fast<T, MODE, BKFAST, Small>(a, stream);
 }
