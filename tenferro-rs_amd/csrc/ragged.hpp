@@ -235,6 +235,21 @@ __device__ __forceinline__ int group_of(const Args& a, int p) {
     }
     return lo;
 }
+// Calls f(g, from, to) for the groups that rows first .. last belong to, in order; the lanes read 64 groups' offsets at a time.
+template <class F> __device__ __forceinline__ void each_group(const Args& a, int first, int last, F f) {
+    const int lane = threadIdx.x & 63;
+    for (int g0 = a.n_groups > 256 ? __builtin_amdgcn_readfirstlane(group_of(a, first)) & ~63 : 0; g0 < a.n_groups; g0 += 64) {
+        int from = 0, to = 0;
+        if (g0 + lane < a.n_groups) from = clamp_row(a.offsets[g0 + lane], a.n_rows), to = clamp_row(a.offsets[g0 + lane + 1], a.n_rows);
+        uint64_t found = __ballot(to > from && to > first && from <= last);
+        while (found) {
+            const int b = __builtin_ctzll(found);
+            found &= found - 1;
+            f(g0 + b, (int)__builtin_amdgcn_readlane(from, b), (int)__builtin_amdgcn_readlane(to, b));
+        }
+        if (__ballot(to > last)) break;
+    }
+}
 // The row of A that row p of the order reads; -1: none (the order names a row that is not there).
 __device__ __forceinline__ int64_t source_row(const Args& a, int p) {
     int64_t s = p;
@@ -356,11 +371,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
 
     if constexpr (MODE == SHARED) {
         constexpr int EW = Num<W>::E, RW = TN * (int)sizeof(W) / 16;
-        const int last = t.first + t.rows - 1;
-        for (int g = group_of(a, t.first); g < a.n_groups; ++g) {
-            const int from = clamp_row(a.offsets[g], a.n_rows), to = clamp_row(a.offsets[g + 1], a.n_rows);
-            if (from > last) break;
-            if (to <= from) continue;
+        each_group(a, t.first, t.first + t.rows - 1, [&](int g, int from, int to) {
             const TB* const Eg = (const TB*)a.E + g * a.e_group;
             auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
 #pragma unroll
@@ -381,7 +392,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                 }
             };
             k_loop<W, true, BKFAST, XT, YT, false>(acc, lds, a.r, wm, wn, lane, from - t.first, to - t.first, load);
-        }
+        });
     }
 
     const TA* const A = (const TA*)a.A;

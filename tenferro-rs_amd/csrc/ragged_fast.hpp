@@ -257,12 +257,8 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         // V is scaled by a power of two, which is undone here.  The pair's halves are 2 pad k's against E twice.  Rows of
         // another group keep what they have -- selected, not multiplied by zero, which infinite factors would survive.
         const u32x4 V = buffer_of((const char*)a.V + (int64_t)t.first * a.v_row * 2, (uint32_t)((t.rows - 1) * a.v_row * 2 + 2 * a.pad * 2));
-        const int last = t.first + t.rows - 1;
-        for (int g = __builtin_amdgcn_readfirstlane(group_of(a, t.first)); g < a.n_groups; ++g) {
-            const int from = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[g], a.n_rows)) - t.first;
-            const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[g + 1], a.n_rows)) - t.first;
-            if (from + t.first > last) break;
-            if (to <= from || to <= 0) continue;
+        each_group(a, t.first, t.first + t.rows - 1, [&](int g, int from, int to) {
+            from -= t.first, to -= t.first;
             const u32x4 E = buffer_of((const char*)a.E + g * a.e_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.e_n * 2 + a.r * 2 : (a.r - 1) * a.e_k * 2 + a.N * 2));
             for (int k0 = 0; k0 < 2 * a.pad; k0 += BK) {
                 __syncthreads();   // the last stage has been read
@@ -306,7 +302,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
                     }
                 }
             }
-        }
+        });
         __syncthreads();
         if (a.up) {
             const int first_of = clamp_row(a.offsets[0], a.n_rows), end_of = clamp_row(a.offsets[a.n_groups], a.n_rows);

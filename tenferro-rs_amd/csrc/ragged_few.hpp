@@ -72,29 +72,45 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void ragged_few_kernel(const Arg
     if constexpr (MODE == SHARED) {
         // The groups of the rows are dealt to the waves; a row takes its own group's products only.
         const auto V = __builtin_amdgcn_make_buffer_rsrc((char*)a.V + (int64_t)t.first * a.v_row * 2, 0, (int)(uint32_t)(t.rows * a.v_row * 2), 0x00020000);
-        const int last = t.first + t.rows - 1;
-        int turn = 0;
-        for (int g = __builtin_amdgcn_readfirstlane(group_of(a, t.first)); g < a.n_groups; ++g) {
-            const int f = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[g], a.n_rows)) - t.first;
-            const int e = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[g + 1], a.n_rows)) - t.first;
-            if (f + t.first > last) break;
-            if (e <= f || e <= 0) continue;
-            if (turn++ % FEW_WAVES != wave) continue;
-            const auto F = __builtin_amdgcn_make_buffer_rsrc((char*)a.E + g * a.e_group * 2, 0, (int)(uint32_t)((a.N - 1) * a.e_n * 2 + a.r * 2), 0x00020000);
-            for (int k0 = 0; k0 < a.pad; k0 += 32) {
-                const int rank = k0 + q * 8;
+        constexpr int AT_ONCE = 4;   // groups whose factors are asked for together
+        for (int k0 = 0; k0 < a.pad; k0 += 32) {
+            const int rank = k0 + q * 8;
+            u32x4 hi[TR], lo[TR];
+#pragma unroll
+            for (int x = 0; x < TR; ++x) {
+                const uint32_t v = x * 16 + j < t.rows ? (uint32_t)((x * 16 + j) * a.v_row * 2) + rank * 2 : NOWHERE;
+                hi[x] = __builtin_amdgcn_raw_buffer_load_b128(V, v, 0, 0);
+                lo[x] = __builtin_amdgcn_raw_buffer_load_b128(V, v == NOWHERE ? NOWHERE : v + a.pad * 2, 0, 0);
+            }
+            int turn = 0, mine = 0, froms[AT_ONCE], tos[AT_ONCE];
+            u32x4 factor[AT_ONCE];
+            auto multiply = [&](int count) {
+#pragma unroll
+                for (int c = 0; c < AT_ONCE; ++c) {
+                    if (c >= count) break;
+#pragma unroll
+                    for (int x = 0; x < TR; ++x) {
+                        const int r = x * 16 + j;
+                        if (tos[c] <= x * 16 || froms[c] >= x * 16 + 16) continue;
+                        const f32x4 sum = NT::mma(factor[c], lo[x], NT::mma(factor[c], hi[x], low[x]));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) low[x][i] = r >= froms[c] && r < tos[c] ? sum[i] : low[x][i];
+                    }
+                }
+            };
+            each_group(a, t.first, t.first + t.rows - 1, [&](int g, int f, int e) {
+                if (turn++ % FEW_WAVES != wave) return;
+                const auto F = __builtin_amdgcn_make_buffer_rsrc((char*)a.E + g * a.e_group * 2, 0, (int)(uint32_t)((a.N - 1) * a.e_n * 2 + a.r * 2), 0x00020000);
                 const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(F, rank < a.r && n0 + j < a.N ? (uint32_t)((n0 + j) * a.e_n * 2) + rank * 2 : NOWHERE, 0, 0);
 #pragma unroll
-                for (int x = 0; x < TR; ++x) {
-                    const int r = x * 16 + j;
-                    if (e <= x * 16 || f >= x * 16 + 16) continue;
-                    const uint32_t v = r < t.rows ? (uint32_t)(r * a.v_row * 2) + rank * 2 : NOWHERE;
-                    f32x4 sum = NT::mma(b, __builtin_amdgcn_raw_buffer_load_b128(V, v, 0, 0), low[x]);
-                    sum = NT::mma(b, __builtin_amdgcn_raw_buffer_load_b128(V, r < t.rows ? v + a.pad * 2 : NOWHERE, 0, 0), sum);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) low[x][i] = r >= f && r < e ? sum[i] : low[x][i];
+                for (int c = 0; c < AT_ONCE; ++c)
+                    if (c == mine) factor[c] = b, froms[c] = f - t.first, tos[c] = e - t.first;
+                if (++mine == AT_ONCE) {
+                    multiply(AT_ONCE);
+                    mine = 0;
                 }
-            }
+            });
+            multiply(mine);
         }
         const int first_of = clamp_row(a.offsets[0], a.n_rows), end_of = clamp_row(a.offsets[a.n_groups], a.n_rows);
 #pragma unroll

@@ -100,12 +100,12 @@ int32_t launch_thin(const Args& a, void* stream) {
     const int64_t blocks = row_tiles(a, THIN_ROWS);
     if (blocks <= 0) return TFH_OK;
     static const bool once = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT>), hipFuncAttributeMaxDynamicSharedMemorySize, thin_lds<T, BKFAST, YT>());
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT>), hipFuncAttributeMaxDynamicSharedMemorySize, thin_lds<YT>());
         return true;
     }();
     (void)once;
     static const std::string label = std::string("(ragged_thin_kernel<") + type_name<T>() + (BKFAST ? ", k, " : ", n, ") + std::to_string(32 * YT) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT>), dim3((unsigned)blocks), dim3(64 * THIN_WAVES), (thin_lds<T, BKFAST, YT>()), (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT>), dim3((unsigned)blocks), dim3(64 * thin_waves<YT>()), (thin_lds<YT>()), (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 

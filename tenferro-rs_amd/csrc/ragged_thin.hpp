@@ -1,16 +1,20 @@
 // ragged_thin.hpp -- the adapters' middle product V[p, :] = scale * X[src(p), :] . F[g] for 16-bit operands: a long k and
 // few columns (r <= 128), so that one pass over X is what it costs and the matrix cores are idle most of the time.
 //
-// A block has 32 rows of one group and all r columns; its eight waves share out k (64 of it at a time), each with the
-// operands straight from memory in registers, a step ahead, and add their sums up in LDS.  (Tiles through LDS with every
-// wave on the same k would have a few kilobytes in flight per CU; this has 64.)
+// A block has 32 rows of one group and all r columns; its waves share out k, 64 of it at a time, each with tiles of its own
+// in LDS that its own loads fill some steps ahead -- whole lines of every row, which loads in operand position would ask for
+// in four pieces -- and no barrier until their sums meet.
 #pragma once
 #include "ragged_fast.hpp"
 
 namespace tfh {
 namespace ragged {
 
-constexpr int THIN_WAVES = 8, THIN_ROWS = 32;
+constexpr int THIN_ROWS = 32;
+// Waves of a block and steps that each has in LDS or on their way, by what 32 YT columns leave room for.
+template <int YT> constexpr int thin_waves() { return YT == 1 ? 8 : 4; }
+template <int YT> constexpr int thin_ahead() { return YT == 2 ? 3 : 2; }
+template <int YT> constexpr int thin_lds() { return thin_waves<YT>() * thin_ahead<YT>() * (THIN_ROWS + 32 * YT) * 128; }
 
 // V's row p as a pair of numbers of the operands' type, v = up (hi + lo): 16 bits of it in bf16, 22 in f16, so that it is
 // no rounding of its own beside the result's.  f16 alone has a short exponent: its rows are brought to [2^7, 2^8) first.
@@ -48,82 +52,78 @@ __device__ __forceinline__ void store_pair(const Args& a, int64_t p, const float
     }
 }
 
-template <class T, bool BKFAST, int YT> constexpr int thin_lds() { return THIN_WAVES * THIN_ROWS * 32 * YT * 4; }
-
 template <class T, bool BKFAST, int YT>
-__global__ __launch_bounds__(64 * THIN_WAVES, 1) void ragged_thin_kernel(const Args a) {
-    constexpr int TN = 32 * YT, RB = TN / 8;   // RB: chunks of a row of k of F
+__global__ __launch_bounds__((64 * thin_waves<YT>()), 1) void ragged_thin_kernel(const Args a) {
+    constexpr int TN = 32 * YT, RB = TN / 8, WAVES = thin_waves<YT>(), AHEAD = thin_ahead<YT>();   // RB: chunks of a row of k of F
+    constexpr int SLOT = (THIN_ROWS + TN) * 128, LOADS = 4 + 4 * YT;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     char* const lds = (char*)smem_raw;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Tile t;
     if (!find_tile(a, THIN_ROWS, 1, blockIdx.x, t)) return;
     const int row = lane & 31, half = lane >> 5;
-    const int64_t s = row < t.rows ? source_row(a, t.first + row) : -1;
-    const auto A = __builtin_amdgcn_make_buffer_rsrc((void*)a.A, 0, (int)(uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2), 0x00020000);
-    const auto B = __builtin_amdgcn_make_buffer_rsrc((char*)a.B + t.group * a.b_group * 2, 0,
-                                                     (int)(uint32_t)(BKFAST ? (a.N - 1) * a.b_n * 2 + a.K * 2 : (a.K - 1) * a.b_k * 2 + a.N * 2), 0x00020000);
-    const uint32_t va = s >= 0 ? (uint32_t)(s * a.a_row * 2) : NOWHERE;
-    uint32_t vb[YT];
+    const u32x4 A = buffer_of(a.A, (uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2));
+    const u32x4 B = buffer_of((const char*)a.B + t.group * a.b_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.b_n * 2 + a.K * 2 : (a.K - 1) * a.b_k * 2 + a.N * 2));
+    // k-fast: a load has 8 rows, lane l the chunk (l ^ row) % 8 of row l / 8
+    const int cr = lane >> 3, kc = ((lane ^ cr) & 7) * 8;
+    uint32_t va[4], vb[4 * YT];
 #pragma unroll
-    for (int y = 0; y < YT; ++y) vb[y] = y * 32 + row < a.N ? (uint32_t)((y * 32 + row) * a.b_n * 2) : NOWHERE;
+    for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + cr;
+        const int64_t s = r < t.rows ? source_row(a, t.first + r) : -1;
+        va[i] = s >= 0 ? (uint32_t)(s * a.a_row * 2) + kc * 2 : NOWHERE;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * YT; ++i) {
+        if constexpr (BKFAST) {
+            vb[i] = 8 * i + cr < a.N ? (uint32_t)((8 * i + cr) * a.b_n * 2) + kc * 2 : NOWHERE;
+        } else {
+            const int id = lane + 64 * i, k = id / RB, n = ((id % RB) ^ (rowfast_swizzle<T>(k) & (RB - 1))) * 8;
+            vb[i] = n < a.N ? (uint32_t)(k * a.b_k * 2) + n * 2 : NOWHERE;
+        }
+    }
     f32x16 acc[YT];
 #pragma unroll
     for (int y = 0; y < YT; ++y)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[y][r] = 0;
-    // a step: 64 k's, 16 for each h; lane (row, half) has chunk 2 h + half of its row
-    constexpr int AHEAD = YT == 1 ? 4 : YT == 2 ? 2 : 1;   // steps whose loads are in flight, by the registers they take
-    u32x4 na[AHEAD][4], nb[AHEAD][4 * YT];
-    auto load = [&](int k0, u32x4 (&la)[4], u32x4 (&lb)[4 * YT]) {
+    const int steps = (a.K + 63) / 64, mine = steps > wave ? (steps - wave + WAVES - 1) / WAVES : 0;   // of this wave
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + wave * (AHEAD * SLOT);
+    auto issue = [&](int step, int slot) {   // (behind the last step: nothing)
+        const bool there = step < mine;
+        const int k0 = (step * WAVES + wave) * 64;
+        const uint32_t oa = scalar_of(there ? k0 * 2 : 0), ob = scalar_of(!there ? 0 : BKFAST ? k0 * 2 : (uint32_t)(k0 * a.b_k * 2)), to = scalar_of(lds0 + slot * SLOT);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int k = k0 + 16 * h + 8 * half;
-            la[h] = __builtin_amdgcn_raw_buffer_load_b128(A, k < a.K && va != NOWHERE ? va + k * 2 : NOWHERE, 0, 0);
-        }
+        for (int i = 0; i < 4; ++i) load_to_lds(A, there && k0 + kc < a.K ? va[i] : NOWHERE, oa, to + i * 1024);
 #pragma unroll
         for (int i = 0; i < 4 * YT; ++i) {
-            uint32_t v;
-            if constexpr (BKFAST) {
-                const int k = k0 + 16 * (i / YT) + 8 * half;
-                v = k < a.K && vb[i % YT] != NOWHERE ? vb[i % YT] + k * 2 : NOWHERE;
-            } else {
-                const int id = lane + 64 * i, k = k0 + id / RB, n = (id % RB) * 8;
-                v = k < a.K && n < a.N ? (uint32_t)(k * a.b_k * 2) + n * 2 : NOWHERE;
-            }
-            lb[i] = __builtin_amdgcn_raw_buffer_load_b128(B, v, 0, 0);
+            const int k = k0 + (BKFAST ? kc : (lane + 64 * i) / RB);
+            load_to_lds(B, there && k < a.K ? vb[i] : NOWHERE, ob, to + THIN_ROWS * 128 + i * 1024);
         }
     };
-    char* const mine = lds + wave * (64 * TN * 2);   // row-fast F: this wave's own tile, to be read across
-    constexpr int STRIDE = 64 * THIN_WAVES;
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) load(wave * 64 + d * STRIDE, na[d], nb[d]);   // (beyond K: zeros)
-    for (int k0 = wave * 64; k0 < a.K; k0 += AHEAD * STRIDE) {
+    for (int d = 0; d < AHEAD; ++d) issue(d, d);
+    int slot = 0;
+    for (int s = 0; s < mine; ++s) {
+        const char* const tile = lds + wave * (AHEAD * SLOT) + slot * SLOT;
+        wait_loads<(AHEAD - 1) * LOADS>();
+        u32x4 fa[4], fb[4 * YT];
 #pragma unroll
-        for (int d = 0; d < AHEAD; ++d) {
-            u32x4 fa[4], fb[4 * YT];
+        for (int h = 0; h < 4; ++h) {
+            fa[h] = fragment32<T, THIN_ROWS, true>(tile, 0, h, lane);
 #pragma unroll
-            for (int h = 0; h < 4; ++h) fa[h] = na[d][h];
-#pragma unroll
-            for (int i = 0; i < 4 * YT; ++i) fb[i] = nb[d][i];
-            load(k0 + (d + AHEAD) * STRIDE, na[d], nb[d]);
-            if constexpr (!BKFAST) {
-#pragma unroll
-                for (int i = 0; i < 4 * YT; ++i) {
-                    const int id = lane + 64 * i;
-                    *(u32x4*)(mine + rowfast_at<T, TN>(id / RB, id % RB)) = fb[i];
-                }
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int i = 0; i < 4 * YT; ++i) fb[i] = fragment32<T, TN, false>(mine, (i % YT) * 32, i / YT, lane);
-                __builtin_amdgcn_wave_barrier();
-            }
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int y = 0; y < YT; ++y) acc[y] = mma32<T>(fb[h * YT + y], fa[h], acc[y]);
+            for (int y = 0; y < YT; ++y) fb[h * YT + y] = fragment32<T, TN, BKFAST>(tile + THIN_ROWS * 128, y * 32, h, lane);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read, before the slot is filled again
+        __builtin_amdgcn_sched_barrier(0);
+        issue(s + AHEAD, slot);
+        slot = slot + 1 < AHEAD ? slot + 1 : 0;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int y = 0; y < YT; ++y) acc[y] = mma32<T>(fb[h * YT + y], fa[h], acc[y]);
     }
+    wait_loads<0>();
     // the waves' sums, in the order of the waves
     __syncthreads();
     constexpr int PART = THIN_ROWS * TN * 4;
@@ -137,14 +137,14 @@ __global__ __launch_bounds__(64 * THIN_WAVES, 1) void ragged_thin_kernel(const A
         }
     __syncthreads();
     const float scale = (float)a.alpha * (a.scales ? ((const float*)a.scales)[t.group] : 1.0f);
-    for (int r = wave; r < t.rows; r += THIN_WAVES) {
+    for (int r = wave; r < t.rows; r += WAVES) {
         float v[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c = lane + 64 * i;
             if (c < TN) {
 #pragma unroll
-                for (int w = 0; w < THIN_WAVES; ++w) v[i] += *(const float*)(lds + w * PART + r * (TN * 4) + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
+                for (int w = 0; w < WAVES; ++w) v[i] += *(const float*)(lds + w * PART + r * (TN * 4) + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
                 v[i] *= scale;
             }
         }
