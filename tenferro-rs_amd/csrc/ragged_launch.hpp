@@ -72,7 +72,7 @@ int32_t launch_shape(const Args& a, void* stream) {
 }
 template <class T, bool BKFAST>
 int32_t launch_shared(const Args& a, void* stream) {
-    // tiles by group read W once for each group's rows; worth it where they fill most of a tile.  (f16 scales its rows'
+    // Tiles by group read W once for each group's rows; worth it where those fill most of a tile.  (f16 scales its rows'
     // low-rank part back before the rest is added, which the large tile's one loop has no place for.)
     if constexpr (__is_same(T, __bf16))
         if (a.n_rows / (a.n_groups + 1) > 192) {
@@ -82,18 +82,19 @@ int32_t launch_shared(const Args& a, void* stream) {
         }
     return launch_fast<T, SHARED, BKFAST, Middle>(a, stream);
 }
-template <class T, int MODE, int TR, int STEPS>
-int32_t launch_few_steps(const Args& a, void* stream) {
+template <class T, int MODE, int TR>
+int32_t launch_few(const Args& a, void* stream) {
     const int64_t blocks = (MODE == ROWS ? row_tiles(a, 16 * TR) : tiles(a.n_rows, 16 * TR)) * tiles(a.N, 16);
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
+    static const bool once = [] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_few_kernel<T, MODE, TR>), hipFuncAttributeMaxDynamicSharedMemorySize, few_lds<TR>());
+        return true;
+    }();
+    (void)once;
     static const std::string label = std::string("(ragged_few_kernel<") + type_name<T>() + ", " + mode_name(MODE) + ", " + std::to_string(16 * TR) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR, STEPS>), dim3((unsigned)blocks), dim3(64 * FEW_WAVES), 0, (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR>), dim3((unsigned)blocks), dim3(few_threads<MODE>()), few_lds<TR>(), (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
-}
-template <class T, int MODE, int TR>
-int32_t launch_few(const Args& a, void* stream) {
-    return a.K <= 4 * 32 * FEW_WAVES ? launch_few_steps<T, MODE, TR, 4>(a, stream) : launch_few_steps<T, MODE, TR, 16>(a, stream);
 }
 template <class T, bool BKFAST, int YT>
 int32_t launch_thin(const Args& a, void* stream) {
@@ -114,12 +115,21 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
     // B's columns contiguous: its tiles keep the direction in which they are read
     const bool columns = a.b_n == 1 && a.b_k != 1;
     if constexpr (sizeof(T) == 2) {
+        // Few rows of few groups, likewise: 8 rows of as many 2048 x 1024 matrices take 14 us so and 22 with 32 x 128 tiles, 64
+        // rows of 50 of them 72 and 41 (the matrices bound that, and larger blocks read them better).
+        if (kind == PRODUCT_ROWS && !columns && few_takes<ROWS>(a)) {
+            const int64_t used = a.n_groups < a.n_rows ? a.n_groups : a.n_rows, each = a.n_rows / used, t16 = tiles(a.N, 16);
+            if (each <= 16 && (a.n_rows / 16 + used) * t16 <= 1024) return launch_few<T, ROWS, 1>(a, stream);
+            if (each <= 32 && (a.n_rows / 32 + used) * t16 <= 1024) return launch_few<T, ROWS, 2>(a, stream);
+            if (each <= 64 && (a.n_rows / 64 + used) * t16 <= 1024) return launch_few<T, ROWS, 4>(a, stream);
+        }
         if (kind == PRODUCT_ROWS && fast_takes<ROWS>(a, !columns))
             return columns ? launch_shape<T, ROWS, false>(a, stream) : launch_shape<T, ROWS, true>(a, stream);
         if (kind == PRODUCT_OUTER && fast_takes<OUTER>(a, false)) return launch_shape<T, OUTER, false>(a, stream);
-        if (kind == PRODUCT_SHARED && a.pad > 0 && a.n_rows <= 128 && !columns && few_takes<SHARED>(a))
-            return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream)
-                   : a.n_rows <= 64 ? launch_few<T, SHARED, 4>(a, stream) : launch_few<T, SHARED, 8>(a, stream);
+        // Few rows: sixteen columns a block.  64 rows by 4096 columns and k's take 16 us so and 86 with 128 x 128 tiles, whose 32
+        // blocks leave the machine idle; 1024 blocks take as long as those tiles do with 128.
+        if (kind == PRODUCT_SHARED && a.pad > 0 && !columns && few_takes<SHARED>(a) && tiles(a.n_rows, 64) * tiles(a.N, 16) <= 1024)
+            return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream) : launch_few<T, SHARED, 4>(a, stream);
         if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_shared<T, false>(a, stream) : launch_shared<T, true>(a, stream);
         if (kind == PRODUCT_OUTER_V && a.pad > 0) return launch_fast<T, PAIR, false, Middle>(a, stream);
         if (kind == PRODUCT_MIDDLE && thin_takes(a, !columns)) {
