@@ -132,6 +132,23 @@ __device__ __forceinline__ u32x4 load_chunk(const S* p, int64_t stride, int coun
     return v;
 }
 
+// The same in two parts for rows of elements next to each other, at least E of them: a load of the E elements up to the row's
+// end where that lies inside the chunk, which nothing waits for, and, when it is wanted, what of it is put in place.
+template <class T> __device__ __forceinline__ u32x4 load_unit(const T* p) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+template <class T> __device__ __forceinline__ void settle_unit(u32x4& v, int count) {
+    constexpr int E = Num<T>::E;
+    struct { uint64_t lo, hi; } w = __builtin_bit_cast(decltype(w), v);
+    const int s = count >= E ? 0 : count <= 0 ? 128 : (E - count) * (int)sizeof(T) * 8;   // bits that are not there
+    if (s >= 128) w = {0, 0};
+    else if (s >= 64) w = {w.hi >> (s - 64), 0};
+    else if (s > 0) w = {w.lo >> s | w.hi << (64 - s), w.hi >> s};
+    v = __builtin_bit_cast(u32x4, w);
+}
+
 // ---- tiles in LDS -------------------------------------------------------------------------------------------------
 // An operand's tile is 128 bytes of k by TM rows.  k-fast: [row][8 chunks], the chunk index XORed with the row so that
 // the 16 rows of a fragment read spread over the banks.  row-fast: [k][TM elements], whose 16-bit fragments are read by
@@ -260,10 +277,12 @@ __device__ __forceinline__ int64_t source_row(const Args& a, int p) {
     return s < a.a_rows ? s : -1;
 }
 
-// ---- the kernel for every type, layout and direction ------------------------------------------------------------------
-// Tiles of 32 XT x 32 YT, four waves, operands through registers into a double-buffered LDS tile (the loads of the next
-// 128 bytes of k are in flight while the present ones are multiplied).
+// ---- the kernels for every type, layout and direction -----------------------------------------------------------------
+// Tiles of 32 XT x 32 YT, four waves, operands through registers into a double-buffered LDS tile, 128 bytes of k at a time;
+// the loads run two such stages ahead (one in large tiles).
 constexpr int GENERAL_THREADS = 256;
+// Waits for this wave's LDS accesses only: global loads stay in flight over the barrier.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // One stage (128 bytes of k of type C) of a wave's 16 XT x 16 YT results.  Where not all rows take part, those in
 // [from, to) of the tile take the products and the others keep what they have: a row that is not a group's must not see
@@ -293,14 +312,17 @@ __device__ __forceinline__ void multiply_stage(typename Num<C>::acc4 (&acc)[XT][
         }
     }
 }
-// A whole k loop: load(i, k0, ra, rb) fetches a stage's chunks.
-template <class C, bool AKFAST, bool BKFAST, int XT, int YT, bool ALL, class Load>
-__device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], char* lds, int kend, int wm, int wn, int lane, int from, int to, Load load) {
+// A whole k loop: load(k0, ra, rb) fetches a stage's chunks, settle(k0, ra, rb) makes them what the tiles take.  Loads two
+// stages ahead are made for those behind the last one too (of anything that is there): were they left out on a condition, the wait
+// for one stage's would have to count on that, and would wait for the next one's as well.
+template <class C, bool AKFAST, bool BKFAST, int XT, int YT, bool ALL, class Load, class Settle>
+__device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], char* lds, int kend, int wm, int wn, int lane, int from, int to, Load load,
+                                       Settle settle) {
     constexpr int TM = 32 * XT, TN = 32 * YT, BK = 128 / (int)sizeof(C);
     constexpr int RA = TM * (int)sizeof(C) / 16, RB = TN * (int)sizeof(C) / 16;   // chunks of a row of k in a row-fast tile
     const int tid = threadIdx.x, cc = tid & 7, cr = tid >> 3;
-    u32x4 ra[XT], rb[YT];
-    auto store_stage = [&](char* stage) {
+    auto store_stage = [&](char* stage, int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+        settle(k0, ra, rb);
 #pragma unroll
         for (int i = 0; i < XT; ++i) {
             const int id = tid + GENERAL_THREADS * i;
@@ -315,27 +337,50 @@ __device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], cha
         }
     };
     if (kend <= 0) return;
-    __syncthreads();
-    load(0, ra, rb);
-    store_stage(lds);
-    __syncthreads();
-    int at = 0;
-    for (int k0 = 0; k0 < kend; k0 += BK) {
-        const bool more = k0 + BK < kend;
-        if (more) load(k0 + BK, ra, rb);
-        multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds + at, wm, wn, lane, from, to);
-        at ^= (TM + TN) * 128;
-        if (more) store_stage(lds + at);
-        __syncthreads();
+    constexpr int STAGE = (TM + TN) * 128;
+    if constexpr (XT + YT > 4) {   // a large tile's registers hold one stage beside the one that is multiplied
+        u32x4 a0[XT], b0[YT];
+        load(0, a0, b0);
+        lds_barrier();
+        store_stage(lds, 0, a0, b0);
+        lds_barrier();
+        int at = 0;
+        for (int k0 = 0; k0 < kend; k0 += BK) {
+            if (k0 + BK < kend) load(k0 + BK, a0, b0);
+            multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds + at, wm, wn, lane, from, to);
+            at ^= STAGE;
+            if (k0 + BK < kend) store_stage(lds + at, k0 + BK, a0, b0);
+            lds_barrier();
+        }
+    } else {
+        u32x4 a0[XT], b0[YT], a1[XT], b1[YT];
+        load(0, a0, b0);
+        load(BK, a1, b1);
+        lds_barrier();   // the last loop's tiles have been read
+        store_stage(lds, 0, a0, b0);
+        lds_barrier();
+        int k0 = 0;
+        for (; k0 + BK < kend; k0 += 2 * BK) {
+            load(k0 + 2 * BK, a0, b0);
+            multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds, wm, wn, lane, from, to);
+            store_stage(lds + STAGE, k0 + BK, a1, b1);
+            lds_barrier();
+            load(k0 + 3 * BK, a1, b1);
+            multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds + STAGE, wm, wn, lane, from, to);
+            if (k0 + 2 * BK < kend) store_stage(lds, k0 + 2 * BK, a0, b0);
+            lds_barrier();
+        }
+        if (k0 < kend) multiply_stage<C, AKFAST, BKFAST, XT, YT, ALL>(acc, lds, wm, wn, lane, from, to);
     }
 }
 
-// TA, TB: the operands' types; C: the type multiplied in (theirs, or that of the sums); TO: the result's.
-template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, int XT, int YT>
+// TA, TB: the operands' types; C: the type multiplied in (theirs, or that of the sums); TO: the result's.  UNIT: both operands
+// contiguous in the direction in which they are read (B along k if BKFAST), of type C, and no shorter than a chunk.
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT>
 __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(const Args a) {
     typedef Num<C> NT;
     typedef typename NT::acc W;
-    constexpr int E = NT::E, TM = 32 * XT, TN = 32 * YT;
+    constexpr int E = NT::E, TM = 32 * XT, TN = 32 * YT, BK = 128 / (int)sizeof(C);
     constexpr bool AKFAST = MODE != OUTER;
     __shared__ __align__(16) char lds[2 * (TM + TN) * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1, q = lane >> 4, j = lane & 15;
@@ -391,7 +436,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                     }
                 }
             };
-            k_loop<W, true, BKFAST, XT, YT, false>(acc, lds, a.r, wm, wn, lane, from - t.first, to - t.first, load);
+            k_loop<W, true, BKFAST, XT, YT, false>(acc, lds, a.r, wm, wn, lane, from - t.first, to - t.first, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
         });
     }
 
@@ -404,38 +449,122 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
     const TB* const B = (const TB*)a.B + (MODE == ROWS && real ? t.group * a.b_group : 0);
     const int kend = MODE == OUTER ? t.rows : real ? a.K : 0;
     constexpr int RA = TM * (int)sizeof(C) / 16, RB = TN * (int)sizeof(C) / 16;
-    auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+    // How many elements of chunk i are there, for the stage at k0.  (A row of A that is none, in outer mode, reads as zeros.)
+    auto count_a = [&](int i, int k0) {
+        const int id = tid + GENERAL_THREADS * i;
+        return AKFAST ? (arow[i] >= 0 ? kend - k0 - cc * E : 0) : k0 + id / RA < kend ? a.M - m0 - (id % RA) * E : 0;
+    };
+    auto count_b = [&](int i, int k0) {
+        const int id = tid + GENERAL_THREADS * i;
+        return BKFAST ? (n0 + cr + 32 * i < a.N ? kend - k0 - cc * E : 0) : k0 + id / RB < kend ? a.N - n0 - (id % RB) * E : 0;
+    };
+    if constexpr (UNIT) {
+        // Where this thread's chunks of a stage start, moved back to the row's last E elements where that ends inside one; rows and
+        // columns beyond the tile's read the first ones.
+        const int64_t step_b = BKFAST ? BK : BK * a.b_k;
+        const TA* pa[XT];
+        const TB* pb[YT];
 #pragma unroll
         for (int i = 0; i < XT; ++i) {
-            const int id = tid + GENERAL_THREADS * i;
-            if constexpr (AKFAST) {
-                const int k = k0 + cc * E;
-                ra[i] = load_chunk<TA, C>(A + arow[i] * a.a_row + k * a.a_col, a.a_col, arow[i] >= 0 ? kend - k : 0);
-            } else {
-                const int k = k0 + id / RA, m = m0 + (id % RA) * E;
-                const int64_t s = k < kend ? source_row(a, t.first + k) : -1;
-                ra[i] = load_chunk<TA, C>(A + s * a.a_row + m * a.a_col, a.a_col, s >= 0 ? a.M - m : 0);
-            }
+            const int id = tid + GENERAL_THREADS * i, m = m0 + (id % RA) * E;
+            if constexpr (AKFAST) pa[i] = A + (arow[i] > 0 ? arow[i] * a.a_row : 0) + cc * E;
+            else pa[i] = A + (m + E <= a.M ? m : a.M - E);
         }
 #pragma unroll
         for (int i = 0; i < YT; ++i) {
-            const int id = tid + GENERAL_THREADS * i;
-            if constexpr (BKFAST) {
-                const int k = k0 + cc * E, n = n0 + cr + 32 * i;
-                rb[i] = load_chunk<TB, C>(B + n * a.b_n + k * a.b_k, a.b_k, n < a.N ? kend - k : 0);
-            } else {
-                const int k = k0 + id / RB, n = n0 + (id % RB) * E;
-                int64_t s = k;
-                if constexpr (MODE == OUTER) {
-                    s = -1;
-                    if (k < kend) s = t.first + k;
-                    if (s >= a.b_rows) s = -1;
-                }
-                rb[i] = load_chunk<TB, C>(B + s * a.b_k + n * a.b_n, a.b_n, k < kend && s >= 0 ? a.N - n : 0);
-            }
+            const int id = tid + GENERAL_THREADS * i, n = n0 + (id % RB) * E;
+            if constexpr (BKFAST) pb[i] = B + (n0 + cr + 32 * i < a.N ? (n0 + cr + 32 * i) * a.b_n : 0) + cc * E;
+            else pb[i] = B + ((MODE == OUTER ? t.first : 0) + id / RB) * a.b_k + (n + E <= a.N ? n : a.N - E);
         }
-    };
-    k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load);
+        const bool edge_b = !BKFAST && n0 + TN > a.N;   // both the same for all of a wave
+        bool edge;
+        if constexpr (AKFAST) {
+            bool gone = false;
+#pragma unroll
+            for (int i = 0; i < XT; ++i) gone |= arow[i] < 0;
+            edge = __any(gone);
+        } else {
+            edge = m0 + TM > a.M || (a.gather && a.order) || t.first + kend > a.a_rows;
+        }
+        uint32_t none = 0;   // outer: chunks of a stage on their way whose row of A is none, the stages' bits apart
+        const int kwhole = kend / BK * BK;   // whole stages move the pointers on, those behind them leave them there
+        auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+            if constexpr (!AKFAST) {
+                const bool found = !(a.gather && a.order) && t.first + kend <= a.a_rows;
+#pragma unroll
+                for (int i = 0; i < XT; ++i) {
+                    const int id = tid + GENERAL_THREADS * i, k = k0 + id / RA;
+                    const int64_t s = k >= kend ? -1 : found ? t.first + k : source_row(a, t.first + k);
+                    const uint32_t bit = 1u << (((k0 / BK) & 3) * 8 + i);
+                    none = s < 0 ? none | bit : none & ~bit;
+                    ra[i] = load_unit<TA>(pa[i] + (s < 0 ? 0 : s) * a.a_row);
+                }
+            }
+            if (k0 < kwhole) {
+                if constexpr (AKFAST)
+#pragma unroll
+                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i]), pa[i] += BK;
+#pragma unroll
+                for (int i = 0; i < YT; ++i) rb[i] = load_unit<TB>(pb[i]), pb[i] += step_b;
+            } else {
+                const int count = kend - k0 - cc * E;
+                if constexpr (AKFAST)
+#pragma unroll
+                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i] - (count >= E ? 0 : count > 0 ? E - count : kwhole + cc * E));
+#pragma unroll
+                for (int i = 0; i < YT; ++i) {
+                    const int id = tid + GENERAL_THREADS * i;
+                    if constexpr (BKFAST) rb[i] = load_unit<TB>(pb[i] - (count >= E ? 0 : count > 0 ? E - count : kwhole + cc * E));
+                    else rb[i] = load_unit<TB>(pb[i] - (k0 + id / RB < kend ? 0 : (kwhole + id / RB) * a.b_k));
+                }
+            }
+        };
+        auto settle = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+            const bool whole = k0 + BK <= kend;
+            if (!whole || edge)
+#pragma unroll
+                for (int i = 0; i < XT; ++i) {
+                    int count = count_a(i, k0);
+                    if constexpr (!AKFAST)
+                        if (none >> (((k0 / BK) & 3) * 8 + i) & 1) count = 0;
+                    settle_unit<C>(ra[i], count);
+                }
+            if (!whole || edge_b)
+#pragma unroll
+                for (int i = 0; i < YT; ++i) settle_unit<C>(rb[i], count_b(i, k0));
+        };
+        k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load, settle);
+    } else {
+        auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
+#pragma unroll
+            for (int i = 0; i < XT; ++i) {
+                const int id = tid + GENERAL_THREADS * i;
+                int count = count_a(i, k0);
+                const TA* p;
+                if constexpr (AKFAST) {
+                    p = A + arow[i] * a.a_row + (k0 + cc * E) * a.a_col;
+                } else {
+                    const int64_t s = count > 0 ? source_row(a, t.first + k0 + id / RA) : -1;
+                    if (s < 0) count = 0;
+                    p = A + s * a.a_row + (m0 + (id % RA) * E) * a.a_col;
+                }
+                ra[i] = load_chunk<TA, C>(p, a.a_col, count);
+            }
+#pragma unroll
+            for (int i = 0; i < YT; ++i) {
+                const int id = tid + GENERAL_THREADS * i;
+                const TB* p;
+                if constexpr (BKFAST) {
+                    p = B + (n0 + cr + 32 * i) * a.b_n + (k0 + cc * E) * a.b_k;
+                } else {
+                    const int64_t k = MODE == OUTER ? t.first + k0 + id / RB : k0 + id / RB;
+                    p = B + k * a.b_k + (n0 + (id % RB) * E) * a.b_n;
+                }
+                rb[i] = load_chunk<TB, C>(p, BKFAST ? a.b_k : a.b_n, count_b(i, k0));
+            }
+        };
+        k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
+    }
 
     W alpha = (W)a.alpha;
     const W beta = (W)a.beta;

@@ -28,20 +28,43 @@ template <class T> constexpr const char* type_name() {
 }
 constexpr const char* mode_name(int mode) { return mode == ROWS ? "rows" : mode == OUTER ? "outer" : mode == SHARED ? "shared" : "pair"; }
 
-template <class TA, class TB, class C, class TO, int MODE, bool BKFAST>
-int32_t launch_general(const Args& a, void* stream) {
-    constexpr int XT = 2, YT = 2;
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT>
+int32_t launch_general_tiles(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, 32 * YT);
     const int64_t blocks = MODE == ROWS ? row_tiles(a, 32 * XT) * tn
                            : MODE == OUTER ? a.n_groups * tiles(a.M, 32 * XT) * tn : tiles(a.n_rows, 32 * XT) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
     static const std::string label = std::string("(ragged_general_kernel<") + type_name<TA>() + ", " + type_name<TB>() + ", " + type_name<C>() + ", " +
-                                     type_name<TO>() + ", " + mode_name(MODE) + (BKFAST ? ", k>)" : ", n>)");
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, XT, YT>), dim3((unsigned)blocks), dim3(GENERAL_THREADS), 0, (hipStream_t)stream, a);
+                                     type_name<TO>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") + (UNIT ? "unit, " : "any, ") +
+                                     std::to_string(32 * XT) + "x" + std::to_string(32 * YT) + ">)";
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, UNIT, XT, YT>), dim3((unsigned)blocks), dim3(GENERAL_THREADS), 0, (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
-
+// Whether both operands are contiguous in the direction in which the kernel reads them, and long enough for a chunk.
+template <class C, int MODE, bool BKFAST> bool unit_strides(const Args& a) {
+    constexpr int E = Num<C>::E;
+    if (a.a_rows < 1) return false;   // not one row to read where there is none to multiply
+    if (MODE == OUTER) return a.a_col == 1 && a.M >= E && a.b_n == 1 && a.N >= E;
+    return a.a_col == 1 && a.K >= E && (BKFAST ? a.b_k == 1 : a.b_n == 1 && a.N >= E);
+}
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST>
+int32_t launch_general(const Args& a, void* stream) {
+    if constexpr (__is_same(TA, C) && __is_same(TB, C))
+        if (unit_strides<C, MODE, BKFAST>(a)) {
+            // 128 x 128 tiles where the rows fill them and there are enough for the machine: of 16 bits from one a compute unit on
+            // (32 768 rows of 16 groups, 2047 x 1023: 241 us against 377; 168 of them, 3000 x 1001 x 777: 31 against 25), of f32, where
+            // the matrix units take 16 times as long, from eight (2048 x 1024: 1096 against 1172; 24 000 rows of 48 groups, 512 x 384: 140
+            // against 108).  f64's sums take registers that such tiles do not have.
+            if constexpr (sizeof(C) < 8) {
+                const int64_t rows = MODE == OUTER ? a.M : MODE == ROWS ? a.n_rows / a.n_groups : a.n_rows;
+                const int64_t blocks = (MODE == OUTER ? a.n_groups * tiles(a.M, 128) : MODE == ROWS ? a.n_rows / 128 + a.n_groups / 2 : tiles(a.n_rows, 128)) * tiles(a.N, 128);
+                if (rows > 96 && a.N > 96 && blocks >= (sizeof(C) == 4 ? 2048 : 256)) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 4, 4>(a, stream);
+            }
+            return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 2, 2>(a, stream);
+        }
+    return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, false, 2, 2>(a, stream);
+}
 template <class T, int MODE, bool BKFAST, class S>
 int32_t launch_fast(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, S::TN);
