@@ -14,61 +14,87 @@ namespace tfh {
 namespace ragged {
 namespace {
 
-constexpr int AT_ONCE = 8;   // choices of a token whose loads are in flight together
+constexpr int CHUNKS = 2;   // 16-byte pieces of a row that a lane has in flight for each of the choices
 
-template <class T>
-__device__ __forceinline__ void store_chunk(T* p, int64_t stride, int count, const T (&e)[Num<T>::E]) {
-    if (count >= Num<T>::E && stride == 1) {
-        __builtin_memcpy(p, e, 16);
+// E elements of a row from its n-th on, of which the row has `total`.  UNIT: next to each other, and E of them at least; a piece
+// that the row ends in is its last E elements instead.
+template <class T, bool UNIT> __device__ __forceinline__ u32x4 piece(const T* row, int64_t stride, int n, int total) {
+    constexpr int E = Num<T>::E;
+    if constexpr (UNIT) return load_unit<T>(row + (n + E <= total ? n : total - E));
+    else return load_chunk<T, T>(row + n * stride, stride, total - n);
+}
+template <class T, bool UNIT> __device__ __forceinline__ void put_piece(T* row, int64_t stride, int n, int total, const T (&e)[Num<T>::E]) {
+    constexpr int E = Num<T>::E;
+    if constexpr (UNIT) {
+        if (n < total) __builtin_memcpy(row + (n + E <= total ? n : total - E), e, 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < Num<T>::E; ++i)
-            if (i < count) p[i * stride] = e[i];
+        for (int i = 0; i < E; ++i)
+            if (n + i < total) row[(n + i) * stride] = e[i];
+    }
+}
+// The places and weights of choices j0 .. j0 + F of token t, the same for the whole wave.
+template <int F, class W> __device__ __forceinline__ void choices_of(const CombineArgs& a, int64_t t, int j0, int (&p)[F], W (&w)[F]) {
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+        p[j] = -1;
+        w[j] = 0;
+        if (j0 + j < a.fan) {
+            p[j] = a.positions[t * a.fan + j0 + j];
+            if (p[j] >= a.n_rows) p[j] = -1;
+            if (p[j] >= 0) w[j] = a.w ? ((const W*)a.w)[t * a.w_token + (j0 + j) * a.w_fan] : (W)1;
+        }
     }
 }
 
-template <class T>
+template <class T, int F, bool UNIT>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
     typedef typename Num<T>::acc W;
     constexpr int E = Num<T>::E;
-    const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, step = 64 * E * gridDim.y;
+    const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.tokens) return;
-    for (int n = (blockIdx.y * 64 + lane) * E; n < a.n; n += 64 * E * gridDim.y) {
-        W sum[E] = {};
-        for (int j0 = 0; j0 < a.fan; j0 += AT_ONCE) {
-            u32x4 v[AT_ONCE];
-            W w[AT_ONCE];
+    int p[F];
+    W w[F];
+    choices_of(a, t, 0, p, w);
+    for (int n0 = (blockIdx.y * 64 + lane) * E; n0 < a.n; n0 += CHUNKS * step) {
+        W sum[CHUNKS][E] = {};
+        for (int j0 = 0;;) {
+            u32x4 v[F][CHUNKS];
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                w[j] = 0;
-                int p = -1;
-                if (j0 + j < a.fan) {
-                    p = a.positions[t * a.fan + j0 + j];
-                    if (p >= a.n_rows) p = -1;
-                    if (p >= 0) w[j] = a.w ? ((const W*)a.w)[t * a.w_token + (j0 + j) * a.w_fan] : (W)1;
-                }
-                v[j] = load_chunk<T, T>((const T*)a.x + p * a.x_row + n * a.x_n, a.x_n, p >= 0 ? a.n - n : 0);
-            }
+            for (int j = 0; j < F; ++j)
+                if (p[j] >= 0)
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                T e[E];
-                __builtin_memcpy(e, &v[j], 16);
+                    for (int c = 0; c < CHUNKS; ++c) v[j][c] = piece<T, UNIT>((const T*)a.x + p[j] * a.x_row, a.x_n, n0 + c * step, a.n);
 #pragma unroll
-                for (int i = 0; i < E; ++i) sum[i] += w[j] * (W)e[i];
-            }
+            for (int j = 0; j < F; ++j)
+                if (p[j] >= 0)
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        T e[E];
+                        __builtin_memcpy(e, &v[j][c], 16);
+#pragma unroll
+                        for (int i = 0; i < E; ++i) sum[c][i] += w[j] * (W)e[i];
+                    }
+            j0 += F;
+            if (j0 >= a.fan) break;
+            choices_of(a, t, j0, p, w);
         }
-        T out[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[i] = (T)sum[i];
-        store_chunk<T>((T*)a.y + t * a.y_row + n * a.y_n, a.y_n, a.n - n, out);
+        for (int c = 0; c < CHUNKS; ++c) {
+            T out[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) out[i] = (T)sum[c][i];
+            put_piece<T, UNIT>((T*)a.y + t * a.y_row, a.y_n, n0 + c * step, a.n, out);
+        }
+        if (a.fan > F) choices_of(a, t, 0, p, w);
     }
 }
 
-template <class T>
+template <class T, int F, bool UNIT>
 __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, int token_blocks) {
     typedef typename Num<T>::acc W;
-    constexpr int E = Num<T>::E;
+    constexpr int E = Num<T>::E, STEP = 64 * E;
     const int lane = threadIdx.x & 63;
     if ((int)blockIdx.x >= token_blocks) {
         // the rows behind the last group get zeros
@@ -76,53 +102,52 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, 
         const T zero[E] = {};
         const int from = clamp_row(a.offsets[a.n_groups], a.n_rows);
         for (int64_t p = from + ((int)blockIdx.x - token_blocks) * 4 + (threadIdx.x >> 6); p < a.n_rows; p += ((int)gridDim.x - token_blocks) * 4)
-            for (int n = lane * E; n < a.n; n += 64 * E) store_chunk<T>((T*)a.dx + p * a.dx_row + n * a.dx_n, a.dx_n, a.n - n, zero);
+            for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT>((T*)a.dx + p * a.dx_row, a.dx_n, n, a.n, zero);
         return;
     }
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.tokens) return;
-    for (int j0 = 0; j0 < a.fan; j0 += AT_ONCE) {
-        W w[AT_ONCE], dot[AT_ONCE];
-        int p[AT_ONCE];
+    for (int j0 = 0; j0 < a.fan; j0 += F) {
+        W w[F], dot[F] = {};
+        int p[F];
+        choices_of(a, t, j0, p, w);
+        for (int n0 = lane * E; n0 < a.n; n0 += CHUNKS * STEP) {
+            u32x4 d[CHUNKS], v[F][CHUNKS];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            p[j] = -1;
-            w[j] = dot[j] = 0;
-            if (j0 + j < a.fan) {
-                p[j] = a.positions[t * a.fan + j0 + j];
-                if (p[j] >= a.n_rows) p[j] = -1;
-                if (p[j] >= 0) w[j] = a.w ? ((const W*)a.w)[t * a.w_token + (j0 + j) * a.w_fan] : (W)1;
-            }
-        }
-        for (int n = lane * E; n < a.n; n += 64 * E) {
-            const u32x4 d = load_chunk<T, T>((const T*)a.y + t * a.y_row + n * a.y_n, a.y_n, a.n - n);
-            u32x4 v[AT_ONCE];
+            for (int c = 0; c < CHUNKS; ++c) d[c] = piece<T, UNIT>((const T*)a.y + t * a.y_row, a.y_n, n0 + c * STEP, a.n);
             if (a.dw)
 #pragma unroll
-                for (int j = 0; j < AT_ONCE; ++j)
-                    v[j] = load_chunk<T, T>((const T*)a.x + p[j] * a.x_row + n * a.x_n, a.x_n, p[j] >= 0 ? a.n - n : 0);
-            T de[E];
-            __builtin_memcpy(de, &d, 16);
+                for (int j = 0; j < F; ++j)
+                    if (p[j] >= 0)
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                if (p[j] < 0) continue;
-                if (a.dw) {
-                    T e[E];
-                    __builtin_memcpy(e, &v[j], 16);
+                        for (int c = 0; c < CHUNKS; ++c) v[j][c] = piece<T, UNIT>((const T*)a.x + p[j] * a.x_row, a.x_n, n0 + c * STEP, a.n);
 #pragma unroll
-                    for (int i = 0; i < E; ++i) dot[j] += (W)e[i] * (W)de[i];
-                }
-                if (a.dx) {
-                    T out[E];
+            for (int c = 0; c < CHUNKS; ++c) {
+                T de[E];
+                __builtin_memcpy(de, &d[c], 16);
+                // elements that the piece before has: of a row's last piece, which may start before n, and of none behind the row
+                const int n = n0 + c * STEP, seen = !UNIT ? 0 : n >= a.n ? E : n + E > a.n ? n + E - a.n : 0;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) out[i] = (T)(w[j] * (W)de[i]);
-                    store_chunk<T>((T*)a.dx + p[j] * a.dx_row + n * a.dx_n, a.dx_n, a.n - n, out);
+                for (int j = 0; j < F; ++j) {
+                    if (p[j] < 0) continue;
+                    if (a.dw) {
+                        T e[E];
+                        __builtin_memcpy(e, &v[j][c], 16);
+#pragma unroll
+                        for (int i = 0; i < E; ++i) dot[j] += i >= seen ? (W)e[i] * (W)de[i] : (W)0;
+                    }
+                    if (a.dx) {
+                        T out[E];
+#pragma unroll
+                        for (int i = 0; i < E; ++i) out[i] = (T)(w[j] * (W)de[i]);
+                        put_piece<T, UNIT>((T*)a.dx + p[j] * a.dx_row, a.dx_n, n, a.n, out);
+                    }
                 }
             }
         }
         if (a.dw) {
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
+            for (int j = 0; j < F; ++j) {
 #pragma unroll
                 for (int s = 1; s < 64; s <<= 1) dot[j] += __shfl_xor(dot[j], s, 64);
                 if (lane == 0 && j0 + j < a.fan) ((W*)a.dw)[t * a.dw_token + (j0 + j) * a.dw_fan] = dot[j];
@@ -135,18 +160,29 @@ template <class T> constexpr const char* name_of(const char* bf16, const char* f
     return __is_same(T, __bf16) ? bf16 : __is_same(T, _Float16) ? f16 : __is_same(T, float) ? f32 : f64;
 }
 
-template <class T> int32_t combine_of(const CombineArgs& a, hipStream_t st) {
+template <class T, int F, bool UNIT> int32_t combine_as(const CombineArgs& a, hipStream_t st) {
     const int64_t blocks = (a.tokens + 3) / 4, pieces = (a.n + 64 * Num<T>::E - 1) / (64 * Num<T>::E);
     // few tokens: their columns are dealt to several blocks, so that more waves wait for memory
     const int64_t split = blocks >= 512 ? 1 : pieces < 512 / blocks ? pieces : 512 / blocks;
-    TFH_LAUNCH_NAMED(name_of<T>("(combine_kernel<bf16>)", "(combine_kernel<f16>)", "(combine_kernel<float>)", "(combine_kernel<double>)"), combine_kernel<T>, dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
+    TFH_LAUNCH_NAMED(name_of<T>("(combine_kernel<bf16>)", "(combine_kernel<f16>)", "(combine_kernel<float>)", "(combine_kernel<double>)"),
+                     (combine_kernel<T, F, UNIT>), dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
     return hip_check(hipGetLastError(), "combine launch");
 }
-template <class T> int32_t combine_grad_of(const CombineArgs& a, hipStream_t st) {
+template <class T, int F, bool UNIT> int32_t combine_grad_as(const CombineArgs& a, hipStream_t st) {
     const int64_t blocks = (a.tokens + 3) / 4, rest = a.n_rows < 256 ? (a.n_rows + 3) / 4 : 64;
     TFH_LAUNCH_NAMED(name_of<T>("(combine_grad_kernel<bf16>)", "(combine_grad_kernel<f16>)", "(combine_grad_kernel<float>)", "(combine_grad_kernel<double>)"),
-                     combine_grad_kernel<T>, dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
+                     (combine_grad_kernel<T, F, UNIT>), dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
     return hip_check(hipGetLastError(), "combine gradient launch");
+}
+template <class T> int32_t combine_of(const CombineArgs& a, hipStream_t st) {
+    const bool unit = a.x_n == 1 && a.y_n == 1 && a.n >= Num<T>::E;
+    if (!unit) return combine_as<T, 4, false>(a, st);
+    return a.fan <= 2 ? combine_as<T, 2, true>(a, st) : a.fan <= 4 ? combine_as<T, 4, true>(a, st) : combine_as<T, 8, true>(a, st);
+}
+template <class T> int32_t combine_grad_of(const CombineArgs& a, hipStream_t st) {
+    const bool unit = (!a.dw || a.x_n == 1) && a.y_n == 1 && (!a.dx || a.dx_n == 1) && a.n >= Num<T>::E;
+    if (!unit) return combine_grad_as<T, 4, false>(a, st);
+    return a.fan <= 2 ? combine_grad_as<T, 2, true>(a, st) : a.fan <= 4 ? combine_grad_as<T, 4, true>(a, st) : combine_grad_as<T, 8, true>(a, st);
 }
 
 }  // namespace

@@ -5,8 +5,9 @@
 //
 // No atomic decides an order: a wave takes its rows 64 at a time, the lanes of one index find each other with one ballot
 // per bit of it, and the rows of earlier lanes, waves and blocks are counted before.  Up to SMALL_ROWS rows it is one
-// launch of one block; beyond that three (counts per block and group, their prefix along the blocks, the placing).
-// What bounds it: the small form is latency (a load, two passes over LDS counters, a store); the large one the three
+// launch of one block; beyond that two (counts per block and group; the placing, each block of which adds up what the blocks
+// before it have), or, where that would be many counts to read for every block, three (their prefix along the blocks between).
+// What bounds it: the small form is latency (a load, two passes over LDS counters, a store); the large one the
 // launches, each of which moves a few megabytes.
 #include <hip/hip_runtime.h>
 
@@ -19,8 +20,11 @@ namespace {
 
 constexpr int WAVES = 16, THREADS = WAVES * 64;
 constexpr int ROUNDS = 8;                              // 64 rows each, a wave's share of a block
-constexpr int BLOCK_ROWS = WAVES * 64 * ROUNDS;        // 8192
-constexpr int SMALL_ROWS = BLOCK_ROWS;
+constexpr int FEW_ROUNDS = 4;                          // the same where a block's counters are few (FEW_BINS): twice the blocks
+constexpr int FEW_BINS = 320;
+constexpr int SMALL_ROWS = WAVES * 64 * ROUNDS;        // 8192
+constexpr int64_t JOINED_COUNTS = 1 << 14;             // counts that every placing block reads by itself
+constexpr int rounds_for(int64_t bins) { return bins <= FEW_BINS ? FEW_ROUNDS : ROUNDS; }
 
 __device__ __forceinline__ int key_of(const GroupArgs& a, int i) {
     const int64_t at = a.inner == 1 ? (int64_t)i * a.s_outer : (int64_t)(i / a.inner) * a.s_outer + (int64_t)(i % a.inner) * a.s_inner;
@@ -52,57 +56,87 @@ __device__ void prefix(int* v, int bins, int* sums) {
     __syncthreads();
 }
 
-// counts[bin][block] -> how many rows of the bin the earlier blocks have; the bin's total behind them at [bins][...].
-__global__ __launch_bounds__(256) void group_count_kernel(const GroupArgs a) {
+template <int R> __global__ __launch_bounds__(THREADS) void group_count_kernel(const GroupArgs a) {
     extern __shared__ int lds_i[];
     const int bins = a.n_groups + 1;
-    for (int b = threadIdx.x; b < bins; b += 256) lds_i[b] = 0;
-    __syncthreads();
-    const int64_t from = (int64_t)blockIdx.x * BLOCK_ROWS;
-#pragma unroll 4
-    for (int r = threadIdx.x; r < BLOCK_ROWS; r += 256)
-        if (from + r < a.n_rows) atomicAdd(&lds_i[key_of(a, (int)(from + r))], 1);   // whole numbers: any order, one result
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256) a.counts[(int64_t)b * a.blocks + blockIdx.x] = lds_i[b];
-}
-__global__ __launch_bounds__(64) void group_prefix_kernel(const GroupArgs a) {
-    int* const row = a.counts + (int64_t)blockIdx.x * a.blocks;
-    const int lane = threadIdx.x;
-    int before = 0;
-    for (int b0 = 0; b0 < a.blocks; b0 += 64) {
-        const int c = b0 + lane < a.blocks ? row[b0 + lane] : 0;
-        int upto = c;
+    const int64_t from = (int64_t)blockIdx.x * THREADS * R + threadIdx.x;
+    int key[R];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += o;
-        }
-        if (b0 + lane < a.blocks) row[b0 + lane] = before + upto - c;
-        before += __shfl(upto, 63, 64);
+    for (int r = 0; r < R; ++r) key[r] = from + r * THREADS < a.n_rows ? key_of(a, (int)(from + r * THREADS)) : -1;
+    for (int b = threadIdx.x; b < bins; b += THREADS) lds_i[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (key[r] >= 0) atomicAdd(&lds_i[key[r]], 1);   // whole numbers: any order, one result
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += THREADS) a.counts[(int64_t)blockIdx.x * bins + b] = lds_i[b];
+}
+// counts[block][bin] -> how many rows of the bin the earlier blocks have; the bins' totals behind the last block's.  A lane a
+// bin; the blocks are shared out to the waves.
+__global__ __launch_bounds__(THREADS) void group_prefix_kernel(const GroupArgs a) {
+    __shared__ int sums[WAVES][64];
+    const int bins = a.n_groups + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x * 64 + lane;
+    const int per = (a.blocks + WAVES - 1) / WAVES, from = wave * per, to = from + per < a.blocks ? from + per : a.blocks;
+    int mine = 0;
+    if (b < bins)
+#pragma unroll 8
+        for (int k = from; k < to; ++k) mine += a.counts[(int64_t)k * bins + b];
+    sums[wave][lane] = mine;
+    __syncthreads();
+    if (b >= bins) return;
+    int before = 0;
+    for (int w = 0; w < wave; ++w) before += sums[w][lane];
+#pragma unroll 8
+    for (int k = from; k < to; ++k) {
+        const int c = a.counts[(int64_t)k * bins + b];
+        a.counts[(int64_t)k * bins + b] = before;
+        before += c;
     }
-    if (lane == 0) a.counts[(int64_t)(a.n_groups + 1) * a.blocks + blockIdx.x] = before;
+    if (wave == WAVES - 1) a.counts[(int64_t)a.blocks * bins + b] = before;
 }
 
-template <bool SMALL>
+enum Counted { NONE = 0, JOINED = 1, PREFIXED = 2 };   // one block; counts to add up; their prefixes
+template <int COUNTED, int R>
 __global__ __launch_bounds__(THREADS) void group_place_kernel(const GroupArgs a) {
-    extern __shared__ int lds_i[];   // [bins] first places, [16], then [waves][bins] counters
+    extern __shared__ int lds_i[];   // [bins] first places, [16], [waves][bins] counters, [bins] what earlier blocks have (not NONE)
     const int bins = a.n_groups + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int* const start = lds_i;
     int* const sums = lds_i + bins;
     int* const count = lds_i + bins + 16 + wave * bins;
     int* const counts = lds_i + bins + 16;
     int bits = 32 - __builtin_clz(a.n_groups);
-    const int64_t first = (int64_t)blockIdx.x * BLOCK_ROWS + wave * (64 * ROUNDS);
-    int key[ROUNDS];
+    const int64_t first = (int64_t)blockIdx.x * THREADS * R + wave * (64 * R);
+    int key[R];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
+    for (int r = 0; r < R; ++r) {
         const int64_t i = first + r * 64 + lane;
         key[r] = i < a.n_rows ? key_of(a, (int)i) : -1;
     }
+    int* const before = counts + WAVES * bins;
     for (int i = tid; i < bins * WAVES; i += THREADS) counts[i] = 0;
+    if constexpr (COUNTED == JOINED)
+        for (int b = tid; b < bins; b += THREADS) start[b] = before[b] = 0;
+    if constexpr (COUNTED == PREFIXED)
+        for (int b = tid; b < bins; b += THREADS)
+            start[b] = a.counts[(int64_t)a.blocks * bins + b], before[b] = a.counts[(int64_t)blockIdx.x * bins + b];
     __syncthreads();
+    if constexpr (COUNTED == JOINED) {
+        // the blocks' counts, bins next to each other: (THREADS / P) bins at a time
+        const int width = bins <= 64 ? 64 : bins <= 128 ? 128 : 256, part = tid / width, parts = THREADS / width;
+        for (int b = tid % width; b < bins; b += width) {
+            int earlier = 0, later = 0;
+#pragma unroll 16
+            for (int k = part; k < a.blocks; k += parts) {
+                const int c = a.counts[(int64_t)k * bins + b];
+                if (k < (int)blockIdx.x) earlier += c;
+                else later += c;
+            }
+            atomicAdd(&before[b], earlier);
+            atomicAdd(&start[b], earlier + later);
+        }
+    }
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
+    for (int r = 0; r < R; ++r)
         if (key[r] >= 0) atomicAdd(&count[key[r]], 1);
     __syncthreads();
     // per bin: this block's first place in it, and each wave's
@@ -113,16 +147,16 @@ __global__ __launch_bounds__(THREADS) void group_place_kernel(const GroupArgs a)
             counts[w * bins + b] = n;
             n += c;
         }
-        start[b] = SMALL ? n : a.counts[(int64_t)bins * a.blocks + b];
+        if (COUNTED == NONE) start[b] = n;
     }
     __syncthreads();
     prefix(start, bins, sums);
     if (blockIdx.x == 0)
         for (int b = tid; b < bins; b += THREADS) a.offsets[b] = start[b];
-    for (int b = lane; b < bins; b += 64) count[b] += start[b] + (SMALL ? 0 : a.counts[(int64_t)b * a.blocks + blockIdx.x]);
+    for (int b = lane; b < bins; b += 64) count[b] += start[b] + (COUNTED == NONE ? 0 : before[b]);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
+    for (int r = 0; r < R; ++r) {
         if (first + r * 64 >= a.n_rows) break;
         const bool here = key[r] >= 0;
         uint64_t same = __ballot(here);
@@ -146,26 +180,34 @@ __global__ __launch_bounds__(THREADS) void group_place_kernel(const GroupArgs a)
 
 size_t group_rows_workspace(int64_t n_rows, int32_t n_groups) {
     if (n_rows <= SMALL_ROWS) return 0;
-    const int64_t blocks = (n_rows + BLOCK_ROWS - 1) / BLOCK_ROWS;
+    const int64_t each = THREADS * rounds_for(n_groups + 1), blocks = (n_rows + each - 1) / each;
     return (size_t)(n_groups + 1) * (blocks + 1) * sizeof(int32_t);
 }
 
+namespace {
+template <int COUNTED, int R> void launch_place(const GroupArgs& a, hipStream_t st) {
+    const int bins = a.n_groups + 1, lds = (bins * (WAVES + 1 + (COUNTED != NONE)) + 16) * (int)sizeof(int);
+    if (lds > 64 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&group_place_kernel<COUNTED, R>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    TFH_LAUNCH_NAMED("(group_place_kernel)", (group_place_kernel<COUNTED, R>), dim3((unsigned)a.blocks), dim3(THREADS), lds, st, a);
+}
+template <int R> void launch_large(const GroupArgs& a, hipStream_t st) {
+    const int bins = a.n_groups + 1;
+    hipLaunchKernelGGL(group_count_kernel<R>, dim3((unsigned)a.blocks), dim3(THREADS), bins * sizeof(int), st, a);
+    if (bins * a.blocks <= JOINED_COUNTS) return launch_place<JOINED, R>(a, st);
+    hipLaunchKernelGGL(group_prefix_kernel, dim3((bins + 63) / 64), dim3(THREADS), 0, st, a);
+    launch_place<PREFIXED, R>(a, st);
+}
+}  // namespace
+
 int32_t launch_group_rows(GroupArgs a, void* stream) {
     hipStream_t st = (hipStream_t)stream;
-    const int bins = a.n_groups + 1;
-    a.blocks = a.n_rows > 0 ? (a.n_rows + BLOCK_ROWS - 1) / BLOCK_ROWS : 1;
-    const int lds = (bins * (WAVES + 1) + 16) * (int)sizeof(int);
-    if (lds > 64 * 1024) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&group_place_kernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&group_place_kernel<false>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    }
-    if (a.n_rows <= SMALL_ROWS) {
-        TFH_LAUNCH_TIMED(group_place_kernel<true>, dim3(1), dim3(THREADS), lds, st, a);
-    } else {
-        hipLaunchKernelGGL(group_count_kernel, dim3(a.blocks), dim3(256), bins * sizeof(int), st, a);
-        hipLaunchKernelGGL(group_prefix_kernel, dim3(bins), dim3(64), 0, st, a);
-        TFH_LAUNCH_TIMED(group_place_kernel<false>, dim3(a.blocks), dim3(THREADS), lds, st, a);
-    }
+    const int rounds = rounds_for(a.n_groups + 1), each = THREADS * rounds;
+    a.blocks = a.n_rows <= SMALL_ROWS ? 1 : (a.n_rows + each - 1) / each;
+    if (a.n_rows <= THREADS) launch_place<NONE, 1>(a, st);
+    else if (a.n_rows <= SMALL_ROWS) launch_place<NONE, ROUNDS>(a, st);
+    else if (rounds == ROUNDS) launch_large<ROUNDS>(a, st);
+    else launch_large<FEW_ROUNDS>(a, st);
     return hip_check(hipGetLastError(), "row grouping launch");
 }
 

@@ -17,7 +17,7 @@ struct GroupArgs {
     int32_t* offsets;
     int32_t* order;
     int32_t* positions;       // may be null
-    int32_t* counts;          // [n_groups + 1][blocks] in the workspace (more than one block)
+    int32_t* counts;          // [blocks + 1][n_groups + 1] in the workspace (more than one block)
     int32_t blocks;
 };
 size_t group_rows_workspace(int64_t n_rows, int32_t n_groups);
