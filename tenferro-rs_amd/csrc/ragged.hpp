@@ -242,6 +242,40 @@ __device__ __forceinline__ bool find_tile(const Args& a, int tm, int tiles_n, ui
     }
     return false;
 }
+// Outer products: every group has as many tiles, but each takes as long as the group has rows.  They are dealt to the XCDs in
+// patches of up to 4 x 4, which share operands in an XCD's L2, the longest group's first (of up to 64 groups; of more, one
+// wave's worth of sorting, the sums even out) and forth and back over the XCDs, so that all of them end at about the same time.
+struct Patches {
+    int tm, tn, pm, pn, across, each;   // a group's tiles, a patch's, patches along M, patches of a group
+    __host__ __device__ Patches(const Args& a, int TM, int TN) {
+        tm = (a.M + TM - 1) / TM, tn = (a.N + TN - 1) / TN;
+        pm = tm < 4 ? tm : 4, pn = tn < 4 ? tn : 4;
+        across = (tm + pm - 1) / pm, each = across * ((tn + pn - 1) / pn);
+    }
+    __host__ __device__ int64_t blocks(int n_groups) const { return ((int64_t)n_groups * each + 7) / 8 * 8 * (pm * pn); }
+};
+__device__ __forceinline__ bool outer_tile(const Args& a, int TM, int TN, uint32_t block, Tile& t) {
+    const Patches s(a, TM, TN);
+    const uint32_t size = s.pm * s.pn, xcd = block % gemm::XCDS, at = block / gemm::XCDS, turn = at / size, w = at % size;
+    const uint32_t patch = turn * gemm::XCDS + (turn & 1 ? gemm::XCDS - 1 - xcd : xcd);
+    if (patch >= (uint32_t)a.n_groups * s.each) return false;
+    const uint32_t rank = patch / s.each, u = patch % s.each;
+    t.tile_m = (u % s.across) * s.pm + w % s.pm, t.tile_n = (u / s.across) * s.pn + w / s.pm;
+    if (t.tile_m >= s.tm || t.tile_n >= s.tn) return false;
+    t.group = rank;
+    if (a.n_groups <= 64) {
+        const int lane = threadIdx.x & 63;
+        const int from = lane < a.n_groups ? clamp_row(a.offsets[lane], a.n_rows) : 0, to = lane < a.n_groups ? clamp_row(a.offsets[lane + 1], a.n_rows) : 0;
+        const int64_t mine = lane < a.n_groups ? (int64_t)(to > from ? to - from : 0) * 64 + 63 - lane : -1;
+        uint32_t longer = 0;
+        for (int g = 0; g < a.n_groups; ++g) longer += __shfl(mine, g, 64) > mine;
+        t.group = __builtin_ctzll(__ballot(longer == rank && lane < a.n_groups));
+    }
+    t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows));
+    const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group + 1], a.n_rows));
+    t.rows = to > t.first ? to - t.first : 0;
+    return true;
+}
 // The group that holds row p (clamped offsets ascending), n_groups for the rows behind the last one.
 __device__ __forceinline__ int group_of(const Args& a, int p) {
     int lo = 0, hi = a.n_groups;   // the first group that ends behind p
@@ -389,13 +423,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
     if constexpr (MODE == ROWS) {
         if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
     } else if constexpr (MODE == OUTER) {
-        const int tiles_m = (a.M + TM - 1) / TM;
-        const uint64_t id = gemm::logical_block(blockIdx.x, gridDim.x);
-        t.group = (int)(id / ((uint64_t)tiles_m * tiles_n));
-        gemm::tile_of((uint32_t)(id % ((uint64_t)tiles_m * tiles_n)), tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.first = clamp_row(a.offsets[t.group], a.n_rows);
-        const int to = clamp_row(a.offsets[t.group + 1], a.n_rows);
-        t.rows = to > t.first ? to - t.first : 0;
+        if (!outer_tile(a, TM, TN, blockIdx.x, t)) return;
     } else {
         const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
         gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);

@@ -126,10 +126,17 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     uint32_t va[CA], vb[CB];
     u32x4 A, B;
     uint32_t step_a = BK * 2, step_b = BK * 2;     // bytes from a stage to the next
-    int32_t next_row = -1;                         // outer, gathered: lane l holds the row of A for the next stage's l-th k
+    // Outer, gathered: where the rows of A for the stages to come start, in bytes (NOWHERE: there is none), 64 a register, the next ones in the first.  The compiler's wait for
+    // what is looked up here waits for the loads into LDS too, so it is LOOK x 64 rows at once and seldom.
+    constexpr int LOOK = 4;
+    uint32_t next_rows[LOOK];
     auto look_up = [&](int k0) {
-        if constexpr (!AKFAST)
-            if (a.gather && a.order) next_row = k0 + lane < kend ? (int)source_row(a, t.first + k0 + lane) : -1;
+#pragma unroll
+        for (int i = 0; i < LOOK; ++i) {
+            const int k = k0 + 64 * i + lane;
+            const int row = k < kend ? (int)source_row(a, t.first + k) : -1;
+            next_rows[i] = row >= 0 ? (uint32_t)row * (uint32_t)(a.a_row * 2) : NOWHERE;
+        }
     };
     if constexpr (AKFAST) {
         A = buffer_of(a.A, (uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2));
@@ -149,7 +156,6 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
             const int id = tid + 256 * i, k = id / RA, m = m0 + ((id % RA) ^ (rowfast_swizzle<T>(k) & (RA - 1))) * 8;
             va[i] = m < a.M ? (gather ? 0 : (uint32_t)(k * a.a_row * 2)) + m * 2 : NOWHERE;
         }
-        look_up(0);
     }
     if constexpr (BKFAST) {
         B = buffer_of((const char*)a.B + (MODE == ROWS && real ? t.group * a.b_group * 2 : 0), (uint32_t)((a.N - 1) * a.b_n * 2 + a.K * 2));
@@ -194,12 +200,25 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         }
         if constexpr (!AKFAST) {
             if (a.gather && a.order && s < stages) {
+                const int k0 = s * BK;
+                if (k0 % (64 * LOOK) == 0) {
+                    look_up(k0);
+                } else if (k0 % 64 == 0) {
+#pragma unroll
+                    for (int i = 0; i + 1 < LOOK; ++i) next_rows[i] = next_rows[i + 1];
+                }
 #pragma unroll
                 for (int i = 0; i < CA; ++i) {
-                    const int row = __shfl(next_row, (tid + 256 * i) / RA, 64);   // (-1 behind the group's last row)
-                    now.va[i] = row >= 0 && va[i] != NOWHERE ? va[i] + (uint32_t)row * (uint32_t)(a.a_row * 2) : NOWHERE;
+                    uint32_t row;   // (a wave's chunks are of two or four rows)
+                    if constexpr (RA == 32) {
+                        const int k = k0 % 64 + 2 * wave + 8 * i;
+                        const uint32_t r0 = __builtin_amdgcn_readlane(next_rows[0], k), r1 = __builtin_amdgcn_readlane(next_rows[0], k + 1);
+                        row = lane < 32 ? r0 : r1;
+                    } else {
+                        row = __shfl(next_rows[0], k0 % 64 + (tid + 256 * i) / RA, 64);
+                    }
+                    now.va[i] = __builtin_elementwise_add_sat(va[i], row);   // what is nowhere stays there
                 }
-                look_up((s + 1) * BK);
             }
         }
         if (s >= stages - 1) {
@@ -514,13 +533,7 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
             }
         }
     } else if constexpr (MODE == OUTER || MODE == PAIR) {
-        const int tiles_m = (a.M + TM - 1) / TM;
-        const uint32_t id = (uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), each = (uint32_t)tiles_m * tiles_n;
-        t.group = (int)(id / each);
-        gemm::tile_of(id % each, tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.first = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group], a.n_rows));
-        const int to = __builtin_amdgcn_readfirstlane(clamp_row(a.offsets[t.group + 1], a.n_rows));
-        t.rows = to > t.first ? to - t.first : 0;
+        if (!outer_tile(a, TM, TN, blockIdx.x, t)) return;
     } else {
         const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
         gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);

@@ -32,7 +32,7 @@ template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNI
 int32_t launch_general_tiles(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, 32 * YT);
     const int64_t blocks = MODE == ROWS ? row_tiles(a, 32 * XT) * tn
-                           : MODE == OUTER ? a.n_groups * tiles(a.M, 32 * XT) * tn : tiles(a.n_rows, 32 * XT) * tn;
+                           : MODE == OUTER ? Patches(a, 32 * XT, 32 * YT).blocks(a.n_groups) : tiles(a.n_rows, 32 * XT) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
     static const std::string label = std::string("(ragged_general_kernel<") + type_name<TA>() + ", " + type_name<TB>() + ", " + type_name<C>() + ", " +
@@ -69,7 +69,7 @@ template <class T, int MODE, bool BKFAST, class S>
 int32_t launch_fast(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, S::TN);
     const int64_t blocks = MODE == ROWS || (MODE == SHARED && S::BY_GROUP) ? row_tiles(a, S::TM) * tn
-                           : MODE == OUTER || MODE == PAIR ? a.n_groups * tiles(a.M, S::TM) * tn : tiles(a.n_rows, S::TM) * tn;
+                           : MODE == OUTER || MODE == PAIR ? Patches(a, S::TM, S::TN).blocks(a.n_groups) : tiles(a.n_rows, S::TM) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
     static const bool once = [] {
@@ -83,7 +83,7 @@ int32_t launch_fast(const Args& a, void* stream) {
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 typedef Shape<2, 2, 4, 4, 128, 3, 2> Large;     // 256 x 256
-typedef Shape<2, 2, 4, 4, 64, 5, 5> LargeOuter;
+typedef Shape<2, 2, 4, 2, 64, 3, 3> LargeOuter;
 typedef Shape<2, 2, 2, 2> Middle;   // 128 x 128
 typedef Shape<1, 4, 1, 1> Small;    // 32 x 128
 template <class T, int MODE, bool BKFAST>
