@@ -435,12 +435,26 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
                 }
         }
         __syncthreads();
+        // four columns a thread; the direction in which the result is contiguous goes along the lanes
         const int rows = a.M - m0 < TM ? a.M - m0 : TM;
-        const bool down = a.c_row == 1;   // the direction in which the result is contiguous goes along the lanes
-        auto at = [&](int r, int c) { return *(const float*)(lds + r * (TN * 4) + (((c >> 2) ^ (r & 15)) << 4) + (c & 3) * 4); };
-        for (int id = tid; id < rows * a.r; id += 256) {
-            const int r = down ? id % rows : id / a.r, c = down ? id / rows : id % a.r;
-            ((T*)a.C)[t.group * a.c_group + (m0 + r) * a.c_row + c * a.c_n] = (T)(alpha * (at(r, c) + at(r, c + a.pad)));
+        const bool down = a.c_row == 1, across = a.c_n == 1 && a.c_row % 4 == 0 && a.c_group % 4 == 0 && ((uintptr_t)a.C & 7) == 0;
+        for (int id = tid; id < TM * 16; id += 256) {
+            const int r = down ? id % TM : id / 16, c = 4 * (down ? id / TM : id % 16);
+            if (r >= rows || c >= a.r) continue;
+            const char* const row = lds + r * (TN * 4);
+            const f32x4 hi = *(const f32x4*)(row + (((c >> 2) ^ (r & 15)) << 4));
+            const f32x4 lo = *(const f32x4*)(row + ((((c + a.pad) >> 2) ^ (r & 15)) << 4));
+            T* const out = (T*)a.C + t.group * a.c_group + (m0 + r) * a.c_row + c * a.c_n;
+            T v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (T)(alpha * (hi[i] + lo[i]));
+            if (across && c + 4 <= a.r) {
+                __builtin_memcpy(out, v, 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < a.r) out[i * a.c_n] = v[i];
+            }
         }
         return;
     }
@@ -520,8 +534,8 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
         if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
         if constexpr (TM == 256) {
             // a group's last tile is seldom full: half or a quarter of the rows in half or 0.4 of the time
-            typedef Shape<1, 4, 2, 2, S::KB, S::SA, S::SB> Quarter;
-            typedef Shape<2, 2, 2, 4, S::KB, S::SA, S::SB> Half;
+            typedef Shape<1, 4, 2, S::YT / 2, S::KB, S::SA, S::SB> Quarter;
+            typedef Shape<2, 2, 2, S::YT, S::KB, S::SA, S::SB> Half;
             static_assert(Quarter::TN == TN && Half::TN == TN && Half::LDS <= S::LDS, "the same columns");
             if (t.rows <= 64) {
                 fast_tile<T, MODE, BKFAST, Quarter, true>(a, t, lds);

@@ -83,13 +83,23 @@ int32_t launch_fast(const Args& a, void* stream) {
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 typedef Shape<2, 2, 4, 4, 128, 3, 2> Large;     // 256 x 256
-typedef Shape<2, 2, 4, 2, 64, 3, 3> LargeOuter;
+typedef Shape<2, 2, 4, 2, 64, 3, 3> Tall;      // 256 x 128, two to a compute unit
 typedef Shape<2, 2, 2, 2> Middle;   // 128 x 128
+typedef Shape<2, 2, 1, 2, 128, 3, 3> Slim;   // 64 x 128
 typedef Shape<1, 4, 1, 1> Small;    // 32 x 128
+// Whether tiles of 256 x 256, one to a compute unit, come in rounds of the machine's 256 units that are nearly full.  If not,
+// tiles of half the columns, two to a unit, take a tenth longer for the same work and leave less of the machine idle (bf16, 32
+// groups of 32 768 rows, uneven, 2048 x 1024, two and a quarter rounds: 154 us against 174; 65 536 rows, 2048 x 2048, nine
+// rounds: 633 against 582).  Of the groups' last tiles one half is full on average.
+inline bool fills_rounds(const Args& a) {
+    const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
+    const int64_t tn = tiles(a.N, 256), t = groups > 1 ? (a.n_rows * 2 / 256 + groups) * tn / 2 : tiles(a.n_rows, 256) * tn;
+    return tiles(t, 256) * 256 * 5 < t * 6;
+}
 template <class T, int MODE, bool BKFAST>
 int32_t launch_shape(const Args& a, void* stream) {
     const int64_t rows = MODE == OUTER ? a.M : a.n_rows / a.n_groups;
-    if (rows > 192) return launch_fast<T, MODE, BKFAST, std::conditional_t<MODE == OUTER, LargeOuter, Large>>(a, stream);
+    if (rows > 192) return MODE == OUTER || !fills_rounds(a) ? launch_fast<T, MODE, BKFAST, Tall>(a, stream) : launch_fast<T, MODE, BKFAST, Large>(a, stream);
     if (rows > 48) return launch_fast<T, MODE, BKFAST, Middle>(a, stream);
     return launch_fast<T, MODE, BKFAST, Small>(a, stream);
 }
@@ -101,7 +111,7 @@ int32_t launch_shared(const Args& a, void* stream) {
         if (a.n_rows / (a.n_groups + 1) > 192) {
             Args g = a;
             g.zero_rest = 1;
-            return launch_fast<T, SHARED, BKFAST, Large>(g, stream);
+            return fills_rounds(g) ? launch_fast<T, SHARED, BKFAST, Large>(g, stream) : launch_fast<T, SHARED, BKFAST, Tall>(g, stream);
         }
     return launch_fast<T, SHARED, BKFAST, Middle>(a, stream);
 }
@@ -154,7 +164,9 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         if (kind == PRODUCT_SHARED && a.pad > 0 && !columns && few_takes<SHARED>(a) && tiles(a.n_rows, 64) * tiles(a.N, 16) <= 1024)
             return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream) : launch_few<T, SHARED, 4>(a, stream);
         if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_shared<T, false>(a, stream) : launch_shared<T, true>(a, stream);
-        if (kind == PRODUCT_OUTER_V && a.pad > 0) return launch_fast<T, PAIR, false, Middle>(a, stream);
+        // (eight groups of 4096 rows, 4096 and 2048 x 64: 26 us in tiles of 64 rows, three stages on their way, 34 in those of 128)
+        if (kind == PRODUCT_OUTER_V && a.pad > 0)
+            return a.n_groups * tiles(a.M, 128) < 512 ? launch_fast<T, PAIR, false, Slim>(a, stream) : launch_fast<T, PAIR, false, Middle>(a, stream);
         if (kind == PRODUCT_MIDDLE && thin_takes(a, !columns)) {
             if (columns) return a.N <= 32 ? launch_thin<T, false, 1>(a, stream) : a.N <= 64 ? launch_thin<T, false, 2>(a, stream) : launch_thin<T, false, 4>(a, stream);
             return a.N <= 32 ? launch_thin<T, true, 1>(a, stream) : a.N <= 64 ? launch_thin<T, true, 2>(a, stream) : launch_thin<T, true, 4>(a, stream);
