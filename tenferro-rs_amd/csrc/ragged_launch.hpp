@@ -87,14 +87,17 @@ typedef Shape<2, 2, 4, 2, 64, 3, 3> Tall;      // 256 x 128, two to a compute un
 typedef Shape<2, 2, 2, 2> Middle;   // 128 x 128
 typedef Shape<2, 2, 1, 2, 128, 3, 3> Slim;   // 64 x 128
 typedef Shape<1, 4, 1, 1> Small;    // 32 x 128
-// Whether tiles of 256 x 256, one to a compute unit, come in rounds of the machine's 256 units that are nearly full.  If not,
-// tiles of half the columns, two to a unit, take a tenth longer for the same work and leave less of the machine idle (bf16, 32
-// groups of 32 768 rows, uneven, 2048 x 1024, two and a quarter rounds: 154 us against 174; 65 536 rows, 2048 x 2048, nine
-// rounds: 633 against 582).  Of the groups' last tiles one half is full on average.
+// Whether tiles of 256 x 256, one to a compute unit, come in rounds of the machine's 256 units that are full enough.  If not,
+// tiles of half the columns, two to a unit: those take a tenth longer for the same work where k is 2048, a fifth from 4096 on and
+// hardly any where it is short, since one works while the other starts or ends, and leave less of the machine idle.  (bf16, uneven
+// groups, large and tall tiles: 65 536 rows of 64, 2048 x 2048, nine rounds: 582 and 633 us; 32 768 of 32, 1024 x 2048, four and a
+// half: 187 and 168; 8192 of 16, 2048 x 2048, one and a quarter: 104 and 91; 4096 of 8, 0.6: 54 and 56.)  Of the groups' last
+// tiles one half is full on average.
 inline bool fills_rounds(const Args& a) {
     const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
     const int64_t tn = tiles(a.N, 256), t = groups > 1 ? (a.n_rows * 2 / 256 + groups) * tn / 2 : tiles(a.n_rows, 256) * tn;
-    return tiles(t, 256) * 256 * 5 < t * 6;
+    const int64_t k = a.K < 4096 ? a.K : 4096;
+    return t < 256 ? t > 128 : tiles(t, 256) * 256 * 20480 <= t * (20480 + k);
 }
 template <class T, int MODE, bool BKFAST>
 int32_t launch_shape(const Args& a, void* stream) {
