@@ -147,6 +147,21 @@ def test_grouping_reads_strided_indices(tf, torch):
         assert g.offsets.tolist() == offsets and g.order.tolist() == order and g.positions.tolist() == positions
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,fan,groups", [(1025, 1, 3), (150000, 2, 256), (16385, 1, 319), (20000, 1, 320), (300000, 1, 2048)])
+def test_grouping_of_many_rows(tf, torch, tokens, fan, groups):
+    rng = np.random.default_rng(groups)
+    ids = torch.from_numpy(rng.integers(-1, groups + 1, (tokens, fan))).cuda()
+    g = tf.RowGroups.from_ids(ids, groups)
+    flat = torch.where((ids.reshape(-1) < 0) | (ids.reshape(-1) >= groups), groups, ids.reshape(-1))
+    key, order = torch.sort(flat, stable=True)
+    positions = torch.empty_like(order)
+    positions[order] = torch.arange(len(order), device="cuda")
+    assert torch.equal(g.order.long(), order)
+    assert torch.equal(g.offsets.long(), torch.searchsorted(key, torch.arange(groups + 1, device="cuda")))
+    assert torch.equal(g.positions.long(), torch.where(flat < groups, positions, -1))
+
+
 # ------------------------------------------------------------------------------------------------------ products
 def ragged_reference(torch, a, b, offsets, order, fan, gather):
     """c and the sums of absolute values, zeros for rows of no group."""
@@ -361,6 +376,49 @@ def test_ragged_product_of_uneven_groups_of_many_rows(tf, torch, name):
         close(db, torch.stack([A[s].t() @ D[s] for s in cut]), torch.stack([A[s].abs().t() @ D[s].abs() for s in cut]), 1023, name)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("K,N", [(136, 2600), (135, 2599), (20, 12008), (1100, 130)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_ragged_product_in_tiles_of_every_size(tf, torch, name, K, N, how):
+    # wide results of many rows, short and long sums, rows that start 16-byte aligned and rows that do not; the reference in blocks
+    rng = np.random.default_rng(K)
+    counts = [0, 1, 1023, 0, 257, 256, 5, 128, 600, 0, 31]
+    offsets, rows = np.cumsum([0] + counts), sum(counts)
+    a, b, dc = tensor(torch, rng, (rows, K), name), tensor(torch, rng, (len(counts), K, N), name, K ** -0.5), tensor(torch, rng, (rows, N), name)
+    g = tf.RowGroups(torch.tensor(offsets, dtype=torch.int32, device="cuda"), n_rows=rows)
+    got = tf.ragged_gemm(a.cuda(), layout(torch, b, how), g)
+    da, db = tf.ragged_gemm_backward(a.cuda(), layout(torch, b, how), dc.cuda(), g)
+    for i, n in enumerate(counts):
+        s = slice(offsets[i], offsets[i] + n)
+        A, B, D = a[s].cuda().double(), b[i].cuda().double(), dc[s].cuda().double()
+        close(got[s], A @ B, A.abs() @ B.abs(), K, name)
+        close(da[s], D @ B.t().contiguous(), D.abs() @ B.abs().t().contiguous(), N, name)
+        close(db[i], A.t().contiguous() @ D, A.abs().t().contiguous() @ D.abs(), n, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16"])
+@pytest.mark.parametrize("K,N", [(128, 2600), (127, 2599)])
+def test_ragged_gradient_of_gathered_rows_of_long_groups(tf, torch, name, K, N):
+    # several hundred rows of a group, each read by way of the order, some of which lead nowhere
+    rng = np.random.default_rng(N)
+    tokens, groups = 700, 3
+    ids = choices(rng, tokens, 2, groups)
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    gone = rng.choice(offsets[-1], 20, replace=False)
+    order = np.asarray(order)
+    order[gone[:10]], order[gone[10:]] = -1, 2 * tokens + 5
+    a, dc = tensor(torch, rng, (tokens, K), name), tensor(torch, rng, (2 * tokens, N), name)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    db = torch.empty(groups, K, N, dtype=a.dtype, device="cuda")
+    tf.ragged_gemm_grad_into(a.cuda(), dc.cuda(), tf.RowGroups(i32(offsets), i32(order), fan=2), 1.0, 0.0, db, gather=True)
+    for i in range(groups):
+        p = [p for p in range(offsets[i], offsets[i + 1]) if 0 <= order[p] < 2 * tokens]
+        A, D = a[order[p] // 2].double(), dc[p].double()
+        close(db[i], A.t() @ D, A.abs().t() @ D.abs(), len(p), name)
+
+
 # ------------------------------------------------------------------------------------------------------ joining
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", TYPES)
@@ -469,6 +527,26 @@ def test_an_adapter_that_is_no_number_stays_with_its_rows(tf, torch, name):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("K,N,R", [(72, 6104, 24), (71, 6101, 7), (264, 328, 16)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_adapters_of_many_rows_keep_what_is_no_number(tf, torch, name, K, N, R, how):
+    # tiles of every size; one adapter infinite, one partly no number, rows of none between them: the others' rows are as they
+    # should be, theirs are no numbers
+    rng = np.random.default_rng(N)
+    ids = np.repeat([2, -1, 0, 1, 3, 0], [260, 7, 300, 5, 290, 130])
+    x, w = tensor(torch, rng, (len(ids), K), name), tensor(torch, rng, (K, N), name, K ** -0.5)
+    a, b = tensor(torch, rng, (4, K, R), name, K ** -0.5), tensor(torch, rng, (4, R, N), name)
+    broken_a, broken_b = a.clone(), b.clone()
+    broken_b[1], broken_a[3, K // 2, R - 1] = float("inf"), float("nan")
+    got = tf.adapter_gemm(x.cuda(), layout(torch, w, how), layout(torch, broken_a, how), layout(torch, broken_b, how), made(tf, torch, ids, 4)).cpu()
+    want, size, low = adapter_reference(torch, x, w, a, b, None, ids)
+    kept = torch.from_numpy((ids != 1) & (ids != 3))
+    close(got[kept], want[kept], size[kept], K + R, name, MIDDLE[name] * low[kept])
+    assert not got[~kept].isfinite().any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name,big", [("float16", 3.0e4), ("bfloat16", 1.0e30), ("float32", 1.0e30)])
 def test_an_adapters_middle_may_exceed_the_operands_range(tf, torch, name, big):
     # x a is 64 * big (beyond f16's largest 65504), x a b again in range
@@ -545,6 +623,23 @@ def test_calls_on_another_stream_and_on_tensors(tf, torch):
     assert isinstance(out, tf.Tensor) and out.event is not None
     assert np.array_equal(out.to_numpy(), want.cpu().numpy())
     assert tf.Tensor.from_torch(x.bfloat16()).to_numpy().dtype == np.float32
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(tf, torch):
+    # the same operands on two streams, nothing waited for in between: workspaces of their own
+    x, up, down, ids, gates, dy = layer_inputs(torch, 11, "bfloat16", tokens=2000, fan=2, groups=5, K=136, N=264)
+    low_a, low_b = up[:, :, :8].contiguous(), up[:, :8, :].contiguous()
+    flat = tf.RowGroups.from_ids(ids[:, 0], up.shape[0])
+    want = (expert_layer(tf, x, up, down, ids, gates)[0], tf.adapter_gemm(x, up[0].contiguous(), low_a, low_b, flat))
+    torch.cuda.synchronize()
+    out = []
+    for side in [torch.cuda.Stream() for _ in range(2)] * 3:
+        with torch.cuda.stream(side):
+            out.append((expert_layer(tf, x, up, down, ids, gates)[0], tf.adapter_gemm(x, up[0].contiguous(), low_a, low_b, flat)))
+    torch.cuda.synchronize()
+    for got in out:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.gpu
