@@ -348,13 +348,17 @@ __device__ __forceinline__ void multiply_stage(typename Num<C>::acc4 (&acc)[XT][
 }
 // A whole k loop: load(k0, ra, rb) fetches a stage's chunks, settle(k0, ra, rb) makes them what the tiles take.  Loads two
 // stages ahead are made for those behind the last one too (of anything that is there): were they left out on a condition, the wait
-// for one stage's would have to count on that, and would wait for the next one's as well.
-template <class C, bool AKFAST, bool BKFAST, int XT, int YT, bool ALL, class Load, class Settle>
-__device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], char* lds, int kend, int wm, int wn, int lane, int from, int to, Load load,
-                                       Settle settle) {
+// for one stage's would have to count on that, and would wait for the next one's as well.  With KW teams of four waves, team w takes
+// the stages w, w + KW, ...; all of them go through the loop as often, so that they meet at its barriers.
+template <class C, bool AKFAST, bool BKFAST, int XT, int YT, int KW, bool ALL, class Load, class Settle>
+__device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], char* lds, int k_end, int wm, int wn, int lane, int team, int from, int to,
+                                       Load load_at, Settle settle_at) {
     constexpr int TM = 32 * XT, TN = 32 * YT, BK = 128 / (int)sizeof(C);
+    const int kend = KW == 1 ? k_end : (k_end + KW * BK - 1) / (KW * BK) * BK;   // of the team's own stages, which are next to each other here
+    auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) { load_at(k0 * KW + team * BK, ra, rb); };
+    auto settle = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) { settle_at(k0 * KW + team * BK, ra, rb); };
     constexpr int RA = TM * (int)sizeof(C) / 16, RB = TN * (int)sizeof(C) / 16;   // chunks of a row of k in a row-fast tile
-    const int tid = threadIdx.x, cc = tid & 7, cr = tid >> 3;
+    const int tid = threadIdx.x % GENERAL_THREADS, cc = tid & 7, cr = tid >> 3;
     auto store_stage = [&](char* stage, int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
         settle(k0, ra, rb);
 #pragma unroll
@@ -409,15 +413,18 @@ __device__ __forceinline__ void k_loop(typename Num<C>::acc4 (&acc)[XT][YT], cha
 }
 
 // TA, TB: the operands' types; C: the type multiplied in (theirs, or that of the sums); TO: the result's.  UNIT: both operands
-// contiguous in the direction in which they are read (B along k if BKFAST), of type C, and no shorter than a chunk.
-template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT>
-__global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(const Args a) {
+// contiguous in the direction in which they are read (B along k if BKFAST), of type C, and no shorter than a chunk.  KW: teams of
+// four waves that share out k, for launches of few blocks, whose time is that of one block's loads after each other.
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT, int KW>
+__global__ __launch_bounds__(GENERAL_THREADS * KW, KW == 1 ? 2 : 4) void ragged_general_kernel(const Args a) {
     typedef Num<C> NT;
     typedef typename NT::acc W;
     constexpr int E = NT::E, TM = 32 * XT, TN = 32 * YT, BK = 128 / (int)sizeof(C);
     constexpr bool AKFAST = MODE != OUTER;
-    __shared__ __align__(16) char lds[2 * (TM + TN) * 128];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1, q = lane >> 4, j = lane & 15;
+    __shared__ __align__(16) char all_lds[KW * 2 * (TM + TN) * 128];
+    const int tid = threadIdx.x % GENERAL_THREADS, team = KW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / GENERAL_THREADS);
+    char* const lds = all_lds + team * 2 * (TM + TN) * 128;
+    const int lane = tid & 63, wave = tid >> 6, wm = wave & 1, wn = wave >> 1, q = lane >> 4, j = lane & 15;
     const int tiles_n = (a.N + TN - 1) / TN;
     Tile t;
     if constexpr (MODE == ROWS) {
@@ -464,7 +471,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                     }
                 }
             };
-            k_loop<W, true, BKFAST, XT, YT, false>(acc, lds, a.r, wm, wn, lane, from - t.first, to - t.first, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
+            k_loop<W, true, BKFAST, XT, YT, KW, false>(acc, lds, a.r, wm, wn, lane, team, from - t.first, to - t.first, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
         });
     }
 
@@ -489,20 +496,20 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
     if constexpr (UNIT) {
         // Where this thread's chunks of a stage start, moved back to the row's last E elements where that ends inside one; rows and
         // columns beyond the tile's read the first ones.
-        const int64_t step_b = BKFAST ? BK : BK * a.b_k;
+        const int64_t step_b = KW * (BKFAST ? BK : BK * a.b_k);
         const TA* pa[XT];
         const TB* pb[YT];
 #pragma unroll
         for (int i = 0; i < XT; ++i) {
             const int id = tid + GENERAL_THREADS * i, m = m0 + (id % RA) * E;
-            if constexpr (AKFAST) pa[i] = A + (arow[i] > 0 ? arow[i] * a.a_row : 0) + cc * E;
+            if constexpr (AKFAST) pa[i] = A + (arow[i] > 0 ? arow[i] * a.a_row : 0) + team * BK + cc * E;
             else pa[i] = A + (m + E <= a.M ? m : a.M - E);
         }
 #pragma unroll
         for (int i = 0; i < YT; ++i) {
             const int id = tid + GENERAL_THREADS * i, n = n0 + (id % RB) * E;
-            if constexpr (BKFAST) pb[i] = B + (n0 + cr + 32 * i < a.N ? (n0 + cr + 32 * i) * a.b_n : 0) + cc * E;
-            else pb[i] = B + ((MODE == OUTER ? t.first : 0) + id / RB) * a.b_k + (n + E <= a.N ? n : a.N - E);
+            if constexpr (BKFAST) pb[i] = B + (n0 + cr + 32 * i < a.N ? (n0 + cr + 32 * i) * a.b_n : 0) + team * BK + cc * E;
+            else pb[i] = B + ((MODE == OUTER ? t.first : 0) + team * BK + id / RB) * a.b_k + (n + E <= a.N ? n : a.N - E);
         }
         const bool edge_b = !BKFAST && n0 + TN > a.N;   // both the same for all of a wave
         bool edge;
@@ -515,7 +522,8 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
             edge = m0 + TM > a.M || (a.gather && a.order) || t.first + kend > a.a_rows;
         }
         uint32_t none = 0;   // outer: chunks of a stage on their way whose row of A is none, the stages' bits apart
-        const int kwhole = kend / BK * BK;   // whole stages move the pointers on, those behind them leave them there
+        // whole stages move the pointers on, those behind them leave them there, at k = k_at
+        const int kwhole = kend / BK * BK, k_at = KW == 1 ? kwhole : team * BK + (kwhole > team * BK ? (kwhole - team * BK + KW * BK - 1) / (KW * BK) * (KW * BK) : 0);
         auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
             if constexpr (!AKFAST) {
                 const bool found = !(a.gather && a.order) && t.first + kend <= a.a_rows;
@@ -523,7 +531,7 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                 for (int i = 0; i < XT; ++i) {
                     const int id = tid + GENERAL_THREADS * i, k = k0 + id / RA;
                     const int64_t s = k >= kend ? -1 : found ? t.first + k : source_row(a, t.first + k);
-                    const uint32_t bit = 1u << (((k0 / BK) & 3) * 8 + i);
+                    const uint32_t bit = 1u << (((k0 / (KW * BK)) & 3) * 8 + i);
                     none = s < 0 ? none | bit : none & ~bit;
                     ra[i] = load_unit<TA>(pa[i] + (s < 0 ? 0 : s) * a.a_row);
                 }
@@ -531,19 +539,19 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
             if (k0 < kwhole) {
                 if constexpr (AKFAST)
 #pragma unroll
-                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i]), pa[i] += BK;
+                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i]), pa[i] += KW * BK;
 #pragma unroll
                 for (int i = 0; i < YT; ++i) rb[i] = load_unit<TB>(pb[i]), pb[i] += step_b;
             } else {
                 const int count = kend - k0 - cc * E;
                 if constexpr (AKFAST)
 #pragma unroll
-                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i] - (count >= E ? 0 : count > 0 ? E - count : kwhole + cc * E));
+                    for (int i = 0; i < XT; ++i) ra[i] = load_unit<TA>(pa[i] - (count >= E ? 0 : count > 0 ? E - count : k_at + cc * E));
 #pragma unroll
                 for (int i = 0; i < YT; ++i) {
                     const int id = tid + GENERAL_THREADS * i;
-                    if constexpr (BKFAST) rb[i] = load_unit<TB>(pb[i] - (count >= E ? 0 : count > 0 ? E - count : kwhole + cc * E));
-                    else rb[i] = load_unit<TB>(pb[i] - (k0 + id / RB < kend ? 0 : (kwhole + id / RB) * a.b_k));
+                    if constexpr (BKFAST) rb[i] = load_unit<TB>(pb[i] - (count >= E ? 0 : count > 0 ? E - count : k_at + cc * E));
+                    else rb[i] = load_unit<TB>(pb[i] - (k0 + id / RB < kend ? 0 : (k_at + id / RB) * a.b_k));
                 }
             }
         };
@@ -554,14 +562,14 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                 for (int i = 0; i < XT; ++i) {
                     int count = count_a(i, k0);
                     if constexpr (!AKFAST)
-                        if (none >> (((k0 / BK) & 3) * 8 + i) & 1) count = 0;
+                        if (none >> (((k0 / (KW * BK)) & 3) * 8 + i) & 1) count = 0;
                     settle_unit<C>(ra[i], count);
                 }
             if (!whole || edge_b)
 #pragma unroll
                 for (int i = 0; i < YT; ++i) settle_unit<C>(rb[i], count_b(i, k0));
         };
-        k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load, settle);
+        k_loop<C, AKFAST, BKFAST, XT, YT, KW, true>(acc, lds, kend, wm, wn, lane, team, 0, 0, load, settle);
     } else {
         auto load = [&](int k0, u32x4 (&ra)[XT], u32x4 (&rb)[YT]) {
 #pragma unroll
@@ -591,7 +599,23 @@ __global__ __launch_bounds__(GENERAL_THREADS, 2) void ragged_general_kernel(cons
                 rb[i] = load_chunk<TB, C>(p, BKFAST ? a.b_k : a.b_n, count_b(i, k0));
             }
         };
-        k_loop<C, AKFAST, BKFAST, XT, YT, true>(acc, lds, kend, wm, wn, lane, 0, 0, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
+        k_loop<C, AKFAST, BKFAST, XT, YT, KW, true>(acc, lds, kend, wm, wn, lane, team, 0, 0, load, [](int, u32x4 (&)[XT], u32x4 (&)[YT]) {});
+    }
+
+    if constexpr (KW > 1) {   // the teams' sums, added in their order
+        static_assert(sizeof(acc) * GENERAL_THREADS <= 2 * (TM + TN) * 128, "a team's sums fit its tiles");
+        __syncthreads();
+        if (team > 0) __builtin_memcpy(lds + tid * sizeof(acc), acc, sizeof(acc));
+        __syncthreads();
+        if (team > 0) return;
+        for (int w = 1; w < KW; ++w) {
+            typename NT::acc4 more[XT][YT];
+            __builtin_memcpy(more, all_lds + w * 2 * (TM + TN) * 128 + tid * sizeof(acc), sizeof(acc));
+#pragma unroll
+            for (int x = 0; x < XT; ++x)
+#pragma unroll
+                for (int y = 0; y < YT; ++y) acc[x][y] += more[x][y];
+        }
     }
 
     W alpha = (W)a.alpha;

@@ -28,7 +28,7 @@ template <class T> constexpr const char* type_name() {
 }
 constexpr const char* mode_name(int mode) { return mode == ROWS ? "rows" : mode == OUTER ? "outer" : mode == SHARED ? "shared" : "pair"; }
 
-template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT>
+template <class TA, class TB, class C, class TO, int MODE, bool BKFAST, bool UNIT, int XT, int YT, int KW = 1>
 int32_t launch_general_tiles(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, 32 * YT);
     const int64_t blocks = MODE == ROWS ? row_tiles(a, 32 * XT) * tn
@@ -37,8 +37,8 @@ int32_t launch_general_tiles(const Args& a, void* stream) {
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
     static const std::string label = std::string("(ragged_general_kernel<") + type_name<TA>() + ", " + type_name<TB>() + ", " + type_name<C>() + ", " +
                                      type_name<TO>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") + (UNIT ? "unit, " : "any, ") +
-                                     std::to_string(32 * XT) + "x" + std::to_string(32 * YT) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, UNIT, XT, YT>), dim3((unsigned)blocks), dim3(GENERAL_THREADS), 0, (hipStream_t)stream, a);
+                                     std::to_string(32 * XT) + "x" + std::to_string(32 * YT) + (KW > 1 ? ", " + std::to_string(KW) : std::string()) + ">)";
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, UNIT, XT, YT, KW>), dim3((unsigned)blocks), dim3(GENERAL_THREADS * KW), 0, (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 // Whether both operands are contiguous in the direction in which the kernel reads them, and long enough for a chunk.
@@ -61,6 +61,13 @@ int32_t launch_general(const Args& a, void* stream) {
                 const int64_t blocks = (MODE == OUTER ? a.n_groups * tiles(a.M, 128) : MODE == ROWS ? a.n_rows / 128 + a.n_groups / 2 : tiles(a.n_rows, 128)) * tiles(a.N, 128);
                 if (rows > 96 && a.N > 96 && blocks >= (sizeof(C) == 4 ? 2048 : 256)) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 4, 4>(a, stream);
             }
+            // Fewer than two blocks a compute unit wait for their loads, stage after stage: tiles of 32 x 32 then, four times the
+            // blocks, and four teams to share out k, from eight stages on (f64, 236 rows, 1472 x 38: 65 us against 24; 200 bf16 rows of
+            // four groups, 4001 x 1001: 63 and 29; f64, 1600 rows of eight, 256 x 640: 27 and 29; 1024 x 640: 81 and 67.  702 blocks,
+            // f32, 3000 rows, 1000 x 800: 79 and 87)
+            const int64_t few = MODE == OUTER ? Patches(a, 64, 64).blocks(a.n_groups) : (MODE == ROWS ? row_tiles(a, 64) : tiles(a.n_rows, 64)) * tiles(a.N, 64);
+            const int64_t k = MODE == OUTER ? a.n_rows / a.n_groups : a.K;
+            if (few < 512 && k * (int)sizeof(C) >= 1024) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 1, 1, 4>(a, stream);
             return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 2, 2>(a, stream);
         }
     return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, false, 2, 2>(a, stream);
