@@ -25,13 +25,14 @@ class tfh_row_groups(C.Structure):
                 ("n_groups", C.c_int32), ("fan", C.c_int32)]
 
 
-_CODES = {}
+_CODES, _TYPES = {}, {}
 
 
 def _codes():
     if not _CODES:
         import torch
         _CODES.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.float64: F64})
+        _TYPES.update({c: t for t, c in _CODES.items()})
     return _CODES
 
 
@@ -63,7 +64,7 @@ def _device(t):
         return t.logical_memory_space_.space_id
     if not t.is_cuda:
         raise NoCompatibleComputeDevice("no compatible compute device for this operation on MainMemory")
-    return t.device.index
+    return t.get_device()
 
 
 def _code(t):
@@ -84,20 +85,22 @@ class _Call:
     def __init__(self, like, operands, groups, stream, sums=()):
         import torch
         self.torch, self.like = torch, like
+        _CODES or _codes()
         self.device = _device(like)
         self.dtype = _code(like)
         wide = F64 if self.dtype == F64 else F32
-        self.used = [t for t in operands if t is not None] + [t for t in sums if t is not None]
-        for t in self.used:
-            if _device(t) != self.device:
-                raise CrossMemorySpaceOperation(f"cross-memory-space operation between {GpuMemory(self.device)!r} and {GpuMemory(_device(t))!r}",
-                                                GpuMemory(self.device), GpuMemory(_device(t)))
-        for t in operands:
-            if t is not None and _code(t) != self.dtype:
-                raise InvalidArgument("invalid argument: operands of different element types")
-        for t in sums:
-            if t is not None and _code(t) != wide:
-                raise InvalidArgument("invalid argument: weights and scales are f32 (f64 beside f64 operands)")
+        self.used = [like]
+        for sort, wanted, why in ((operands, self.dtype, "operands of different element types"),
+                                  (sums, wide, "weights and scales are f32 (f64 beside f64 operands)")):
+            for t in sort:
+                if t is None:
+                    continue
+                if _device(t) != self.device:
+                    raise CrossMemorySpaceOperation(f"cross-memory-space operation between {GpuMemory(self.device)!r} and {GpuMemory(_device(t))!r}",
+                                                    GpuMemory(self.device), GpuMemory(_device(t)))
+                if _code(t) != wanted:
+                    raise InvalidArgument("invalid argument: " + why)
+                self.used.append(t)
         if groups is not None:
             if groups.device != self.device:
                 raise CrossMemorySpaceOperation(f"cross-memory-space operation between {GpuMemory(self.device)!r} and {GpuMemory(groups.device)!r}",
@@ -109,6 +112,7 @@ class _Call:
         if torch.cuda.current_device() != self.device:
             self.guard = torch.cuda.device(self.device)
         self.ordered = False
+        self.place = None
 
     def __enter__(self):
         if self.guard is not None:
@@ -130,11 +134,12 @@ class _Call:
             _check(lib().tfh_stream_wait_event(self.stream, CompletionEvent(self.current)._h))
             self.ordered = True
         dtype = self.dtype if dtype is None else dtype
-        tdt = dtype if isinstance(dtype, torch.dtype) else {c: t for t, c in _codes().items()}[dtype]
         if like is not None and not isinstance(like, Tensor):
             t = torch.empty_like(like)
         else:
-            t = torch.empty(dims, dtype=tdt, device=self.torch.device("cuda", self.device))
+            if self.place is None:
+                self.place = torch.device("cuda", self.device) if isinstance(self.like, Tensor) else self.like.device
+            t = torch.empty(dims, dtype=dtype if isinstance(dtype, torch.dtype) else _TYPES[dtype], device=self.place)
         self.used.append(t)
         return t
 
