@@ -20,7 +20,7 @@ namespace ragged {
 // A scalar operand of the loads below.  A vector instruction's write of a scalar register (readfirstlane is one) must lie
 // five wait states before a load that reads it; the compiler sees to that for its own loads, not for those in asm.  Moved
 // here by the scalar unit, which waits for it, the value is one that a load may read at once.  (A spilled scalar register
-// would come back through a vector instruction: the kernels that use these loads have to be built without scalar spills.)
+// comes back through a vector instruction, wherever the compiler puts it: the loads' own s_nop 4 makes up for that one.)
 __device__ __forceinline__ uint32_t scalar_of(uint32_t v) {
     uint32_t s;
     asm("s_mov_b32 %0, %1" : "=s"(s) : "s"(__builtin_amdgcn_readfirstlane(v)));
@@ -93,12 +93,11 @@ template <int WM_, int WN_, int XT_, int YT_, int KB_ = 128, int SA_ = 2, int SB
     static_assert(SB_ >= 2 && (SA_ == SB_ || SA_ == SB_ + 1), "the waits below count on it");
     static constexpr int WM = WM_, WN = WN_, XT = XT_, YT = YT_, TM = 32 * WM * XT, TN = 32 * WN * YT, KB = KB_, SA = SA_, SB = SB_;
     static constexpr int TILE_A = TM * KB, TILE_B = TN * KB, LDS = SA * TILE_A + SB * TILE_B;
-    static constexpr bool BY_GROUP = TM > 128;
     static constexpr int BLOCKS = XT * YT > 8 ? 1 : 2;   // of a CU: registers and LDS leave room for so many
 };
 
-// One tile: its k loop and its results.  BY_GROUP: its rows are of one group (of none: t.group == a.n_groups).
-template <class T, int MODE, bool BKFAST, class S, bool BY_GROUP>
+// One tile: its k loop and its results.  Its rows are of one group (of none: t.group == a.n_groups), but in shared mode of any.
+template <class T, int MODE, bool BKFAST, class S>
 __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* lds) {
     static_assert(sizeof(T) == 2, "16-bit operands");
     constexpr int XT = S::XT, YT = S::YT, TM = S::TM, TN = S::TN, KB = S::KB, BK = KB / 2, SA = S::SA, SB = S::SB;
@@ -171,11 +170,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
             vb[i] = n < a.N ? (uint32_t)(k * a.b_k * 2) + n * 2 : NOWHERE;
         }
     }
-    // Large shared tiles: the low-rank part is the first stages of the loop, V[p, :] as A's and E[g] as B's.
-    constexpr bool EXT = MODE == SHARED && BY_GROUP;
-    int ext = 0;
-    if constexpr (EXT) ext = t.group < a.n_groups ? 2 * a.pad / BK : 0;
-    const int main_stages = (kend + BK - 1) / BK, stages = ext + main_stages;
+    const int stages = (kend + BK - 1) / BK;
 
     // What the loads of a stage are: buffers, the chunks' offsets in them, and scalar offsets that go on from stage to stage.
     // Offsets change at the ends of the parts only, by a branch that is seldom taken, and the loop's loads take them as they are.
@@ -185,15 +180,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     } now;
     auto stage_a = [&](int s) {   // s one more than before
         now.oa += step_a;
-        if constexpr (EXT) {
-            if (s < ext) {   // the halves of the pair, one after the other
-                now.A = buffer_of((const char*)a.V + (int64_t)t.first * a.v_row * 2, (uint32_t)((t.rows - 1) * a.v_row * 2 + 2 * a.pad * 2));
-                now.oa = 0;
-#pragma unroll
-                for (int i = 0; i < CA; ++i) now.va[i] = cr + RPI * i < t.rows ? (uint32_t)((cr + RPI * i) * a.v_row * 2) + (s * BK + kc) * 2 : NOWHERE;
-            }
-        }
-        if (s == ext) {
+        if (s == 0) {
             now.A = A, now.oa = 0;
 #pragma unroll
             for (int i = 0; i < CA; ++i) now.va[i] = va[i];
@@ -223,44 +210,31 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         }
         if (s >= stages - 1) {
             const bool gone = s >= stages;   // behind the last stage: nothing; in it: nothing beyond the last k
-            const int k0 = (s - ext) * BK;
+            const int k0 = s * BK;
             if (gone) now.oa = 0;
 #pragma unroll
             for (int i = 0; i < CA; ++i) {
                 const int k = k0 + (AKFAST ? kc : (tid + 256 * i) / RA);
-                now.va[i] = gone || (main_stages > 0 && k >= kend) ? NOWHERE : now.va[i];
+                now.va[i] = gone || k >= kend ? NOWHERE : now.va[i];
             }
         }
         now.oa = scalar_of(now.oa);
     };
     auto stage_b = [&](int s) {
         now.ob += step_b;
-        if constexpr (EXT) {
-            if (s < ext) {   // ranks beyond r read as zeros on both sides
-                const int k0 = s * BK;
-                now.B = buffer_of((const char*)a.E + t.group * a.e_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.e_n * 2 + a.r * 2 : (a.r - 1) * a.e_k * 2 + a.N * 2));
-                now.ob = 0;
-#pragma unroll
-                for (int i = 0; i < CB; ++i) {
-                    const int id = tid + 256 * i, kk = BKFAST ? kc : id / RB, k = k0 + kk, rank = k >= a.pad ? k - a.pad : k;
-                    const int n = BKFAST ? n0 + cr + RPI * i : n0 + ((id % RB) ^ (rowfast_swizzle<T>(kk) & (RB - 1))) * 8;
-                    now.vb[i] = n < a.N && rank < a.r ? (uint32_t)(n * a.e_n * 2) + (uint32_t)(rank * a.e_k * 2) : NOWHERE;
-                }
-            }
-        }
-        if (s == ext) {
+        if (s == 0) {
             now.B = B, now.ob = 0;
 #pragma unroll
             for (int i = 0; i < CB; ++i) now.vb[i] = vb[i];
         }
         if (s >= stages - 1) {
             const bool gone = s >= stages;
-            const int k0 = (s - ext) * BK;
+            const int k0 = s * BK;
             if (gone) now.ob = 0;
 #pragma unroll
             for (int i = 0; i < CB; ++i) {
                 const int k = k0 + (BKFAST ? kc : (tid + 256 * i) / RB);
-                now.vb[i] = gone || (main_stages > 0 && k >= kend) ? NOWHERE : now.vb[i];
+                now.vb[i] = gone || k >= kend ? NOWHERE : now.vb[i];
             }
         }
         now.ob = scalar_of(now.ob);
@@ -271,7 +245,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         else fb[set][i] = fragment32<T, TN, BKFAST, KB>(lds + slot_b, (wn * YT + i) * 32, h, lane);
     };
     constexpr int FRAGS = XT + YT, CHUNKS = CA + CB;
-    if constexpr (MODE == SHARED && !BY_GROUP) {
+    if constexpr (MODE == SHARED) {
         // V . E[g] for the groups that the tile's rows belong to, before the accumulators hold anything else: in f16 a row's
         // V is scaled by a power of two, which is undone here.  The pair's halves are 2 pad k's against E twice.  Rows of
         // another group keep what they have -- selected, not multiplied by zero, which infinite factors would survive.
@@ -522,15 +496,12 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
 
 template <class T, int MODE, bool BKFAST, class S>
 __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args a) {
-    // shared mode: large tiles belong to one group each (the host sets zero_rest: the rows of no group are one more), small
-    // ones span as many as their rows are of, so that few rows of many groups do not read W once for each
-    constexpr bool BY_GROUP = MODE == ROWS || (MODE == SHARED && S::BY_GROUP);
     constexpr int TM = S::TM, TN = S::TN;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     char* const lds = (char*)smem_raw;
     const int tiles_n = (a.N + TN - 1) / TN;
     Tile t;
-    if constexpr (BY_GROUP) {
+    if constexpr (MODE == ROWS) {
         if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
         if constexpr (TM == 256) {
             // a group's last tile is seldom full: half or a quarter of the rows in half or 0.4 of the time
@@ -538,11 +509,11 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
             typedef Shape<2, 2, 2, S::YT, S::KB, S::SA, S::SB> Half;
             static_assert(Quarter::TN == TN && Half::TN == TN && Half::LDS <= S::LDS, "the same columns");
             if (t.rows <= 64) {
-                fast_tile<T, MODE, BKFAST, Quarter, true>(a, t, lds);
+                fast_tile<T, MODE, BKFAST, Quarter>(a, t, lds);
                 return;
             }
             if (t.rows <= 128) {
-                fast_tile<T, MODE, BKFAST, Half, true>(a, t, lds);
+                fast_tile<T, MODE, BKFAST, Half>(a, t, lds);
                 return;
             }
         }
@@ -555,7 +526,7 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
         t.first = t.tile_m * TM;
         t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
     }
-    fast_tile<T, MODE, BKFAST, S, BY_GROUP>(a, t, lds);
+    fast_tile<T, MODE, BKFAST, S>(a, t, lds);
 }
 
 // Whether the kernel can take a call: rows that start 16-byte aligned and end with a chunk, spans that 32 bits address.

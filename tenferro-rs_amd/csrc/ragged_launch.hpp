@@ -75,7 +75,7 @@ int32_t launch_general(const Args& a, void* stream) {
 template <class T, int MODE, bool BKFAST, class S>
 int32_t launch_fast(const Args& a, void* stream) {
     const int64_t tn = tiles(a.N, S::TN);
-    const int64_t blocks = MODE == ROWS || (MODE == SHARED && S::BY_GROUP) ? row_tiles(a, S::TM) * tn
+    const int64_t blocks = MODE == ROWS ? row_tiles(a, S::TM) * tn
                            : MODE == OUTER || MODE == PAIR ? Patches(a, S::TM, S::TN).blocks(a.n_groups) : tiles(a.n_rows, S::TM) * tn;
     if (blocks <= 0) return TFH_OK;
     if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
@@ -96,15 +96,16 @@ typedef Shape<2, 2, 1, 2, 128, 3, 3> Slim;   // 64 x 128
 typedef Shape<1, 4, 1, 1> Small;    // 32 x 128
 // Whether tiles of 256 x 256, one to a compute unit, come in rounds of the machine's 256 units that are full enough.  If not,
 // tiles of half the columns, two to a unit: those take a tenth longer for the same work where k is 2048, a fifth from 4096 on and
-// hardly any where it is short, since one works while the other starts or ends, and leave less of the machine idle.  (bf16, uneven
-// groups, large and tall tiles: 65 536 rows of 64, 2048 x 2048, nine rounds: 582 and 633 us; 32 768 of 32, 1024 x 2048, four and a
-// half: 187 and 168; 8192 of 16, 2048 x 2048, one and a quarter: 104 and 91; 4096 of 8, 0.6: 54 and 56.)  Of the groups' last
-// tiles one half is full on average.
+// hardly any where it is short, since one works while the other starts or ends, and leave less of the machine idle.  How full the
+// last round is follows from the sizes for one group only; of several, it is half on average, and so are the groups' last tiles.
+// (bf16, uneven groups, large and tall tiles: 65 536 rows of 64, 2048 x 2048, nine rounds: 595 and 640 us; 32 768 of 32,
+// 1024 x 2048, four and a half: 187 and 168; 49 152 of 48, 1024 x 2048, seven: 265 and 253; 8192 of 16, 2048 x 2048, one and a
+// quarter: 104 and 91; 4096 of 8, 0.6: 54 and 56.)
 inline bool fills_rounds(const Args& a) {
-    const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
-    const int64_t tn = tiles(a.N, 256), t = groups > 1 ? (a.n_rows * 2 / 256 + groups) * tn / 2 : tiles(a.n_rows, 256) * tn;
+    const int64_t tn = tiles(a.N, 256), t = a.n_groups > 1 ? (a.n_rows * 2 / 256 + a.n_groups) * tn / 2 : tiles(a.n_rows, 256) * tn;
     const int64_t k = a.K < 4096 ? a.K : 4096;
-    return t < 256 ? t > 128 : tiles(t, 256) * 256 * 20480 <= t * (20480 + k);
+    if (t < 256) return t > 128;
+    return (a.n_groups > 1 ? 2 * t + 256 : tiles(t, 256) * 512) * 20480 <= 2 * t * (20480 + k);
 }
 template <class T, int MODE, bool BKFAST>
 int32_t launch_shape(const Args& a, void* stream) {
@@ -112,18 +113,6 @@ int32_t launch_shape(const Args& a, void* stream) {
     if (rows > 192) return MODE == OUTER || !fills_rounds(a) ? launch_fast<T, MODE, BKFAST, Tall>(a, stream) : launch_fast<T, MODE, BKFAST, Large>(a, stream);
     if (rows > 48) return launch_fast<T, MODE, BKFAST, Middle>(a, stream);
     return launch_fast<T, MODE, BKFAST, Small>(a, stream);
-}
-template <class T, bool BKFAST>
-int32_t launch_shared(const Args& a, void* stream) {
-    // Tiles by group read W once for each group's rows; worth it where those fill most of a tile.  (f16 scales its rows'
-    // low-rank part back before the rest is added, which the large tile's one loop has no place for.)
-    if constexpr (__is_same(T, __bf16))
-        if (a.n_rows / (a.n_groups + 1) > 192) {
-            Args g = a;
-            g.zero_rest = 1;
-            return fills_rounds(g) ? launch_fast<T, SHARED, BKFAST, Large>(g, stream) : launch_fast<T, SHARED, BKFAST, Tall>(g, stream);
-        }
-    return launch_fast<T, SHARED, BKFAST, Middle>(a, stream);
 }
 template <class T, int MODE, int TR>
 int32_t launch_few(const Args& a, void* stream) {
@@ -173,7 +162,9 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         // blocks leave the machine idle; 1024 blocks take as long as those tiles do with 128.
         if (kind == PRODUCT_SHARED && a.pad > 0 && !columns && few_takes<SHARED>(a) && tiles(a.n_rows, 64) * tiles(a.N, 16) <= 1024)
             return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream) : launch_few<T, SHARED, 4>(a, stream);
-        if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_shared<T, false>(a, stream) : launch_shared<T, true>(a, stream);
+        // Tiles of 128 x 128 that span the groups: larger ones of one group each leave more of the rows' tiles half empty (8192 rows
+        // of 16 groups, 4096 x 4096: 285 us against 345; 16 384 of 8: 530 and 580; 4096 of 8, 2048 x 4096: 92 and 112).
+        if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_fast<T, SHARED, false, Middle>(a, stream) : launch_fast<T, SHARED, true, Middle>(a, stream);
         // (eight groups of 4096 rows, 4096 and 2048 x 64: 26 us in tiles of 64 rows, three stages on their way, 34 in those of 128)
         if (kind == PRODUCT_OUTER_V && a.pad > 0)
             return a.n_groups * tiles(a.M, 128) < 512 ? launch_fast<T, PAIR, false, Slim>(a, stream) : launch_fast<T, PAIR, false, Middle>(a, stream);
