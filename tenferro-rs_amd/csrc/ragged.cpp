@@ -265,7 +265,11 @@ Args shared_args(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int6
 // Whether the two are done by the kernels that keep the middle as a pair.
 bool by_pair(int32_t dtype, const Args& middle, const Args& shared) {
     if (dtype != TFH_BF16 && dtype != TFH_F16) return false;
-    return thin_takes(middle, !(middle.b_n == 1 && middle.b_k != 1)) && fast_takes<SHARED>(shared, !(shared.b_n == 1 && shared.b_k != 1));
+    // W's columns contiguous and so few tiles that k has to be shared out, which the kernel for sums does (200 rows, 4096 x 1024, rank
+    // 16: 44 us with the pair's tiles, 16 with that; 400 rows, 512 x 512: 14 and 9; 256 tiles of 64 x 64, 1024 x 1024: 29 and 37)
+    const bool columns = shared.b_n == 1 && shared.b_k != 1;
+    if (columns && shared.K >= 512 && ((shared.n_rows + 63) / 64) * (int64_t)((shared.N + 63) / 64) <= 128) return false;
+    return thin_takes(middle, !(middle.b_n == 1 && middle.b_k != 1)) && fast_takes<SHARED>(shared, !columns);
 }
 // Y = X . W + scales (X . F[g]) . E[g]; `v`: scratch, left as a pair or as sums (`*pair`).
 int32_t both(const Adapter& d, const tfh_view& x, int64_t K, int64_t N, int64_t w_k, int64_t w_n, const tfh_view& f, int f_k, int f_r, const tfh_view& e,

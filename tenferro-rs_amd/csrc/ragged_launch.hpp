@@ -48,6 +48,17 @@ template <class C, int MODE, bool BKFAST> bool unit_strides(const Args& a) {
     if (MODE == OUTER) return a.a_col == 1 && a.M >= E && a.b_n == 1 && a.N >= E;
     return a.a_col == 1 && a.K >= E && (BKFAST ? a.b_k == 1 : a.b_n == 1 && a.N >= E);
 }
+// Fewer than two blocks a compute unit wait for their loads, stage after stage: tiles of 32 x 32 then, four times the blocks of
+// 64 x 64, and four teams to share out k, from eight stages on (f64, 236 rows, 1472 x 38: 65 us against 24; 200 bf16 rows of four
+// groups, 4001 x 1001: 63 and 29; f64, 1600 rows of eight, 256 x 640: 27 and 29; 1024 x 640: 81 and 67.  702 blocks, f32, 3000
+// rows, 1000 x 800: 79 and 87).  `bytes`: of an operand's element.  Aligned 16-bit operands as well, and gradients from more than
+// 512 rows of a group on (200 rows of two groups, 4096 x 512: 38 us against 13; gradients of 8192 of four, 256 x 256: 38 and 11;
+// 16 384 of eight, 512 x 256: 39 and 30; of 32 groups, 128 x 128, 512 rows each: 11 and 13).
+template <int MODE> bool starved(const Args& a, int bytes) {
+    const int64_t blocks = MODE == OUTER ? Patches(a, 64, 64).blocks(a.n_groups) : (MODE == ROWS ? row_tiles(a, 64) : tiles(a.n_rows, 64)) * tiles(a.N, 64);
+    const int64_t k = MODE == OUTER ? a.n_rows / a.n_groups : a.K;
+    return blocks < 512 && k * bytes >= 1024 + (MODE == OUTER ? bytes : 0);
+}
 template <class TA, class TB, class C, class TO, int MODE, bool BKFAST>
 int32_t launch_general(const Args& a, void* stream) {
     if constexpr (__is_same(TA, C) && __is_same(TB, C))
@@ -61,13 +72,7 @@ int32_t launch_general(const Args& a, void* stream) {
                 const int64_t blocks = (MODE == OUTER ? a.n_groups * tiles(a.M, 128) : MODE == ROWS ? a.n_rows / 128 + a.n_groups / 2 : tiles(a.n_rows, 128)) * tiles(a.N, 128);
                 if (rows > 96 && a.N > 96 && blocks >= (sizeof(C) == 4 ? 2048 : 256)) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 4, 4>(a, stream);
             }
-            // Fewer than two blocks a compute unit wait for their loads, stage after stage: tiles of 32 x 32 then, four times the
-            // blocks, and four teams to share out k, from eight stages on (f64, 236 rows, 1472 x 38: 65 us against 24; 200 bf16 rows of
-            // four groups, 4001 x 1001: 63 and 29; f64, 1600 rows of eight, 256 x 640: 27 and 29; 1024 x 640: 81 and 67.  702 blocks,
-            // f32, 3000 rows, 1000 x 800: 79 and 87)
-            const int64_t few = MODE == OUTER ? Patches(a, 64, 64).blocks(a.n_groups) : (MODE == ROWS ? row_tiles(a, 64) : tiles(a.n_rows, 64)) * tiles(a.N, 64);
-            const int64_t k = MODE == OUTER ? a.n_rows / a.n_groups : a.K;
-            if (few < 512 && k * (int)sizeof(C) >= 1024) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 1, 1, 4>(a, stream);
+            if (starved<MODE>(a, sizeof(C))) return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 1, 1, 4>(a, stream);
             return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, true, 2, 2>(a, stream);
         }
     return launch_general_tiles<TA, TB, C, TO, MODE, BKFAST, false, 2, 2>(a, stream);
@@ -155,9 +160,9 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
             if (each <= 32 && (a.n_rows / 32 + used) * t16 <= 1024) return launch_few<T, ROWS, 2>(a, stream);
             if (each <= 64 && (a.n_rows / 64 + used) * t16 <= 1024) return launch_few<T, ROWS, 4>(a, stream);
         }
-        if (kind == PRODUCT_ROWS && fast_takes<ROWS>(a, !columns))
+        if (kind == PRODUCT_ROWS && !starved<ROWS>(a, 2) && fast_takes<ROWS>(a, !columns))
             return columns ? launch_shape<T, ROWS, false>(a, stream) : launch_shape<T, ROWS, true>(a, stream);
-        if (kind == PRODUCT_OUTER && fast_takes<OUTER>(a, false)) return launch_shape<T, OUTER, false>(a, stream);
+        if (kind == PRODUCT_OUTER && !starved<OUTER>(a, 2) && fast_takes<OUTER>(a, false)) return launch_shape<T, OUTER, false>(a, stream);
         // Few rows: sixteen columns a block.  64 rows by 4096 columns and k's take 16 us so and 86 with 128 x 128 tiles, whose 32
         // blocks leave the machine idle; 1024 blocks take as long as those tiles do with 128.
         if (kind == PRODUCT_SHARED && a.pad > 0 && !columns && few_takes<SHARED>(a) && tiles(a.n_rows, 64) * tiles(a.N, 16) <= 1024)
