@@ -8,7 +8,8 @@
 // launch of one block; beyond that two (counts per block and group; the placing, each block of which adds up what the blocks
 // before it have), or, where that would be many counts to read for every block, three (their prefix along the blocks between).
 // What bounds it: the small form is latency (a load, two passes over LDS counters, a store); the large one the
-// launches, each of which moves a few megabytes.
+// launches, each of which moves a few megabytes (1 048 576 indices of 64 bits in 256 groups: 20 us, of which counting 4.7, prefixes
+// 4.7 and placing 11, 0.84 TB/s together; 33.5 million in 64 groups: 370 us, 2.2 TB/s; 256 rows in 128 groups: 3.5 us).
 #include <hip/hip_runtime.h>
 
 #include "launch.hpp"
@@ -20,10 +21,13 @@ namespace {
 
 constexpr int WAVES = 16, THREADS = WAVES * 64;
 constexpr int ROUNDS = 8;                              // 64 rows each, a wave's share of a block
-constexpr int FEW_ROUNDS = 4;                          // the same where a block's counters are few (FEW_BINS): twice the blocks
+constexpr int FEW_ROUNDS = 4;                          // the same where a block's counters are few (FEW_BINS): twice the blocks (1 M rows
+                                                       // of 256 groups: 21 us; with four times the blocks 24)
 constexpr int FEW_BINS = 320;
 constexpr int SMALL_ROWS = WAVES * 64 * ROUNDS;        // 8192
-constexpr int64_t JOINED_COUNTS = 1 << 14;             // counts that every placing block reads by itself
+// Counts that every placing block reads by itself: 64 blocks of 129 take 16 us so in all and 19 with the prefixes' launch, 256
+// blocks of 257 take 40 and 21.
+constexpr int64_t JOINED_COUNTS = 1 << 14;
 constexpr int rounds_for(int64_t bins) { return bins <= FEW_BINS ? FEW_ROUNDS : ROUNDS; }
 
 __device__ __forceinline__ int key_of(const GroupArgs& a, int i) {

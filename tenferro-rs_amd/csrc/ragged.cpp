@@ -11,7 +11,7 @@ namespace tfh {
 namespace ragged {
 namespace {
 
-constexpr int64_t MOST = 0x7fffffff;
+constexpr int64_t MOST = 0x7ff00000;   // rows, extents: 32-bit indices may run past one by the largest step of a loop
 
 bool known(int32_t dtype) { return dtype == TFH_BF16 || dtype == TFH_F16 || dtype == TFH_F32 || dtype == TFH_F64; }
 size_t sums_size(int32_t dtype) { return dtype == TFH_F64 ? 8 : 4; }
@@ -22,7 +22,7 @@ int32_t check_dtype(int32_t dtype) {
 }
 int32_t check_groups(const tfh_row_groups* g, bool positions) {
     if (!g) return set_error(TFH_ERR_INVALID_ARGUMENT, "null row groups");
-    if (g->n_groups < 1) return set_error(TFH_ERR_INVALID_ARGUMENT, "row groups need at least one group, got %d", g->n_groups);
+    if (g->n_groups < 1 || g->n_groups > MOST) return set_error(TFH_ERR_INVALID_ARGUMENT, "row groups need at least one group and less than 2^31 - 2^20, got %d", g->n_groups);
     if (g->n_rows < 0 || g->n_rows > MOST) return set_error(TFH_ERR_INVALID_ARGUMENT, "row groups: %lld rows are out of range", (long long)g->n_rows);
     if (g->fan < 1) return set_error(TFH_ERR_INVALID_ARGUMENT, "row groups: a fan of %d", g->fan);
     if (g->n_rows % g->fan) return set_error(TFH_ERR_INVALID_ARGUMENT, "row groups: %lld rows are no multiple of the fan %d", (long long)g->n_rows, g->fan);

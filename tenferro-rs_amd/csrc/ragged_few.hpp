@@ -15,7 +15,7 @@ namespace ragged {
 
 constexpr int FEW_WAVES = 8;
 template <int MODE> constexpr int few_low_waves() { return MODE == SHARED ? 4 : 0; }
-template <int TR> constexpr int few_ahead() { return TR == 1 ? 4 : TR == 2 ? 3 : TR == 4 ? 2 : 1; }   // what LDS leaves room for
+template <int TR> constexpr int few_ahead() { return TR == 1 ? 4 : TR == 2 ? 3 : 2; }   // what LDS leaves room for
 template <int TR> constexpr int few_lds() { return FEW_WAVES * few_ahead<TR>() * (16 * TR + 16) * 128; }
 template <int MODE> constexpr int few_threads() { return 64 * (FEW_WAVES + few_low_waves<MODE>()); }
 

@@ -3,7 +3,8 @@
 //
 // A block has 32 rows of one group and all r columns; its waves share out k, 64 of it at a time, each with tiles of its own
 // in LDS that its own loads fill some steps ahead -- whole lines of every row, which loads in operand position would ask for
-// in four pieces -- and no barrier until their sums meet.
+// in four pieces -- and no barrier until their sums meet.  64 rows by 4096 k's, rank 16: 9 us, bound by the loads' latency; 8192
+// rows, rank 32: 14 us from caches (4.8 TB/s), 28 from HBM.
 #pragma once
 #include "ragged_fast.hpp"
 

@@ -756,6 +756,19 @@ def test_products_refuse_what_does_not_fit(tf):
     refused(tf, grad(db=V(3, 24, 16)), tf.ShapeMismatch)
 
 
+@pytest.mark.parametrize("big", [0x7ff00001, 0x7fffffff, 1 << 31, 1 << 40])
+def test_what_32_bit_indices_cannot_walk_is_refused(tf, big):
+    L, V, G = tf.lib(), lambda *d: view(tf, d), lambda **k: row_groups(tf, **k)
+    refused(tf, L.tfh_ragged_gemm(4, G(n_rows=1), 0, 1.0, V(1, 16), V(3, 16, big), 0.0, V(1, big), None), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm(4, G(n_rows=1), 0, 1.0, V(1, big), V(3, big, 16), 0.0, V(1, 16), None), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm(4, G(n_rows=big), 0, 1.0, V(big, 16), V(3, 16, 16), 0.0, V(big, 16), None), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm_grad(4, G(n_rows=1), 0, 1.0, V(1, big), V(1, 8), 0.0, V(3, big, 8), None), tf.InvalidArgument)
+    refused(tf, L.tfh_combine_rows(4, G(n_rows=1), V(1, big), None, V(1, big), None), tf.InvalidArgument)
+    refused(tf, L.tfh_group_rows(32, V(big), 4, 4096, 4096, None, 4096, 1 << 40, None), tf.InvalidArgument)
+    if big <= 0x7fffffff:
+        refused(tf, L.tfh_ragged_gemm(4, G(n_groups=big), 0, 1.0, V(8, 16), V(big, 16, 8), 0.0, V(8, 8), None), tf.InvalidArgument)
+
+
 def test_grouping_refuses_what_does_not_fit(tf):
     L = tf.lib()
     run = lambda bits=32, ids=None, n=4, off=4096, order=4096, ws=4096, b=1 << 20: L.tfh_group_rows(bits, ids or view(tf, [8]), n, off, order, None, ws, b, None)
