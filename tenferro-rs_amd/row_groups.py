@@ -26,19 +26,22 @@ class tfh_row_groups(C.Structure):
 
 
 _CODES, _TYPES = {}, {}
+_stream_of = None       # device index -> the handle of torch's current stream
 
 
 def _codes():
+    global _stream_of
     if not _CODES:
         import torch
+        # (the call behind torch.cuda.current_stream, without the object: 1 us of the 10 that a call takes)
+        _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
         _CODES.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.float64: F64})
         _TYPES.update({c: t for t, c in _CODES.items()})
     return _CODES
 
 
 _VIEW_BYTES = C.c_char * C.sizeof(tfh_view)
-_PACKERS = {r: (struct.Struct("<Qiiq%dq" % r).pack_into, struct.Struct("<%dq" % r).pack_into) for r in range(5)}
-_STRIDES_AT = tfh_view.strides.offset
+_PACKERS = [struct.Struct("<Qiiq%dq%dx%dq" % (r, tfh_view.strides.offset - tfh_view.dims.offset - 8 * r, r)).pack_into for r in range(5)]
 
 
 def _view(t):
@@ -51,9 +54,7 @@ def _view(t):
     if rank > 4:
         raise RankMismatch(f"rank mismatch: expected at most 3, got {rank}", 3, rank)
     v = _VIEW_BYTES()
-    head, tail = _PACKERS[rank]
-    head(v, 0, t.data_ptr(), rank, 0, 0, *t.shape)
-    tail(v, _STRIDES_AT, *t.stride())
+    _PACKERS[rank](v, 0, t.data_ptr(), rank, 0, 0, *t.shape, *t.stride())
     return v
 
 
@@ -106,13 +107,12 @@ class _Call:
                 raise CrossMemorySpaceOperation(f"cross-memory-space operation between {GpuMemory(self.device)!r} and {GpuMemory(groups.device)!r}",
                                                 GpuMemory(self.device), GpuMemory(groups.device))
             self.used.append(groups)
-        self.current = torch.cuda.current_stream(self.device).cuda_stream
+        self.current = _stream_of(self.device)
         self.stream = self.current if stream is None else stream
         self.guard = None
         if torch.cuda.current_device() != self.device:
             self.guard = torch.cuda.device(self.device)
         self.ordered = False
-        self.place = None
 
     def __enter__(self):
         if self.guard is not None:
@@ -137,9 +137,13 @@ class _Call:
         if like is not None and not isinstance(like, Tensor):
             t = torch.empty_like(like)
         else:
-            if self.place is None:
-                self.place = torch.device("cuda", self.device) if isinstance(self.like, Tensor) else self.like.device
-            t = torch.empty(dims, dtype=dtype if isinstance(dtype, torch.dtype) else _TYPES[dtype], device=self.place)
+            tdt = dtype if isinstance(dtype, torch.dtype) else _TYPES[dtype]
+            if isinstance(self.like, Tensor):
+                t = torch.empty(dims, dtype=tdt, device=torch.device("cuda", self.device))
+            elif dtype == self.dtype:
+                t = self.like.new_empty(dims)
+            else:
+                t = self.like.new_empty(dims, dtype=tdt)
         self.used.append(t)
         return t
 
@@ -212,7 +216,8 @@ class RowGroups:
         if n_groups < 1:
             raise InvalidArgument(f"invalid argument: {n_groups} groups")
         fan = ids.shape[1] if ids.dim() == 2 else 1
-        current = torch.cuda.current_stream(device).cuda_stream
+        _CODES or _codes()
+        current = _stream_of(device)
         st = current if stream is None else stream
         need = lib().tfh_group_rows_workspace(n, n_groups)
         # one buffer for all: [order | positions | offsets | scratch], each 16-byte aligned
@@ -227,7 +232,10 @@ class RowGroups:
                 _check(lib().tfh_stream_wait_event(st, CompletionEvent(current)._h))
             p = buf.data_ptr()
             _check(lib().tfh_group_rows(bits, _view(ids), n_groups, p + 4 * at_o, p, p + 4 * at_p, p + 4 * at_w, need, st))
-            g = cls(buf[at_o:at_o + n_groups + 1], buf[:n], buf[at_p:at_p + n], fan=max(1, fan))
+            g = cls.__new__(cls)
+            g.offsets, g.order, g.positions = buf[at_o:at_o + n_groups + 1], buf[:n], buf[at_p:at_p + n]
+            g.n_rows, g.n_groups, g.fan, g.device, g.event = n, n_groups, max(1, fan), device, None
+            g._c = tfh_row_groups(p + 4 * at_o, p, p + 4 * at_p, n, n_groups, g.fan)
             if st != current:
                 g.event = CompletionEvent(st)
                 _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
