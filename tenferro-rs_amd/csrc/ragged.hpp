@@ -612,8 +612,7 @@ __global__ __launch_bounds__(GENERAL_THREADS * KW, KW == 1 ? 2 : 4) void ragged_
         __syncthreads();
         if (team > 0) __builtin_memcpy(lds + tid * sizeof(acc), acc, sizeof(acc));
         __syncthreads();
-        if (team > 0) return;
-        for (int w = 1; w < KW; ++w) {
+        for (int w = 1; team == 0 && w < KW; ++w) {
             typename NT::acc4 more[XT][YT];
             __builtin_memcpy(more, all_lds + w * 2 * (TM + TN) * 128 + tid * sizeof(acc), sizeof(acc));
 #pragma unroll
@@ -627,6 +626,55 @@ __global__ __launch_bounds__(GENERAL_THREADS * KW, KW == 1 ? 2 : 4) void ragged_
     const W beta = (W)a.beta;
     if constexpr (MODE == ROWS)
         if (a.scales && real) alpha *= ((const W*)a.scales)[t.group];
+    if (a.c_n == 1 && !a.use_beta) {
+        // Through LDS, so that a wave stores whole runs of a row, 16 bytes a lane; the chunk index is XORed with the row because the
+        // rows of a register would meet in one bank otherwise.  (Straight from the registers a store has 32 bytes of each of 16 rows,
+        // an element a lane: the gradients of 40 matrices of 3776 x 1861 from 50 rows, f16: 620 us so, 320 by LDS.)
+        constexpr int PER = 16 / (int)sizeof(TO), ROW = TN / PER;   // elements of a chunk, chunks of a row
+        static_assert(TM * TN * sizeof(TO) <= 2 * (TM + TN) * 128, "the results fit a team's tiles");
+        auto place = [&](int r, int n) { return all_lds + r * (TN * (int)sizeof(TO)) + (((n / PER) ^ (r & (ROW - 1))) << 4) + n % PER * (int)sizeof(TO); };
+        __syncthreads();
+        if (KW == 1 || team == 0)
+#pragma unroll
+            for (int x = 0; x < XT; ++x)
+#pragma unroll
+                for (int y = 0; y < YT; ++y) {
+                    TO out[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[i] = real ? (TO)(alpha * acc[x][y][i]) : (TO)0;
+                    const int r = (wm * XT + x) * 16 + j, n = (wn * YT + y) * 16;
+                    if constexpr (sizeof(TO) == 8) {   // (every fourth column in a lane)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) *(TO*)place(r, n + NT::row(q, i)) = out[i];
+                    } else {
+                        __builtin_memcpy(place(r, n + NT::row(q, 0)), out, sizeof(out));
+                    }
+                }
+        __syncthreads();
+        const int rows = MODE == OUTER ? (a.M - m0 < TM ? a.M - m0 : TM) : t.rows;
+        for (int id = threadIdx.x; id < rows * ROW; id += GENERAL_THREADS * KW) {
+            const int r = id / ROW, n = id % ROW * PER;
+            if (n0 + n >= a.N) continue;
+            int64_t row = MODE == OUTER ? m0 + r : t.first + r;
+            if constexpr (MODE != OUTER)
+                if (a.scatter && a.order) {
+                    row = a.order[row];
+                    if (row < 0 || row >= a.n_rows) continue;
+                }
+            TO* const c = (TO*)a.C + (MODE == OUTER ? t.group * a.c_group : 0) + row * a.c_row + n0 + n;
+            TO out[PER];
+            __builtin_memcpy(out, place(r, n), 16);
+            if (n0 + n + PER <= a.N) {
+                __builtin_memcpy(c, out, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (n0 + n + i < a.N) c[i] = out[i];
+            }
+        }
+        return;
+    }
+    if (team > 0) return;
 #pragma unroll
     for (int x = 0; x < XT; ++x) {
         const int r = (wm * XT + x) * 16 + j;
