@@ -221,7 +221,7 @@ int32_t tfh_fill(int32_t dtype, const void* value, tfh_view* out, tfh_stream str
  * tfh_row_groups: n_rows rows listed group by group.
  *   offsets    [n_groups + 1], ascending from 0: group g is p = offsets[g] .. offsets[g + 1]; the rows behind
  *              offsets[n_groups] belong to no group
- *   order      [n_rows] or NULL (the rows lie in that order already): place p holds row order[p]
+ *   order      [n_rows] or NULL (the rows lie in that order already): place p holds row order[p], no row twice
  *   positions  [n_rows] or NULL: where row i stands, -1 for a row of no group
  *   fan        rows per source row (a token's choices): row i = t * fan + j is choice j of token t
  * Entries out of range are treated as absent (offsets are clamped to [0, n_rows]); they never lead out of the views.

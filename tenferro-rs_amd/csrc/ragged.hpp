@@ -252,7 +252,7 @@ struct Patches {
         pm = tm < 4 ? tm : 4, pn = tn < 4 ? tn : 4;
         across = (tm + pm - 1) / pm, each = across * ((tn + pn - 1) / pn);
     }
-    __host__ __device__ int64_t blocks(int n_groups) const { return ((int64_t)n_groups * each + 7) / 8 * 8 * (pm * pn); }
+    __host__ __device__ int64_t blocks(int n_groups) const { return ((int64_t)n_groups * across * ((tn + pn - 1) / pn) + 7) / 8 * 8 * (pm * pn); }
 };
 __device__ __forceinline__ bool outer_tile(const Args& a, int TM, int TN, uint32_t block, Tile& t) {
     const Patches s(a, TM, TN);

@@ -559,6 +559,61 @@ def test_an_adapters_middle_may_exceed_the_operands_range(tf, torch, name, big):
     close(tf.adapter_gemm(x.cuda(), w.cuda(), a.cuda(), b.cuda(), made(tf, torch, ids, 2)), want, size, 68, name, MIDDLE[name] * low)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float32", "float64"])
+@pytest.mark.parametrize("K,N", [(64, 48), (37, 21), (600, 72)])
+def test_products_of_views_with_negative_and_zero_strides(tf, torch, name, K, N):
+    rng = np.random.default_rng(K)
+    rows, groups, size = 70, 3, torch.finfo(getattr(torch, name)).bits // 8
+    code = {"bfloat16": tf.BF16, "float32": tf.F32, "float64": tf.F64}[name]
+    a, b = tensor(torch, rng, (rows, K), name), tensor(torch, rng, (groups, K, N), name, K ** -0.5)
+    A, B = a.cuda(), b.cuda()
+    g = tf.RowGroups(torch.tensor([0, 30, 31, 64], dtype=torch.int32, device="cuda"), n_rows=rows)
+    at = lambda t, dims, strides, first: view(tf, dims, strides, t.data_ptr() + first * size)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(va, vb, a, b):
+        c = torch.zeros(rows, N, dtype=A.dtype, device="cuda")
+        vc = at(c, [rows, N], [-N, 1], (rows - 1) * N)          # its rows backwards
+        tf._check(tf.lib().tfh_ragged_gemm(code, C.byref(g._c), 4, 1.0, va, vb, 0.0, vc, stream))
+        want, size_of = ragged_reference(torch, a, b, [0, 30, 31, 64], list(range(rows)), 1, False)
+        close(c.flip(0), want, size_of, K, name)
+
+    plain_a, plain_b = at(A, [rows, K], [K, 1], 0), at(B, [groups, K, N], [K * N, N, 1], 0)
+    run(at(A, [rows, K], [-K, 1], (rows - 1) * K), plain_b, a.flip(0), b)
+    run(at(A, [rows, K], [0, 1], 5 * K), plain_b, a[5].expand(rows, K), b)
+    run(at(A, [rows, K], [K, -1], K - 1), plain_b, a.flip(1), b)
+    run(plain_a, at(B, [groups, K, N], [-K * N, N, 1], (groups - 1) * K * N), a, b.flip(0))
+    run(plain_a, at(B, [groups, K, N], [K * N, -N, 1], (K - 1) * N), a, b.flip(1))
+    run(plain_a, at(B, [groups, K, N], [0, N, 1], K * N), a, b[1].expand(groups, K, N))
+    run(plain_a, at(B, [groups, K, N], [K * N, 0, 1], 0), a, b[:, :1].expand(groups, K, N))
+    db = torch.zeros(groups, K, N, dtype=A.dtype, device="cuda")
+    dc = tensor(torch, rng, (rows, N), name)
+    D = dc.cuda()
+    tf._check(tf.lib().tfh_ragged_gemm_grad(code, C.byref(g._c), 0, 1.0, at(A, [rows, K], [-K, 1], (rows - 1) * K), at(D, [rows, N], [-N, 1], (rows - 1) * N), 0.0,
+                                            at(db, [groups, K, N], [K * N, -N, 1], (K - 1) * N), stream))
+    for i, (x, y) in enumerate([(0, 30), (30, 31), (31, 64)]):
+        X, Y = a.flip(0)[x:y].double(), dc.flip(0)[x:y].double()
+        close(db[i].flip(0), X.t() @ Y, X.abs().t() @ Y.abs(), y - x, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("K,N,R", [(96, 160, 16), (35, 17, 5)])
+def test_adapters_of_rows_that_lie_in_order(tf, torch, name, K, N, R):
+    # no order: the groups' rows one after the other, the last ones of none
+    rng = np.random.default_rng(R)
+    ids = np.repeat([0, 1, 2, -1], [40, 1, 70, 6])
+    x, w = tensor(torch, rng, (len(ids), K), name), tensor(torch, rng, (K, N), name, K ** -0.5)
+    a, b, dy = tensor(torch, rng, (3, K, R), name, K ** -0.5), tensor(torch, rng, (3, R, N), name), tensor(torch, rng, (len(ids), N), name)
+    g = tf.RowGroups(torch.tensor([0, 40, 41, 111], dtype=torch.int32, device="cuda"), n_rows=len(ids))
+    want, size, low = adapter_reference(torch, x, w, a, b, None, ids)
+    close(tf.adapter_gemm(x.cuda(), w.cuda(), a.cuda(), b.cuda(), g), want, size, K + R, name, MIDDLE[name] * low)
+    listed = made(tf, torch, ids, 3)
+    one, other = (tf.adapter_gemm_backward(x.cuda(), w.cuda(), a.cuda(), b.cuda(), dy.cuda(), h) for h in (g, listed))
+    assert all(torch.equal(p, q) for p, q in zip(one, other))
+
+
 # ------------------------------------------------------------------------------------------------------ together, streams, graphs
 def expert_layer(tf, x, up, down, ids, gates):
     groups = tf.RowGroups.from_ids(ids, up.shape[0])
