@@ -48,16 +48,17 @@ template <class C, int MODE, bool BKFAST> bool unit_strides(const Args& a) {
     if (MODE == OUTER) return a.a_col == 1 && a.M >= E && a.b_n == 1 && a.N >= E;
     return a.a_col == 1 && a.K >= E && (BKFAST ? a.b_k == 1 : a.b_n == 1 && a.N >= E);
 }
-// Fewer than two blocks a compute unit wait for their loads, stage after stage: tiles of 32 x 32 then, four times the blocks of
-// 64 x 64, and four teams to share out k, from eight stages on (f64, 236 rows, 1472 x 38: 65 us against 24; 200 bf16 rows of four
-// groups, 4001 x 1001: 63 and 29; f64, 1600 rows of eight, 256 x 640: 27 and 29; 1024 x 640: 81 and 67.  702 blocks, f32, 3000
-// rows, 1000 x 800: 79 and 87).  `bytes`: of an operand's element.  Aligned 16-bit operands as well, and gradients from more than
-// 512 rows of a group on (200 rows of two groups, 4096 x 512: 38 us against 13; gradients of 8192 of four, 256 x 256: 38 and 11;
-// 16 384 of eight, 512 x 256: 39 and 30; of 32 groups, 128 x 128, 512 rows each: 11 and 13).
+// Few blocks wait for their loads, stage after stage: tiles of 32 x 32 then, four times the blocks of 64 x 64, and four teams to
+// share out k, where that has eight stages at least and the blocks are fewer than one a compute unit, or two where k has 32 stages
+// (f64, 236 rows, 1472 x 38: 65 us against 24; 200 bf16 rows of four groups, 4001 x 1001: 63 and 29, of two, 4096 x 512, aligned: 38
+// and 13; 248 blocks, f16, 3001 x 500: 42 and 37; 299 blocks, 1001 x 777: 18 and 29; 330, f64, 256 x 640: 27 and 29, 1024 x 640: 81 and
+// 67; 702, f32, 1000 x 800: 79 and 87).  Gradients: fewer than two, from more than 512 rows of a group on (8192 of four, 256 x 256:
+// 38 and 11; 16 384 of eight, 512 x 256: 38 and 29; of 32 groups, 128 x 128, 512 rows each: 11 and 13).  `bytes`: of an operand's
+// element; aligned 16-bit operands leave their own kernels for this one as well.
 template <int MODE> bool starved(const Args& a, int bytes) {
     const int64_t blocks = MODE == OUTER ? Patches(a, 64, 64).blocks(a.n_groups) : (MODE == ROWS ? row_tiles(a, 64) : tiles(a.n_rows, 64)) * tiles(a.N, 64);
     const int64_t k = MODE == OUTER ? a.n_rows / a.n_groups : a.K;
-    return blocks < 512 && k * bytes >= 1024 + (MODE == OUTER ? bytes : 0);
+    return blocks < (MODE == OUTER || k * bytes >= 4096 ? 512 : 256) && k * bytes >= 1024 + (MODE == OUTER ? bytes : 0);
 }
 template <class TA, class TB, class C, class TO, int MODE, bool BKFAST>
 int32_t launch_general(const Args& a, void* stream) {
