@@ -11,8 +11,9 @@
 // so a fragment has 16 k's products to arrive in, a load those of all slots but one, and there is one barrier per stage.
 //
 // Bound by the matrix cores, and by their power with random numbers.  Reached, bf16: one group of 16 384 rows, 8192 x 4096: 1250
-// TFLOP/s (a library product: 1490); 65 536 gathered rows of 64 uneven groups, 2048 x 2048: 590 us, 930 TFLOP/s, of which the groups'
-// last tiles and the last round cost a tenth; gradients of 32 768 rows of 32 uneven groups, 2048 x 1024: 201 us, 684, with their rows
+// TFLOP/s (a library product: 1490); 65 536 gathered rows of 64 uneven groups, 2048 x 2048: 590 us, 930 TFLOP/s, the matrix cores 46 %
+// busy at 1.8 GHz -- a tile of 32 stages starts and ends with a tenth of its time, the groups' last tiles and the last round cost as
+// much, and LDS is read and written three quarters of the time; gradients of 32 768 rows of 32 uneven groups, 2048 x 1024: 201 us, 684, with their rows
 // looked up (163 us, 843 without); adapters' shared product, 16 384 x 4096 x 4096: 530 us, 1040.
 #pragma once
 #include <utility>
