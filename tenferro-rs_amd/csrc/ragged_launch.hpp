@@ -134,18 +134,27 @@ int32_t launch_few(const Args& a, void* stream) {
     TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR>), dim3((unsigned)blocks), dim3(few_threads<MODE>()), few_lds<TR>(), (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
-template <class T, bool BKFAST, int YT>
-int32_t launch_thin(const Args& a, void* stream) {
+template <class T, bool BKFAST, int YT, int WAVES>
+int32_t launch_thin_waves(const Args& a, void* stream) {
     const int64_t blocks = row_tiles(a, THIN_ROWS);
     if (blocks <= 0) return TFH_OK;
     static const bool once = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT>), hipFuncAttributeMaxDynamicSharedMemorySize, thin_lds<YT>());
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (thin_lds<YT, WAVES>()));
         return true;
     }();
     (void)once;
     static const std::string label = std::string("(ragged_thin_kernel<") + type_name<T>() + (BKFAST ? ", k, " : ", n, ") + std::to_string(32 * YT) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT>), dim3((unsigned)blocks), dim3(64 * thin_waves<YT>()), (thin_lds<YT>()), (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), (thin_lds<YT, WAVES>()), (hipStream_t)stream, a);
     return hip_check(hipGetLastError(), "product over groups of rows");
+}
+
+template <class T, bool BKFAST, int YT>
+int32_t launch_thin(const Args& a, void* stream) {
+    // Eight waves to share out k where each block has a compute unit to itself; four, whose tiles leave room for a second block, beyond
+    // (8192 rows of 16 groups, 4096 k's, from HBM: 31 and 25 us)
+    if constexpr (YT == 1)
+        if (row_tiles(a, THIN_ROWS) <= 256) return launch_thin_waves<T, BKFAST, YT, 8>(a, stream);
+    return launch_thin_waves<T, BKFAST, YT, 4>(a, stream);
 }
 
 template <class T> int32_t launch_product(int kind, const Args& a, void* stream) {

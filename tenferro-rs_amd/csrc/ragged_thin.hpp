@@ -4,7 +4,7 @@
 // A block has 32 rows of one group and all r columns; its waves share out k, 64 of it at a time, each with tiles of its own
 // in LDS that its own loads fill some steps ahead -- whole lines of every row, which loads in operand position would ask for
 // in four pieces -- and no barrier until their sums meet.  64 rows by 4096 k's, rank 16: 9 us, bound by the loads' latency; 8192
-// rows, rank 32: 14 us from caches (4.8 TB/s), 28 from HBM.
+// rows, rank 32: 14 us from caches (4.8 TB/s), 25 from HBM.
 #pragma once
 #include "ragged_fast.hpp"
 
@@ -12,10 +12,9 @@ namespace tfh {
 namespace ragged {
 
 constexpr int THIN_ROWS = 32;
-// Waves of a block and steps that each has in LDS or on their way, by what 32 YT columns leave room for.
-template <int YT> constexpr int thin_waves() { return YT == 1 ? 8 : 4; }
+// Steps that a wave has in LDS or on their way, by what 32 YT columns leave room for.
 template <int YT> constexpr int thin_ahead() { return YT == 2 ? 3 : 2; }
-template <int YT> constexpr int thin_lds() { return thin_waves<YT>() * thin_ahead<YT>() * (THIN_ROWS + 32 * YT) * 128; }
+template <int YT, int WAVES> constexpr int thin_lds() { return WAVES * thin_ahead<YT>() * (THIN_ROWS + 32 * YT) * 128; }
 
 // V's row p as a pair of numbers of the operands' type, v = up (hi + lo): 16 bits of it in bf16, 22 in f16, so that it is
 // no rounding of its own beside the result's.  f16 alone has a short exponent: its rows are brought to [2^7, 2^8) first.
@@ -53,9 +52,9 @@ __device__ __forceinline__ void store_pair(const Args& a, int64_t p, const float
     }
 }
 
-template <class T, bool BKFAST, int YT>
-__global__ __launch_bounds__((64 * thin_waves<YT>()), 1) void ragged_thin_kernel(const Args a) {
-    constexpr int TN = 32 * YT, RB = TN / 8, WAVES = thin_waves<YT>(), AHEAD = thin_ahead<YT>();   // RB: chunks of a row of k of F
+template <class T, bool BKFAST, int YT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 1) void ragged_thin_kernel(const Args a) {
+    constexpr int TN = 32 * YT, RB = TN / 8, AHEAD = thin_ahead<YT>();   // RB: chunks of a row of k of F
     constexpr int SLOT = (THIN_ROWS + TN) * 128, LOADS = 4 + 4 * YT;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     char* const lds = (char*)smem_raw;
