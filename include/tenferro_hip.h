@@ -253,10 +253,18 @@ typedef enum tfh_rows_flag { TFH_ROWS_GATHER_A = 1, TFH_ROWS_SCATTER_C = 2, TFH_
 int32_t tfh_ragged_gemm(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* a,
                         const tfh_view* b, double beta, const tfh_view* c, tfh_stream stream);
 /* The gradient of that product's B: dB[g] = alpha * sum over p in g of A[src(p), :]^T dC[p, :] + beta * dB[g]; a group
- * without rows gets beta * dB[g].  (The gradient of A is tfh_ragged_gemm with dC and B transposed.)
+ * without rows gets beta * dB[g].
  * A [sources, K], dC [n_rows, N], dB [n_groups, K, N]; of the flags TFH_ROWS_GATHER_A. */
 int32_t tfh_ragged_gemm_grad(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* a,
                              const tfh_view* dc, double beta, const tfh_view* db, tfh_stream stream);
+/* The gradient of that product's A: dA[s, :] = alpha * sum over the places p of a group with src(p) = s of dC[p, :] . B[g(p)]^T,
+ * zeros for a row that stands in no group.  The parts of a row that several places read (TFH_ROWS_GATHER_A with a fan above 1, which
+ * needs positions) are added up in the sums' type and rounded once.  dC [n_rows, N], B [n_groups, K, N], dA [sources, K]; of the
+ * flags TFH_ROWS_GATHER_A.  workspace: tfh_ragged_gemm_grad_a_workspace(dtype, n_rows, K, fan, flags) bytes (0 where no parts are
+ * added up), 16-byte aligned. */
+size_t tfh_ragged_gemm_grad_a_workspace(int32_t dtype, int64_t n_rows, int64_t k, int32_t fan, int32_t flags);
+int32_t tfh_ragged_gemm_grad_a(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* dc,
+                               const tfh_view* b, const tfh_view* da, void* workspace, size_t workspace_bytes, tfh_stream stream);
 
 /* Y[t, :] = sum_j weights[t, j] * X[positions[t * fan + j], :]: the rows of a token joined again.  A choice of no group
  * adds nothing.  X [n_rows, N], weights [n_rows / fan, fan] of the sums' type (f32; f64 for TFH_F64) or NULL (ones),

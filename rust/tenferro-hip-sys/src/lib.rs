@@ -195,6 +195,10 @@ extern "C" {
         b: *const tfh_view, beta: f64, c: *const tfh_view, stream: tfh_stream) -> i32;
     pub fn tfh_ragged_gemm_grad(dtype: i32, groups: *const tfh_row_groups, flags: i32, alpha: f64, a: *const tfh_view,
         dc: *const tfh_view, beta: f64, db: *const tfh_view, stream: tfh_stream) -> i32;
+    pub fn tfh_ragged_gemm_grad_a_workspace(dtype: i32, n_rows: i64, k: i64, fan: i32, flags: i32) -> usize;
+    pub fn tfh_ragged_gemm_grad_a(dtype: i32, groups: *const tfh_row_groups, flags: i32, alpha: f64,
+        dc: *const tfh_view, b: *const tfh_view, da: *const tfh_view, workspace: *mut c_void, workspace_bytes: usize,
+        stream: tfh_stream) -> i32;
     pub fn tfh_combine_rows(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view, weights: *const tfh_view,
         y: *const tfh_view, stream: tfh_stream) -> i32;
     pub fn tfh_combine_rows_grad(dtype: i32, groups: *const tfh_row_groups, x: *const tfh_view,

@@ -96,6 +96,21 @@ impl RowGroups {
         check(unsafe { sys::tfh_ragged_gemm_grad(dtype_tag::<T>()?, &g, flags, alpha, &a, &dc, beta, &db, stream.raw()) })
     }
 
+    /// `da[s] = alpha * sum over p in a group with src(p) = s of dc[p] . b[g(p)]^T`.  The returned buffer is the call's
+    /// scratch: keep it until the stream has passed the call.
+    pub fn gemm_grad_a<T: ScalarBase>(&self, flags: i32, alpha: f64, dc: &HipView<T>, b: &HipView<T>, da: &mut HipViewMut<T>, stream: &Stream) -> Result<HipBuffer<u8>> {
+        let k = b.dims().get(1).copied().ok_or_else(|| Error::RankMismatch { expected: 3, got: b.dims().len() })?;
+        let need = unsafe { sys::tfh_ragged_gemm_grad_a_workspace(dtype_tag::<T>()?, self.n_rows as i64, k as i64, self.fan as i32, flags) };
+        let scratch = HipBuffer::<u8>::new(need.max(1), self.offsets.device_id())?;
+        let (g, dc, b, da) = (self.raw(), dc.raw(), b.raw(), da.raw());
+        check(unsafe {
+            sys::tfh_ragged_gemm_grad_a(
+                dtype_tag::<T>()?, &g, flags, alpha, &dc, &b, &da, scratch.as_device_ptr() as *mut c_void, need, stream.raw(),
+            )
+        })?;
+        Ok(scratch)
+    }
+
     /// `y[t] = sum_j weights[t, j] * x[positions[t * fan + j]]`.
     pub fn combine<T: ScalarBase>(&self, x: &HipView<T>, weights: Option<&HipView<T>>, y: &mut HipViewMut<T>, stream: &Stream) -> Result<()> {
         let (g, x, w, y) = (self.raw(), x.raw(), optional(weights), y.raw());

@@ -125,11 +125,13 @@ def lib():
         L.tfh_subscripts_nesting.argtypes = [C.c_void_p, C.c_char_p, C.c_size_t]
         L.tfh_plan_describe.argtypes = [C.c_void_p, C.c_char_p, C.c_size_t]
         P, i32, i64, sz, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_double
-        L.tfh_group_rows_workspace.restype = L.tfh_adapter_workspace.restype = C.c_size_t
+        L.tfh_group_rows_workspace.restype = L.tfh_adapter_workspace.restype = L.tfh_ragged_gemm_grad_a_workspace.restype = C.c_size_t
         L.tfh_group_rows_workspace.argtypes = [i64, i32]
         L.tfh_group_rows.argtypes = [i32, P, i32, P, P, P, P, sz, P]
         L.tfh_ragged_gemm.argtypes = [i32, P, i32, f64, P, P, f64, P, P]
         L.tfh_ragged_gemm_grad.argtypes = [i32, P, i32, f64, P, P, f64, P, P]
+        L.tfh_ragged_gemm_grad_a_workspace.argtypes = [i32, i64, i64, i32, i32]
+        L.tfh_ragged_gemm_grad_a.argtypes = [i32, P, i32, f64, P, P, P, P, sz, P]
         L.tfh_combine_rows.argtypes = [i32, P, P, P, P, P]
         L.tfh_combine_rows_grad.argtypes = [i32, P, P, P, P, P, P, P]
         L.tfh_adapter_workspace.argtypes = [i32, i64, i64, i32]

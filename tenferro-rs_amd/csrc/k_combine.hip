@@ -18,17 +18,16 @@ namespace {
 
 constexpr int CHUNKS = 2;   // 16-byte pieces of a row that a lane has in flight for each of the choices
 
-// E elements of a row from its n-th on, of which the row has `total`.  UNIT: next to each other, and E of them at least; a piece
+// E elements, 16 bytes of a T, of a row from its n-th on, of which the row has `total`.  UNIT: next to each other, and E of them at least; a piece
 // that the row ends in is its last E elements instead.
 template <class T, bool UNIT> __device__ __forceinline__ u32x4 piece(const T* row, int64_t stride, int n, int total) {
     constexpr int E = Num<T>::E;
     if constexpr (UNIT) return load_unit<T>(row + (n + E <= total ? n : total - E));
     else return load_chunk<T, T>(row + n * stride, stride, total - n);
 }
-template <class T, bool UNIT> __device__ __forceinline__ void put_piece(T* row, int64_t stride, int n, int total, const T (&e)[Num<T>::E]) {
-    constexpr int E = Num<T>::E;
+template <class T, bool UNIT, int E> __device__ __forceinline__ void put_piece(T* row, int64_t stride, int n, int total, const T (&e)[E]) {
     if constexpr (UNIT) {
-        if (n < total) __builtin_memcpy(row + (n + E <= total ? n : total - E), e, 16);
+        if (n < total) __builtin_memcpy(row + (n + E <= total ? n : total - E), e, sizeof(e));
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -49,10 +48,11 @@ template <int F, class W> __device__ __forceinline__ void choices_of(const Combi
     }
 }
 
-template <class T, int F, bool UNIT>
+// X: x's type, T or that of the sums (parts of a sum that is rounded here for the first time).
+template <class T, class X, int F, bool UNIT>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
     typedef typename Num<T>::acc W;
-    constexpr int E = Num<T>::E;
+    constexpr int E = Num<X>::E;
     const int lane = threadIdx.x & 63, step = 64 * E * gridDim.y;
     const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.tokens) return;
@@ -67,13 +67,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
             for (int j = 0; j < F; ++j)
                 if (p[j] >= 0)
 #pragma unroll
-                    for (int c = 0; c < CHUNKS; ++c) v[j][c] = piece<T, UNIT>((const T*)a.x + p[j] * a.x_row, a.x_n, n0 + c * step, a.n);
+                    for (int c = 0; c < CHUNKS; ++c) v[j][c] = piece<X, UNIT>((const X*)a.x + p[j] * a.x_row, a.x_n, n0 + c * step, a.n);
 #pragma unroll
             for (int j = 0; j < F; ++j)
                 if (p[j] >= 0)
 #pragma unroll
                     for (int c = 0; c < CHUNKS; ++c) {
-                        T e[E];
+                        X e[E];
                         __builtin_memcpy(e, &v[j][c], 16);
 #pragma unroll
                         for (int i = 0; i < E; ++i) sum[c][i] += w[j] * (W)e[i];
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
             T out[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) out[i] = (T)sum[c][i];
-            put_piece<T, UNIT>((T*)a.y + t * a.y_row, a.y_n, n0 + c * step, a.n, out);
+            put_piece<T, UNIT, E>((T*)a.y + t * a.y_row, a.y_n, n0 + c * step, a.n, out);
         }
         if (a.fan > F) choices_of(a, t, 0, p, w);
     }
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, 
         const T zero[E] = {};
         const int from = clamp_row(a.offsets[a.n_groups], a.n_rows);
         for (int64_t p = from + ((int)blockIdx.x - token_blocks) * 4 + (threadIdx.x >> 6); p < a.n_rows; p += ((int)gridDim.x - token_blocks) * 4)
-            for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT>((T*)a.dx + p * a.dx_row, a.dx_n, n, a.n, zero);
+            for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT, E>((T*)a.dx + p * a.dx_row, a.dx_n, n, a.n, zero);
         return;
     }
     const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, 
                         T out[E];
 #pragma unroll
                         for (int i = 0; i < E; ++i) out[i] = (T)(w[j] * (W)de[i]);
-                        put_piece<T, UNIT>((T*)a.dx + p[j] * a.dx_row, a.dx_n, n, a.n, out);
+                        put_piece<T, UNIT, E>((T*)a.dx + p[j] * a.dx_row, a.dx_n, n, a.n, out);
                     }
                 }
             }
@@ -162,12 +162,12 @@ template <class T> constexpr const char* name_of(const char* bf16, const char* f
     return __is_same(T, __bf16) ? bf16 : __is_same(T, _Float16) ? f16 : __is_same(T, float) ? f32 : f64;
 }
 
-template <class T, int F, bool UNIT> int32_t combine_as(const CombineArgs& a, hipStream_t st) {
-    const int64_t blocks = (a.tokens + 3) / 4, pieces = (a.n + 64 * Num<T>::E - 1) / (64 * Num<T>::E);
+template <class T, class X, int F, bool UNIT> int32_t combine_as(const CombineArgs& a, hipStream_t st) {
+    const int64_t blocks = (a.tokens + 3) / 4, pieces = (a.n + 64 * Num<X>::E - 1) / (64 * Num<X>::E);
     // few tokens: their columns are dealt to several blocks, so that more waves wait for memory
     const int64_t split = blocks >= 512 ? 1 : pieces < 512 / blocks ? pieces : 512 / blocks;
     TFH_LAUNCH_NAMED(name_of<T>("(combine_kernel<bf16>)", "(combine_kernel<f16>)", "(combine_kernel<float>)", "(combine_kernel<double>)"),
-                     (combine_kernel<T, F, UNIT>), dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
+                     (combine_kernel<T, X, F, UNIT>), dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
     return hip_check(hipGetLastError(), "combine launch");
 }
 template <class T, int F, bool UNIT> int32_t combine_grad_as(const CombineArgs& a, hipStream_t st) {
@@ -176,10 +176,14 @@ template <class T, int F, bool UNIT> int32_t combine_grad_as(const CombineArgs& 
                      (combine_grad_kernel<T, F, UNIT>), dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
     return hip_check(hipGetLastError(), "combine gradient launch");
 }
+template <class T, class X> int32_t combine_from(const CombineArgs& a, hipStream_t st) {
+    const bool unit = a.x_n == 1 && a.y_n == 1 && a.n >= Num<X>::E;
+    if (!unit) return combine_as<T, X, 4, false>(a, st);
+    return a.fan <= 2 ? combine_as<T, X, 2, true>(a, st) : a.fan <= 4 ? combine_as<T, X, 4, true>(a, st) : combine_as<T, X, 8, true>(a, st);
+}
 template <class T> int32_t combine_of(const CombineArgs& a, hipStream_t st) {
-    const bool unit = a.x_n == 1 && a.y_n == 1 && a.n >= Num<T>::E;
-    if (!unit) return combine_as<T, 4, false>(a, st);
-    return a.fan <= 2 ? combine_as<T, 2, true>(a, st) : a.fan <= 4 ? combine_as<T, 4, true>(a, st) : combine_as<T, 8, true>(a, st);
+    if (a.x_wide) return combine_from<T, typename Num<T>::acc>(a, st);
+    return combine_from<T, T>(a, st);
 }
 template <class T> int32_t combine_grad_of(const CombineArgs& a, hipStream_t st) {
     const bool unit = (!a.dw || a.x_n == 1) && a.y_n == 1 && (!a.dx || a.dx_n == 1) && a.n >= Num<T>::E;

@@ -79,6 +79,8 @@ int32_t product(int32_t dtype, int kind, const Args& a, void* stream) {
     return e;
 }
 
+int64_t wide_row(int64_t n) { return (n + 3) & ~(int64_t)3; }   // of the sums' type in scratch: 16-byte aligned
+
 Args base_args(const tfh_row_groups& g) {
     Args a = {};
     a.offsets = g.offsets;
@@ -156,6 +158,57 @@ int32_t ragged_gemm_grad(int32_t dtype, const tfh_row_groups* g, int32_t flags, 
     return product(dtype, PRODUCT_OUTER, p, stream);
 }
 
+// The gradient of the product's A.  Where several places read a row, their parts are kept in the sums' type and rounded once, as
+// they are joined: a part may lie beyond the operands' range, or cancel against another, and the row's sum not.
+size_t grad_a_bytes(int32_t dtype, int64_t n_rows, int64_t k, int32_t fan, int32_t flags) {
+    return (flags & TFH_ROWS_GATHER_A) && fan > 1 ? (size_t)n_rows * wide_row(k) * sums_size(dtype) : 0;
+}
+int32_t ragged_gemm_grad_a(int32_t dtype, const tfh_row_groups* g, int32_t flags, double alpha, const tfh_view* dc, const tfh_view* b,
+                           const tfh_view* da, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int32_t e = check_dtype(dtype)) return e;
+    if (flags & ~TFH_ROWS_GATHER_A) return set_error(TFH_ERR_INVALID_ARGUMENT, "unknown flags %d", flags);
+    const bool gather = flags & TFH_ROWS_GATHER_A, joined = gather && g && g->fan > 1;
+    if (int32_t e = check_groups(g, joined)) return e;
+    if (gather && !g->order && g->n_rows) return set_error(TFH_ERR_INVALID_ARGUMENT, "rows are gathered by an order, and there is none");
+    if (int32_t e = rank_of("dC", dc, 2)) return e;
+    if (int32_t e = rank_of("B", b, 3)) return e;
+    const int64_t K = b->dims[1], N = dc->dims[1], sources = gather ? g->n_rows / g->fan : g->n_rows;
+    if (int32_t e = check_extent("K", K)) return e;
+    if (int32_t e = check_extent("N", N)) return e;
+    if (int32_t e = check_view("dC", dc, {g->n_rows, N}, false)) return e;
+    if (int32_t e = check_view("B", b, {g->n_groups, K, N}, false)) return e;
+    if (int32_t e = check_view("dA", da, {sources, K}, true)) return e;
+    if (int32_t e = check_workspace(workspace, workspace_bytes, grad_a_bytes(dtype, g->n_rows, K, g->fan, flags))) return e;
+    if (g->n_rows == 0 || K == 0) return TFH_OK;
+    Args p = base_args(*g);
+    set_a(p, dtype, *dc);
+    p.B = view_ptr(*b, dtype);
+    p.b_group = b->strides[0], p.b_k = b->strides[2], p.b_n = b->strides[1];
+    p.N = (int32_t)K, p.K = (int32_t)N;
+    p.alpha = alpha;
+    p.zero_rest = 1;
+    if (joined) {
+        p.C = workspace, p.c_row = wide_row(K), p.c_n = 1;
+        p.wide = 1;
+    } else {
+        p.C = view_ptr(*da, dtype), p.c_row = da->strides[0], p.c_n = da->strides[1];
+        p.scatter = gather;
+    }
+    if (int32_t e = product(dtype, PRODUCT_ROWS, p, stream)) return e;
+    if (!joined) return TFH_OK;
+    CombineArgs c = {};
+    c.x = workspace, c.x_row = wide_row(K), c.x_n = 1;
+    c.x_wide = 1;
+    c.y = view_ptr(*da, dtype), c.y_row = da->strides[0], c.y_n = da->strides[1];
+    c.positions = g->positions, c.offsets = g->offsets;
+    c.n_rows = g->n_rows, c.tokens = sources;
+    c.n_groups = g->n_groups, c.fan = g->fan, c.n = (int32_t)K;
+    const int prof = prof_begin(PROF_REDUCE, stream);
+    const int32_t e = launch_combine(dtype, c, stream);
+    prof_end(prof, stream);
+    return e;
+}
+
 int32_t combine(int32_t dtype, const tfh_row_groups* g, const tfh_view* x, const tfh_view* w, const tfh_view* y, const tfh_view* dx,
                 const tfh_view* dw, bool gradient, void* stream) {
     if (int32_t e = check_dtype(dtype)) return e;
@@ -192,7 +245,6 @@ int32_t combine(int32_t dtype, const tfh_row_groups* g, const tfh_view* x, const
 
 // The middle product X . A of the adapters, in scratch: rows in the sums' type, 16-byte aligned, or a pair of the operands'
 // type with a power of two per row (f16).
-int64_t wide_row(int64_t rank) { return (rank + 3) & ~(int64_t)3; }
 int64_t pair_pad(int64_t rank) { return (rank + 31) & ~(int64_t)31; }
 size_t middle_bytes(int32_t dtype, int64_t n_rows, int64_t rank) {
     if (rank == 0) return 0;
@@ -411,6 +463,15 @@ int32_t tfh_ragged_gemm(int32_t dtype, const tfh_row_groups* groups, int32_t fla
 int32_t tfh_ragged_gemm_grad(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* a,
                              const tfh_view* dc, double beta, const tfh_view* db, tfh_stream stream) {
     return ragged::guarded("tfh_ragged_gemm_grad", [&] { return ragged::ragged_gemm_grad(dtype, groups, flags, alpha, a, dc, beta, db, stream); });
+}
+size_t tfh_ragged_gemm_grad_a_workspace(int32_t dtype, int64_t n_rows, int64_t k, int32_t fan, int32_t flags) {
+    return !ragged::known(dtype) || n_rows < 0 || k < 0 || n_rows > ragged::MOST || k > ragged::MOST ? 0 : ragged::grad_a_bytes(dtype, n_rows, k, fan, flags);
+}
+int32_t tfh_ragged_gemm_grad_a(int32_t dtype, const tfh_row_groups* groups, int32_t flags, double alpha, const tfh_view* dc,
+                               const tfh_view* b, const tfh_view* da, void* workspace, size_t workspace_bytes, tfh_stream stream) {
+    return ragged::guarded("tfh_ragged_gemm_grad_a", [&] {
+        return ragged::ragged_gemm_grad_a(dtype, groups, flags, alpha, dc, b, da, workspace, workspace_bytes, stream);
+    });
 }
 int32_t tfh_combine_rows(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* weights, const tfh_view* y,
                          tfh_stream stream) {

@@ -94,6 +94,7 @@ struct Args {
     int32_t scatter;          // C's row of p is order[p], else p
     int32_t zero_rest;        // rows: the rows behind the last group are written as zeros, else left alone
     int32_t use_beta;
+    int32_t wide;             // rows: C is of the sums' type (parts that are added up before they are rounded); no beta, no scatter
     double alpha, beta;
     // shared: the low-rank part, V[p, 0 .. r) against E[g, j, n]; rows of no group are without it.  V is of the sums' type, or
     // (pad > 0) a pair of the operands' type: row p is hi[0 .. pad), lo[0 .. pad), V = up[p] (hi + lo), zeros from r on

@@ -27,6 +27,7 @@ int32_t launch_group_rows(GroupArgs a, void* stream);
 struct CombineArgs {
     const void* x;            // [n_rows, n] rows in order
     int64_t x_row, x_n;
+    int32_t x_wide;           // x is of the sums' type (no gradient)
     const void* w;            // [tokens, fan], of the sums' type, or null (ones)
     int64_t w_token, w_fan;
     void* y;                  // [tokens, n]; the gradient's: dy

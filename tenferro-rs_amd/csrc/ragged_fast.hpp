@@ -438,6 +438,32 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
         }
         return;
     }
+    if constexpr (MODE == ROWS)
+        if (a.wide) {
+            // f32 results, 32 WM rows at a time through LDS as in the pair's case
+            static_assert(32 * S::WM * TN * 4 <= S::LDS, "a pass's results fit the stages");
+            constexpr int CHUNKS_W = TN / 4;
+#pragma unroll
+            for (int x = 0; x < XT; ++x) {
+                __syncthreads();
+                const int r = wm * 32 + (lane & 31);
+#pragma unroll
+                for (int y = 0; y < YT; ++y)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int chunk = (wn * YT + y) * 8 + 2 * g + (lane >> 5);
+                        const f32x4 v = {alpha * acc[x][y][4 * g], alpha * acc[x][y][4 * g + 1], alpha * acc[x][y][4 * g + 2], alpha * acc[x][y][4 * g + 3]};
+                        *(f32x4*)(lds + r * (TN * 4) + ((chunk ^ (r & 15)) << 4)) = v;
+                    }
+                __syncthreads();
+                for (int id = tid; id < 32 * S::WM * CHUNKS_W; id += 256) {
+                    const int s = id / CHUNKS_W, chunk = id % CHUNKS_W, row = ((s >> 5) * XT + x) * 32 + (s & 31), n = n0 + 4 * chunk;
+                    if (row >= t.rows || n >= a.N) continue;
+                    *(f32x4*)((float*)a.C + (t.first + row) * a.c_row + n) = *(const f32x4*)(lds + s * (TN * 4) + ((chunk ^ (s & 15)) << 4));
+                }
+            }
+            return;
+        }
     if (a.use_beta && real) {   // the sum is rounded once: nothing in between
 #pragma unroll
         for (int x = 0; x < XT; ++x) {
@@ -542,7 +568,7 @@ inline bool fast_rows(const void* p, int64_t rows, int64_t stride, int64_t inner
 }
 template <int MODE> inline bool fast_takes(const Args& a, bool bkfast) {
     if (MODE == PAIR) return a.pad > 0 && a.pad <= 64 && !a.use_beta && fast_rows(a.A, a.a_rows, a.a_row, a.a_col, a.M) && fast_rows(a.B, a.b_rows, a.b_k, a.b_n, 2 * a.pad);
-    if (a.c_n != 1 || a.c_row % 4 || a.N % 4 || !aligned(a.C, 8)) return false;
+    if (a.c_n != 1 || a.c_row % 4 || a.N % 4 || !aligned(a.C, a.wide ? 16 : 8)) return false;
     if (MODE == OUTER) {
         if (a.c_group % 4) return false;
         return fast_rows(a.A, a.a_rows, a.a_row, a.a_col, a.M) && fast_rows(a.B, a.b_rows, a.b_k, a.b_n, a.N);

@@ -164,6 +164,10 @@ __global__ __launch_bounds__((few_threads<MODE>()), 1) void ragged_few_kernel(co
             row = a.order[row];
             if (row < 0 || row >= a.n_rows) continue;
         }
+        if (MODE == ROWS && a.wide) {
+            ((float*)a.C)[row * a.c_row + (n0 + n) * a.c_n] = real ? v : 0.0f;
+            continue;
+        }
         T* const c = (T*)a.C + row * a.c_row + (n0 + n) * a.c_n;
         if (a.use_beta && real) v += beta * (float)*c;
         *c = (T)(real ? v : 0.0f);

@@ -191,7 +191,9 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         }
     }
     switch (kind) {
-        case PRODUCT_ROWS: return columns ? launch_general<T, T, T, T, ROWS, false>(a, stream) : launch_general<T, T, T, T, ROWS, true>(a, stream);
+        case PRODUCT_ROWS:
+            if (a.wide) return columns ? launch_general<T, T, T, W, ROWS, false>(a, stream) : launch_general<T, T, T, W, ROWS, true>(a, stream);
+            return columns ? launch_general<T, T, T, T, ROWS, false>(a, stream) : launch_general<T, T, T, T, ROWS, true>(a, stream);
         case PRODUCT_MIDDLE: return columns ? launch_general<T, T, T, W, ROWS, false>(a, stream) : launch_general<T, T, T, W, ROWS, true>(a, stream);
         case PRODUCT_SHARED: return columns ? launch_general<T, T, T, T, SHARED, false>(a, stream) : launch_general<T, T, T, T, SHARED, true>(a, stream);
         case PRODUCT_OUTER: return launch_general<T, T, T, T, OUTER, false>(a, stream);

@@ -298,24 +298,18 @@ def ragged_gemm_grad_into(a, dc, groups, alpha, beta, db, gather=False, stream=N
 
 def ragged_gemm_backward(a, b, dc, groups, gather=False, stream=None):
     """The gradients of ragged_gemm(a, b, groups, gather): (da, db), db laid out like b.  With gather a row's choices are
-    added up (positions are needed); each choice's part is rounded to the operands' type before, the sum in 32 bits."""
+    added up in 32 bits (64 for f64) and rounded once; for a fan above 1 positions are needed."""
     _groups(groups)
     _rank("a", a, 2), _rank("b", b, 3)
     if gather and groups.fan > 1:
         groups._need("positions")
     with _Call(a, (a, b, dc), groups, stream) as k:
-        K = _shape(b)[1]
-        bt = b.permute([0, 2, 1]) if isinstance(b, Tensor) else b.transpose(1, 2)
-        joined = gather and groups.fan > 1
-        da = k.empty((groups.n_rows, K))
-        flags = SCATTER_C if gather and not joined else 0
-        _check(lib().tfh_ragged_gemm(k.dtype, _groups(groups), flags | ZERO_REST, 1.0, _view(dc), _view(bt), 0.0, _view(da), k.stream))
-        if joined:
-            rows, da = da, k.empty((groups.n_rows // groups.fan, K))
-            _check(lib().tfh_combine_rows(k.dtype, _groups(groups), _view(rows), None, _view(da), k.stream))
-        db = k.empty(_shape(b), like=b)
-        _check(lib().tfh_ragged_gemm_grad(k.dtype, _groups(groups), GATHER_A if gather else 0, 1.0, _view(a), _view(dc), 0.0,
-                                          _view(db), k.stream))
+        K, flags = _shape(b)[1], GATHER_A if gather else 0
+        da, db = k.empty((groups.n_rows // groups.fan if gather else groups.n_rows, K)), k.empty(_shape(b), like=b)
+        need = lib().tfh_ragged_gemm_grad_a_workspace(k.dtype, groups.n_rows, K, groups.fan, flags)
+        ws = k.empty((need,), k.torch.uint8).data_ptr() if need else None
+        _check(lib().tfh_ragged_gemm_grad_a(k.dtype, _groups(groups), flags, 1.0, _view(dc), _view(b), _view(da), ws, need, k.stream))
+        _check(lib().tfh_ragged_gemm_grad(k.dtype, _groups(groups), flags, 1.0, _view(a), _view(dc), 0.0, _view(db), k.stream))
         da, db = k.result(da), k.result(db)
         k.done(da, db)
     return da, db

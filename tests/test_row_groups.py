@@ -898,3 +898,98 @@ def test_16_bit_types_are_refused_elsewhere(tf, call):
             refused(tf, L.tfh_fill(dt, (C.c_double * 2)(), view(tf, [4]), None), tf.InvalidArgument)
         else:
             refused(tf, L.tfh_conj(dt, view(tf, [4]), view(tf, [4]), None), tf.InvalidArgument)
+
+
+# ------------------------------------------------------------------------------------------------------ sums that are rounded once
+def rows_gradient_reference(torch, dc, b, offsets, order, fan):
+    """The gradient of the gathered rows in 64 bits and the sums of absolute values."""
+    D, B = dc.double(), b.double()
+    want, size = (torch.zeros(len(order) // fan, B.shape[1], dtype=torch.float64) for _ in range(2))
+    for g in range(len(offsets) - 1):
+        p = slice(offsets[g], offsets[g + 1])
+        s = torch.tensor([o // fan for o in order[p]], dtype=torch.long)
+        want.index_add_(0, s, D[p] @ B[g].t())
+        size.index_add_(0, s, D[p].abs() @ B[g].abs().t())
+    return want, size
+
+
+GRADIENT_SHAPES = [  # tokens, fan, groups, K, N: few rows, tiles of every size, k shared out, rows that start at any address
+    (1, 2, 2, 1, 1), (9, 3, 5, 33, 5), (24, 2, 4, 264, 128), (70, 8, 9, 65, 129), (300, 2, 3, 136, 72), (900, 3, 4, 2048, 264), (900, 3, 4, 4104, 128), (700, 2, 2, 2047, 135)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape", GRADIENT_SHAPES, ids=str)
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_the_gradient_of_gathered_rows_is_rounded_once(tf, torch, name, shape, how):
+    # no slack for a rounding of each choice's part: the sum of the parts in 32 bits, as any other
+    tokens, fan, groups, K, N = shape
+    rng = np.random.default_rng(tokens + K)
+    ids = choices(rng, tokens, fan, groups)
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    a, b, dc = tensor(torch, rng, (tokens, K), name), tensor(torch, rng, (groups, K, N), name, N ** -0.5), tensor(torch, rng, (tokens * fan, N), name)
+    want, size = rows_gradient_reference(torch, dc, b, offsets, order, fan)
+    da, _ = tf.ragged_gemm_backward(a.cuda(), layout(torch, b, how), dc.cuda(), made(tf, torch, ids, groups), gather=True)
+    close(da, want, size, N + fan, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,K,N", [(3, 5, 7), (20, 72, 64), (300, 136, 72), (1200, 2048, 264)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_parts_of_a_gradient_beyond_the_range_may_cancel(tf, torch, tokens, K, N, how):
+    # two choices of a token, of opposite sign: the parts are (N - 1) 2^22 and 2^11 more, beyond f16's largest, 65504, their sum is 2^11.
+    # All are whole multiples of 2^11 below 2^(11 + 24): exact in 32 bits, in any order.
+    big = 2.0 ** 11
+    ids = np.stack([np.arange(tokens) % 2, 1 - np.arange(tokens) % 2], 1)
+    b, dc = torch.full((2, K, N), big, dtype=torch.float16), torch.full((2 * tokens, N), big, dtype=torch.float16)
+    b[1], b[1, :, N - 1] = -big, 0
+    dc[:, N - 1] = 1
+    da, _ = tf.ragged_gemm_backward(torch.zeros(tokens, K, dtype=torch.float16, device="cuda"), layout(torch, b, how), dc.cuda(), made(tf, torch, ids, 2), gather=True)
+    assert torch.equal(da.cpu(), torch.full((tokens, K), big, dtype=torch.float16))
+
+
+@pytest.mark.gpu
+def test_the_rows_gradient_by_its_own_entry(tf, torch):
+    # alpha, strides of its operands and its result, rows of no group: zeros
+    rng = np.random.default_rng(21)
+    tokens, fan, groups, K, N = 60, 2, 3, 40, 24
+    ids = choices(rng, tokens, fan, groups, none=0.4)
+    offsets, order, _ = grouping(ids.reshape(-1), groups)
+    b, dc = tensor(torch, rng, (groups, K, N), "bfloat16"), tensor(torch, rng, (tokens * fan, N), "bfloat16")
+    g = made(tf, torch, ids, groups)
+    want, size = rows_gradient_reference(torch, dc, b, offsets, order, fan)
+    L, at = tf.lib(), lambda t: view(tf, list(t.shape), list(t.stride()), t.data_ptr())
+    need = L.tfh_ragged_gemm_grad_a_workspace(tf.BF16, tokens * fan, K, fan, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for how in ("columns", "rows", "pitch", "steps"):
+        out = layout(torch, torch.full((tokens, K), float("nan"), dtype=torch.bfloat16), how)
+        B, D = layout(torch, b, how), layout(torch, dc, how)
+        tf._check(L.tfh_ragged_gemm_grad_a(tf.BF16, C.byref(g._c), 1, -0.5, at(D), at(B), at(out), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+        close(out, -0.5 * want, 0.5 * size, N + fan, "bfloat16")
+        gone = torch.from_numpy(((ids < 0) | (ids >= groups)).all(1))
+        assert gone.any() and not out.cpu()[gone].any()
+
+
+def test_the_rows_gradient_refuses_what_does_not_fit(tf):
+    L, V, G = tf.lib(), lambda *d, **k: view(tf, d, **k), lambda **k: row_groups(tf, **dict(dict(fan=2), **k))
+
+    def run(dt=4, g=None, fl=1, dc=None, b=None, da=None, ws=4096, nb=1 << 20):
+        return L.tfh_ragged_gemm_grad_a(dt, g or G(), fl, 1.0, dc or V(8, 24), b or V(3, 16, 24), da or V(4, 16), ws, nb, None)
+
+    refused(tf, run(dt=3), tf.InvalidArgument)
+    refused(tf, run(fl=2), tf.InvalidArgument)
+    refused(tf, run(g=G(order=None)), tf.InvalidArgument)
+    refused(tf, run(g=G(positions=None)), tf.InvalidArgument)
+    refused(tf, L.tfh_ragged_gemm_grad_a(4, None, 1, 1.0, V(8, 24), V(3, 16, 24), V(4, 16), 4096, 1 << 20, None), tf.InvalidArgument)
+    refused(tf, run(dc=V(7, 24)), tf.ShapeMismatch)
+    refused(tf, run(dc=V(8, 24, 1)), tf.RankMismatch)
+    refused(tf, run(b=V(3, 16, 25)), tf.ShapeMismatch)
+    refused(tf, run(da=V(8, 16)), tf.ShapeMismatch)
+    refused(tf, run(fl=0), tf.ShapeMismatch)
+    refused(tf, run(da=V(4, 16, strides=[0, 1])), tf.InvalidArgument)
+    refused(tf, run(ws=None), tf.InvalidArgument)
+    refused(tf, run(ws=4104), tf.InvalidArgument)
+    need = L.tfh_ragged_gemm_grad_a_workspace(4, 8, 16, 2, 1)
+    assert need == 8 * 16 * 4
+    refused(tf, run(nb=need - 1), tf.InvalidArgument)
+    assert L.tfh_ragged_gemm_grad_a_workspace(4, 8, 16, 2, 0) == 0 and L.tfh_ragged_gemm_grad_a_workspace(4, 8, 16, 1, 1) == 0
