@@ -68,6 +68,17 @@ template <class T> __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32
     if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+// A fragment with zeros for infinities and what is no number: what the lower half of a pair is multiplied by.  The upper half has met
+// them already, and the lower one, a zero or of the other sign, would make no number of that infinity.
+template <class T> __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
+    constexpr uint32_t EXPONENT = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t low = (v[i] & EXPONENT) == EXPONENT ? 0 : v[i] & 0xffff;
+        v[i] = (v[i] & EXPONENT << 16) == EXPONENT << 16 ? low : (v[i] & 0xffff0000) | low;
+    }
+    return v;
+}
 // A k-fast tile with KB = 64 or 128 bytes of k for each row: where a chunk lies, so that any eight consecutive rows' same
 // chunk fills the banks once.
 template <int KB> __device__ __forceinline__ uint32_t turn(uint32_t row) { return KB == 128 ? row & 7 : (row >> 1) & 3; }
@@ -283,7 +294,10 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
                 for (int h = 0; h < H; ++h) {
                     u32x4 eb[YT];
 #pragma unroll
-                    for (int y = 0; y < YT; ++y) eb[y] = fragment32<T, TN, BKFAST, KB>(lds + BASE_B, (wn * YT + y) * 32, h, lane);
+                    for (int y = 0; y < YT; ++y) {
+                        eb[y] = fragment32<T, TN, BKFAST, KB>(lds + BASE_B, (wn * YT + y) * 32, h, lane);
+                        if (k0 + 16 * h >= a.pad) eb[y] = finite_only<T>(eb[y]);
+                    }
 #pragma unroll
                     for (int x = 0; x < XT; ++x) {
                         const int r0 = (wm * XT + x) * 32, r = r0 + (lane & 31);
@@ -399,7 +413,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     // touch 32 rows with 16 bytes each.)
     const float alpha = (float)a.alpha * (MODE == ROWS && a.scales && real ? ((const float*)a.scales)[t.group] : 1.0f), beta = (float)a.beta;
     if constexpr (MODE == PAIR) {
-        // B's columns are a pair, hi and lo `pad` apart: their sums are added here, in f32
+        // B's columns are a pair, hi and lo `pad` apart: their sums are added here, in f32, unless an infinity of A's is in them (finite_only)
         static_assert(TM * TN * 4 <= S::LDS && TN % 64 == 0, "the sums fit the two stages");
         __syncthreads();
 #pragma unroll
@@ -427,7 +441,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
             T* const out = (T*)a.C + t.group * a.c_group + (m0 + r) * a.c_row + c * a.c_n;
             T v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (T)(alpha * (hi[i] + lo[i]));
+            for (int i = 0; i < 4; ++i) v[i] = (T)(alpha * (__builtin_isfinite(hi[i]) ? hi[i] + lo[i] : hi[i]));
             if (across && c + 4 <= a.r) {
                 __builtin_memcpy(out, v, 8);
             } else {

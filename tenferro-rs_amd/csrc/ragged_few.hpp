@@ -111,18 +111,19 @@ __global__ __launch_bounds__((few_threads<MODE>()), 1) void ragged_few_kernel(co
             int turn = 0, mine = 0, froms[AT_ONCE], tos[AT_ONCE];
             u32x4 factor[AT_ONCE];
             auto multiply = [&](int count) {
-#pragma unroll
-                for (int c = 0; c < AT_ONCE; ++c) {
-                    if (c >= count) break;
+                unrolled<AT_ONCE>([&](auto item) {
+                    constexpr int c = decltype(item)::value;
+                    if (c >= count) return;
+                    const u32x4 lower = finite_only<T>(factor[c]);
 #pragma unroll
                     for (int x = 0; x < TR; ++x) {
                         const int r = x * 16 + j;
                         if (tos[c] <= x * 16 || froms[c] >= x * 16 + 16) continue;
-                        const f32x4 sum = NT::mma(factor[c], lo[x], NT::mma(factor[c], hi[x], acc[x]));
+                        const f32x4 sum = NT::mma(lower, lo[x], NT::mma(factor[c], hi[x], acc[x]));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[x][i] = r >= froms[c] && r < tos[c] ? sum[i] : acc[x][i];
                     }
-                }
+                });
             };
             each_group(a, t.first, t.first + t.rows - 1, [&](int g, int f, int e) {
                 if (turn++ % LOW != wave - FEW_WAVES) return;

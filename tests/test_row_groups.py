@@ -993,3 +993,63 @@ def test_the_rows_gradient_refuses_what_does_not_fit(tf):
     assert need == 8 * 16 * 4
     refused(tf, run(nb=need - 1), tf.InvalidArgument)
     assert L.tfh_ragged_gemm_grad_a_workspace(4, 8, 16, 2, 0) == 0 and L.tfh_ragged_gemm_grad_a_workspace(4, 8, 16, 1, 1) == 0
+
+
+# ------------------------------------------------------------------------------------------------------ infinities of the adapters' operands
+def agree(got, want, size, k, name, extra):
+    """As close(), with infinities and what is no number in the same places."""
+    got, want = got.double().cpu(), want.double()
+    fine = want.isfinite()
+    assert torch_equal(got.isnan(), want.isnan()) and torch_equal(got[~fine & ~want.isnan()], want[~fine & ~want.isnan()])
+    close(got[fine], want[fine], size[fine], k, name, extra[fine])
+
+
+def torch_equal(a, b):
+    return a.shape == b.shape and bool((a == b).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,K,N,R", [(9, 64, 48, 8), (60, 136, 264, 16), (700, 192, 264, 64), (1500, 520, 1032, 24), (300, 71, 101, 7)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_infinities_of_adapters_stay_infinities(tf, torch, name, rows, K, N, R, how):
+    # everything positive: an infinite factor gives that infinity in its column, whatever the middle's lower bits are
+    rng = np.random.default_rng(rows)
+    ids = rng.integers(-1, 3, rows)
+    ids[:3] = [0, 1, 2]
+    pos = lambda shape, scale=1.0: (tensor(torch, rng, shape, "float64").abs() * scale + 2.0 ** -6).to(getattr(torch, name))
+    x, w, dy = pos((rows, K)), pos((K, N), K ** -0.5), pos((rows, N))
+    a, b = pos((3, K, R), K ** -0.5), pos((3, R, N), R ** -0.5)
+    inf = float("inf")
+    bi = b.clone()
+    bi[0, R - 1, 3], bi[1, 0, N - 2], bi[2, R // 2, 7] = inf, -inf, inf
+    g = made(tf, torch, ids, 3)
+    on = lambda *ts: [layout(torch, t, how) for t in ts]
+
+    def plain(x, w, a, b):
+        X, W, A, B = (t.double() for t in (x, w, a, b))
+        y, size = X @ W, X @ W
+        low = torch.zeros_like(y)
+        for i in range(3):
+            t = torch.from_numpy(np.nonzero(ids == i)[0])
+            part = X[t] @ A[i] @ B[i]
+            y[t] += part
+            low[t] = part.abs()
+        return y, size + low, low
+
+    want, size, low = plain(x, w, a, bi)
+    assert want.isinf().any() and not want.isnan().any()
+    agree(tf.adapter_gemm(x.cuda(), *on(w, a, bi), g), want, size, K + R, name, MIDDLE[name] * low)
+    # gradients: one infinite entry of x, one of dy, in rows of two groups
+    xi, di = x.clone(), dy.clone()
+    xi[0, 5], di[1, 6] = inf, inf
+    dx, da, db = tf.adapter_gemm_backward(xi.cuda(), *on(w, a, b), di.cuda(), g)
+    want, size, low = plain(di, w.t(), b.transpose(1, 2), a.transpose(1, 2))
+    agree(dx, want, size, N + R, name, MIDDLE[name] * low)
+    X, D, A, B = (t.double() for t in (xi, di, a, b))
+    for i in range(3):
+        t = torch.from_numpy(np.nonzero(ids == i)[0])
+        want = X[t].t() @ (D[t] @ B[i].t())
+        agree(da[i], want, want, len(t) + N, name, MIDDLE[name] * want)
+        want = (X[t] @ A[i]).t() @ D[t]
+        agree(db[i], want, want, len(t) + K, name, MIDDLE[name] * want)
