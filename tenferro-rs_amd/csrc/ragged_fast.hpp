@@ -45,15 +45,12 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
 constexpr uint32_t NOWHERE = 0xfffffff0u;   // an offset beyond every buffer (spans are under MOST_SPAN)
 constexpr int64_t MOST_SPAN = 0xffff0000ll;
 
-// 16 bytes a lane from buffer + offset + scalar into LDS at `to` + 16 * lane.  The compiler does not count these loads:
-// wait_loads() does, before anything they write is read.
-__device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t scalar, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(buffer), "s"(scalar) : "memory");
-}
-// The same in two parts, with one instruction at least in between: where the chunk goes, and the load.
-template <int AT> __device__ __forceinline__ void load_goes_to(uint32_t base) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(base), "n"(AT) : "memory", "scc"); }
-__device__ __forceinline__ void load_there(u32x4 buffer, uint32_t offset, uint32_t scalar) {
-    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(offset), "s"(buffer), "s"(scalar) : "memory");
+// 16 bytes a lane from buffer + offset + scalar into LDS at `to` + AT + 16 * lane.  The compiler does not count these loads:
+// wait_loads() does, before anything they write is read.  Where a load goes is in m0, which is written and read within one
+// statement.  (The compiler reserves that register: it writes it for its own instructions that read it only, of which LDS accesses and
+// products are none.)
+template <int AT = 0> __device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t offset, uint32_t scalar, uint32_t to) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(to), "n"(AT), "v"(offset), "s"(buffer), "s"(scalar) : "memory", "scc");
 }
 template <class F, int... I> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
 template <int N, class F> __device__ __forceinline__ void unrolled(F f) { each_of(std::make_integer_sequence<int, N>{}, f); }
@@ -332,12 +329,10 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     }
     if (stages > 0) {
         // Between two barriers lie H M products, and the loads of a stage of each operand into the slots that the first of them
-        // frees: item c, chunk item_i of operand item_a, beside product place(c).  Evenly, because loads in a row wait for one
+        // frees: item c beside product place(c).  Evenly, because loads in a row wait for one
         // another and hold the products up; with a slot less for the second operand, that one's first.
         constexpr int M = XT * YT;
         constexpr bool SKEW = SA > SB;
-        auto item_a = [](int c) { return SKEW ? c >= CB : c < CA; };
-        auto item_i = [](int c) { return SKEW ? (c >= CB ? c - CB : c) : c < CA ? c : c - CA; };
         auto place = [](int c) { return !SKEW ? c * H * M / CHUNKS : c < CB ? c * M / CB : M + (c - CB) * 2 * M / CA; };
         constexpr int FIRST = SKEW ? CB : (CHUNKS + H - 1) / H;   // items before the stage's end
         now.oa = now.ob = 0;
@@ -380,25 +375,14 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
 #pragma unroll
                     for (int i = m * FRAGS / M; i < (m + 1) * FRAGS / M; ++i)
                         read((h + 1) & 1, i, h == LAST ? next_a : at_a, h == LAST ? next_b : at_b, (h + 1) % H);
-                    bool first = true;
-                    unrolled<CHUNKS>([&](auto item) {
-                        constexpr int c = decltype(item)::value, to = (SKEW ? c >= CB ? c - CB : c : c < CA ? c : c - CA) * 4096;
-                        if (place(c) != from + m || !first) return;
-                        load_goes_to<to>(item_a(c) ? before_a : before_b);
-                        first = false;
-                    });
                     acc[m / YT][m % YT] = mma32<T>(fb[h & 1][m % YT], fa[h & 1][m / YT], acc[m / YT][m % YT]);
-                    first = true;
-                    unrolled<CHUNKS>([&](auto item) {
-                        constexpr int c = decltype(item)::value, to = (SKEW ? c >= CB ? c - CB : c : c < CA ? c : c - CA) * 4096;
+                    unrolled<CHUNKS>([&](auto item) {   // item c: chunk i of the first operand, or of the second
+                        constexpr int c = decltype(item)::value;
+                        constexpr bool first = SKEW ? c >= CB : c < CA;
+                        constexpr int i = SKEW ? (c >= CB ? c - CB : c) : c < CA ? c : c - CA;
                         if (place(c) != from + m) return;
-                        if (!first) {   // (more than one beside a product, in small tiles)
-                            load_goes_to<to>(item_a(c) ? before_a : before_b);
-                            asm volatile("s_nop 0" ::: "memory");
-                        }
-                        first = false;
-                        if (item_a(c)) load_there(now.A, now.va[item_i(c)], now.oa);
-                        else load_there(now.B, now.vb[item_i(c)], now.ob);
+                        if constexpr (first) load_to_lds<i * 4096>(now.A, now.va[i], now.oa, before_a);
+                        else load_to_lds<i * 4096>(now.B, now.vb[i], now.ob, before_b);
                     });
                     __builtin_amdgcn_sched_barrier(0);
                 }

@@ -1053,3 +1053,20 @@ def test_infinities_of_adapters_stay_infinities(tf, torch, name, rows, K, N, R, 
         agree(da[i], want, want, len(t) + N, name, MIDDLE[name] * want)
         want = (X[t] @ A[i]).t() @ D[t]
         agree(db[i], want, want, len(t) + K, name, MIDDLE[name] * want)
+
+
+# ------------------------------------------------------------------------------------------------------ what the sources have to keep to (no GPU)
+def test_a_load_into_lds_writes_its_target_register_in_the_same_statement():
+    # m0 says where the load goes: left to another statement, an instruction of the compiler's in between could change it
+    import glob
+    import re
+    found = 0
+    for path in glob.glob(os.path.join(ROOT, "tenferro-rs_amd", "csrc", "*.h*")):
+        for text in re.findall(r"asm(?:\s+volatile)?\s*\((.*?)\);", open(path).read(), flags=re.S):
+            code = " ".join(re.findall(r'"((?:[^"\\]|\\.)*)"', text.split("::")[0]))
+            if re.search(r"buffer_load\w*.*\blds\b", code):
+                found += 1
+                assert re.search(r"\bm0\b.*buffer_load", code), (path, code)
+            elif re.search(r"\bm0\b", code):
+                raise AssertionError((path, code))
+    assert found
