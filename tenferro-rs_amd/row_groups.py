@@ -15,7 +15,7 @@ import ctypes as C
 import struct
 
 from . import (BF16, F16, F32, F64, CompletionEvent, CrossMemorySpaceOperation, GpuMemory, InvalidArgument,
-               NoCompatibleComputeDevice, RankMismatch, Tensor, _check, _in_flight, lib, tfh_view)
+               NoCompatibleComputeDevice, RankMismatch, ShapeMismatch, Tensor, _check, _in_flight, lib, tfh_view)
 
 GATHER_A, SCATTER_C, ZERO_REST = 1, 2, 4      # TFH_ROWS_*
 
@@ -79,6 +79,12 @@ def _shape(t):
     return t._dims if isinstance(t, Tensor) else t.shape
 
 
+def _hold(event, tensors):
+    """Keeps the tensors' buffers until the event is done, and lets go of those whose event is."""
+    _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
+    _in_flight.append((event, [getattr(t, "_buf", t) for t in tensors]))
+
+
 class _Call:
     """What every call does around its launches: one device for all operands, one element type, the stream and the
     events of Tensors, and buffers kept alive while another stream than torch's uses them."""
@@ -123,8 +129,12 @@ class _Call:
         return self
 
     def __exit__(self, *error):
-        if self.guard is not None:
-            self.guard.__exit__(*error)
+        try:
+            if error[0] is not None and self.stream != self.current:
+                _hold(CompletionEvent(self.stream), self.used)   # an earlier launch of the call may be using them
+        finally:
+            if self.guard is not None:
+                self.guard.__exit__(*error)
 
     def empty(self, dims, dtype=None, like=None):
         """A new buffer from torch's allocator.  Its memory may still be read by earlier work of the current stream: another
@@ -161,8 +171,7 @@ class _Call:
                 if isinstance(t, (Tensor, RowGroups)):
                     t.event = ev
             if other:
-                _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
-                _in_flight.append((ev, [getattr(t, "_buf", t) for t in self.used + list(outputs)]))
+                _hold(ev, self.used + list(outputs))
 
 
 class RowGroups:
@@ -238,9 +247,9 @@ class RowGroups:
             g._c = tfh_row_groups(p + 4 * at_o, p, p + 4 * at_p, n, n_groups, g.fan)
             if st != current:
                 g.event = CompletionEvent(st)
-                _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
-                _in_flight.append((g.event, [buf, ids]))
         finally:
+            if st != current:
+                _hold(CompletionEvent(st), [buf, ids])
             if guard is not None:
                 guard.__exit__(None, None, None)
         return g
@@ -254,6 +263,15 @@ def _groups(groups):
     if not isinstance(groups, RowGroups):
         raise InvalidArgument("invalid argument: groups have to be RowGroups")
     return C.byref(groups._c)
+
+
+def _dims(t, dims):
+    """What a call of several launches asks of an operand, before the first of them."""
+    got = list(_shape(t))
+    if len(got) != len(dims):
+        raise RankMismatch(f"rank mismatch: expected {len(dims)}, got {len(got)}", len(dims), len(got))
+    if got != list(dims):
+        raise ShapeMismatch(f"shape mismatch: expected {list(dims)}, got {got}", list(dims), got)
 
 
 def _rank(what, t, rank):
@@ -300,7 +318,12 @@ def ragged_gemm_backward(a, b, dc, groups, gather=False, stream=None):
     """The gradients of ragged_gemm(a, b, groups, gather): (da, db), db laid out like b.  With gather a row's choices are
     added up in 32 bits (64 for f64) and rounded once; for a fan above 1 positions are needed."""
     _groups(groups)
-    _rank("a", a, 2), _rank("b", b, 3)
+    _rank("b", b, 3), _rank("dc", dc, 2)
+    _dims(a, (groups.n_rows // groups.fan if gather else groups.n_rows, _shape(b)[1]))
+    _dims(b, (groups.n_groups, _shape(b)[1], _shape(dc)[1]))
+    _dims(dc, (groups.n_rows, _shape(b)[2]))
+    if gather:
+        groups._need("order")
     if gather and groups.fan > 1:
         groups._need("positions")
     with _Call(a, (a, b, dc), groups, stream) as k:

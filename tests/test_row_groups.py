@@ -1070,3 +1070,50 @@ def test_a_load_into_lds_writes_its_target_register_in_the_same_statement():
             elif re.search(r"\bm0\b", code):
                 raise AssertionError((path, code))
     assert found
+
+
+# ------------------------------------------------------------------------------------------------------ calls that fail
+@pytest.mark.gpu
+def test_a_call_that_fails_on_another_stream_keeps_what_its_first_launch_uses(tf, torch, monkeypatch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 3)
+    groups = tf.RowGroups.from_ids(ids, up.shape[0])
+    dc = torch.randn(groups.n_rows, up.shape[2], device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for call in ("tfh_ragged_gemm_grad", "tfh_adapter_gemm_grad"):
+        before = len([e for e in tf._in_flight if not e[0].ready()])
+        with monkeypatch.context() as m:
+            m.setattr(tf.lib(), call, lambda *a: 2)
+            with pytest.raises(tf.Error):
+                if call == "tfh_ragged_gemm_grad":
+                    tf.ragged_gemm_backward(x, up, dc, groups, gather=True, stream=side.cuda_stream)
+                else:
+                    flat = tf.RowGroups.from_ids(ids[:, 0], up.shape[0])
+                    low_a, low_b = up[:, :, :8].contiguous(), up[:, :8, :].contiguous()
+                    tf.adapter_gemm_backward(x, up[0].contiguous(), low_a, low_b, dc[:x.shape[0]].contiguous(), flat, stream=side.cuda_stream)
+        held = tf._in_flight[-1][1]
+        assert len(tf._in_flight) > before and any(t is x for t in held) and any(t is up for t in held) == (call == "tfh_ragged_gemm_grad")
+        assert len([t for t in held if isinstance(t, torch.Tensor)]) >= 5      # operands, results and scratch
+    side.synchronize()
+    a = tf.ragged_gemm(x, up, groups, gather=True, stream=side.cuda_stream)     # and lets go of them
+    torch.cuda.synchronize()
+    assert len(tf._in_flight) <= 1 and torch.equal(a, tf.ragged_gemm(x, up, groups, gather=True))
+
+
+@pytest.mark.gpu
+def test_a_gradient_of_several_launches_looks_at_all_operands_first(tf, torch, monkeypatch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 3)
+    groups = tf.RowGroups.from_ids(ids, up.shape[0])
+    dc = torch.zeros(groups.n_rows, up.shape[2], device="cuda")
+    for name in ("tfh_ragged_gemm", "tfh_ragged_gemm_grad", "tfh_ragged_gemm_grad_a"):
+        monkeypatch.setattr(tf.lib(), name, None)                               # nothing may be launched
+    run = lambda a=x, b=up, d=dc, **k: tf.ragged_gemm_backward(a, b, d, groups, **dict(dict(gather=True), **k))
+    for bad in (dict(a=x[1:]), dict(a=x[:, 1:]), dict(d=dc[1:]), dict(d=dc[:, 1:]), dict(b=up[1:]), dict(b=up[:, 1:]), dict(b=up[:, :, 1:]), dict(gather=False)):
+        with pytest.raises(tf.ShapeMismatch):
+            run(**bad)
+    for bad in (dict(a=x[0]), dict(b=up[0]), dict(d=dc[0])):
+        with pytest.raises(tf.RankMismatch):
+            run(**bad)
+    none = tf.RowGroups(groups.offsets, n_rows=groups.n_rows, fan=1)
+    with pytest.raises(tf.InvalidArgument):
+        tf.ragged_gemm_backward(torch.zeros(groups.n_rows, x.shape[1], device="cuda"), up, dc, none, gather=True)
