@@ -8,8 +8,9 @@ reference; beside HipBackend.plan_grouped, whose groups' extents are fixed when 
 
 Operands are torch CUDA tensors or GpuMemory Tensors of bf16, f16, f32 or f64, with any strides; a result is of the
 first operand's kind.  Work is enqueued on `stream` (default: torch's current stream of the operands' device), never
-waited for, and allocates through torch only, so the calls can be captured into a graph.  On a stream other than the
-current one the caller orders the operands' earlier and the results' later use, as with any torch tensor.
+waited for, and allocates through torch only, so the calls can be captured into a graph: on the current stream, and behind
+no event from before the capture (when the graph runs is the caller's to order).  On a stream other than the current one the
+caller orders the operands' earlier and the results' later use, as with any torch tensor.
 """
 import ctypes as C
 import struct
@@ -79,6 +80,19 @@ def _shape(t):
     return t._dims if isinstance(t, Tensor) else t.shape
 
 
+def _capturing():
+    import torch
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _stream(stream, current):
+    if stream is None or stream == current:
+        return current
+    if _capturing():    # its events would have to be kept, and none asked, until the capture ends
+        raise InvalidArgument("invalid argument: while a graph is captured, calls go to the current stream: make that the other one")
+    return stream
+
+
 def _hold(event, tensors):
     """Keeps the tensors' buffers until the event is done, and lets go of those whose event is."""
     _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
@@ -114,7 +128,7 @@ class _Call:
                                                 GpuMemory(self.device), GpuMemory(groups.device))
             self.used.append(groups)
         self.current = _stream_of(self.device)
-        self.stream = self.current if stream is None else stream
+        self.stream = _stream(stream, self.current)
         self.guard = None
         if torch.cuda.current_device() != self.device:
             self.guard = torch.cuda.device(self.device)
@@ -123,8 +137,9 @@ class _Call:
     def __enter__(self):
         if self.guard is not None:
             self.guard.__enter__()
-        for t in self.used:
-            if isinstance(t, (Tensor, RowGroups)) and t.event is not None:
+        pending = [t for t in self.used if isinstance(t, (Tensor, RowGroups)) and t.event is not None]
+        if pending and not _capturing():
+            for t in pending:
                 _check(lib().tfh_stream_wait_event(self.stream, t.event._h))
         return self
 
@@ -163,13 +178,11 @@ class _Call:
 
     def done(self, *outputs):
         other = self.stream != self.current
-        if other or any(isinstance(t, (Tensor, RowGroups)) for t in outputs):
-            if not other and not any(isinstance(t, Tensor) for t in outputs):
-                return
-            ev = CompletionEvent(self.stream)
-            for t in outputs:
-                if isinstance(t, (Tensor, RowGroups)):
-                    t.event = ev
+        tensors = [t for t in outputs if isinstance(t, Tensor)]
+        if other or tensors:
+            ev = None if _capturing() else CompletionEvent(self.stream)
+            for t in tensors:
+                t.event = ev
             if other:
                 _hold(ev, self.used + list(outputs))
 
@@ -227,7 +240,7 @@ class RowGroups:
         fan = ids.shape[1] if ids.dim() == 2 else 1
         _CODES or _codes()
         current = _stream_of(device)
-        st = current if stream is None else stream
+        st = _stream(stream, current)
         need = lib().tfh_group_rows_workspace(n, n_groups)
         # one buffer for all: [order | positions | offsets | scratch], each 16-byte aligned
         at_p, at_o = (n + 3) & ~3, 2 * ((n + 3) & ~3)

@@ -1117,3 +1117,37 @@ def test_a_gradient_of_several_launches_looks_at_all_operands_first(tf, torch, m
     none = tf.RowGroups(groups.offsets, n_rows=groups.n_rows, fan=1)
     with pytest.raises(tf.InvalidArgument):
         tf.ragged_gemm_backward(torch.zeros(groups.n_rows, x.shape[1], device="cuda"), up, dc, none, gather=True)
+
+
+@pytest.mark.gpu
+def test_calls_on_a_side_stream_inside_a_capture_are_refused(tf, torch):
+    # before anything is enqueued, so that the capture goes on; groups and Tensors from before it, with events, are taken
+    x, up, down, ids, gates, dy = layer_inputs(torch, 12)
+    want, groups, h = expert_layer(tf, x, up, down, ids, gates)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    st, T = side.cuda_stream, tf.Tensor.from_torch
+    before = tf.RowGroups.from_ids(ids, up.shape[0], stream=st)
+    held = T(x.clone())
+    tf.ragged_gemm_into(T(x), T(up), before, 1.0, 0.0, T(torch.empty_like(h)), gather=True, stream=st)
+    held.event = before.event
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: tf.RowGroups.from_ids(ids, up.shape[0], stream=st), lambda: tf.ragged_gemm(x, up, groups, gather=True, stream=st),
+                     lambda: tf.combine_rows(h, groups, gates, stream=st)):
+            with pytest.raises(tf.InvalidArgument):
+                call()
+        made_here = tf.RowGroups.from_ids(ids, up.shape[0], stream=torch.cuda.current_stream().cuda_stream)
+        one = tf.ragged_gemm(x, up, before, gather=True)
+        other = tf.ragged_gemm(held, T(up), made_here, gather=True)
+        y = tf.combine_rows(tf.ragged_gemm(one, down, made_here), before, gates)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(one, h) and other.event is None
+        assert np.array_equal(other.to_numpy(), h.cpu().numpy())
+        z = tf.ragged_gemm(x, up, made_here, gather=True, stream=st)            # and outside, on the side stream
+        torch.cuda.synchronize()
+        assert torch.equal(z, h)
