@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
     typedef typename Num<T>::acc W;
     constexpr int E = Num<X>::E;
     const int lane = threadIdx.x & 63, step = 64 * E * gridDim.y;
-    const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.tokens) return;
     int p[F];
     W w[F];
@@ -94,20 +94,20 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
 }
 
 template <class T, int F, bool UNIT>
-__global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, int token_blocks) {
+__global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, int token_blocks, int rest_blocks) {
     typedef typename Num<T>::acc W;
     constexpr int E = Num<T>::E, STEP = 64 * E;
-    const int lane = threadIdx.x & 63;
-    if ((int)blockIdx.x >= token_blocks) {
+    const int lane = threadIdx.x & 63, block = (int)(blockIdx.z * gridDim.x + blockIdx.x);
+    if (block >= token_blocks) {
         // the rows behind the last group get zeros
-        if (!a.dx) return;
+        if (!a.dx || block >= token_blocks + rest_blocks) return;
         const T zero[E] = {};
         const int from = clamp_row(a.offsets[a.n_groups], a.n_rows);
-        for (int64_t p = from + ((int)blockIdx.x - token_blocks) * 4 + (threadIdx.x >> 6); p < a.n_rows; p += ((int)gridDim.x - token_blocks) * 4)
+        for (int64_t p = from + (block - token_blocks) * 4 + (threadIdx.x >> 6); p < a.n_rows; p += rest_blocks * 4)
             for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT, E>((T*)a.dx + p * a.dx_row, a.dx_n, n, a.n, zero);
         return;
     }
-    const int64_t t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = (int64_t)block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.tokens) return;
     for (int j0 = 0; j0 < a.fan; j0 += F) {
         W w[F], dot[F] = {};
@@ -166,14 +166,18 @@ template <class T, class X, int F, bool UNIT> int32_t combine_as(const CombineAr
     const int64_t blocks = (a.tokens + 3) / 4, pieces = (a.n + 64 * Num<X>::E - 1) / (64 * Num<X>::E);
     // few tokens: their columns are dealt to several blocks, so that more waves wait for memory
     const int64_t split = blocks >= 512 ? 1 : pieces < 512 / blocks ? pieces : 512 / blocks;
+    uint32_t x, z;
+    if (int32_t e = launch_grid(blocks, 256, &x, &z)) return e;
     TFH_LAUNCH_NAMED(name_of<T>("(combine_kernel<bf16>)", "(combine_kernel<f16>)", "(combine_kernel<float>)", "(combine_kernel<double>)"),
-                     (combine_kernel<T, X, F, UNIT>), dim3((unsigned)blocks, (unsigned)(split < 1 ? 1 : split)), dim3(256), 0, st, a);
+                     (combine_kernel<T, X, F, UNIT>), dim3(x, (unsigned)(split < 1 ? 1 : split), z), dim3(256), 0, st, a);
     return hip_check(hipGetLastError(), "combine launch");
 }
 template <class T, int F, bool UNIT> int32_t combine_grad_as(const CombineArgs& a, hipStream_t st) {
     const int64_t blocks = (a.tokens + 3) / 4, rest = a.n_rows < 256 ? (a.n_rows + 3) / 4 : 64;
+    uint32_t x, z;
+    if (int32_t e = launch_grid(blocks + rest, 256, &x, &z)) return e;
     TFH_LAUNCH_NAMED(name_of<T>("(combine_grad_kernel<bf16>)", "(combine_grad_kernel<f16>)", "(combine_grad_kernel<float>)", "(combine_grad_kernel<double>)"),
-                     (combine_grad_kernel<T, F, UNIT>), dim3((unsigned)(blocks + rest)), dim3(256), 0, st, a, (int)blocks);
+                     (combine_grad_kernel<T, F, UNIT>), dim3(x, 1, z), dim3(256), 0, st, a, (int)blocks, (int)rest);
     return hip_check(hipGetLastError(), "combine gradient launch");
 }
 template <class T, class X> int32_t combine_from(const CombineArgs& a, hipStream_t st) {

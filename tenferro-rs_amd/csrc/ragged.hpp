@@ -104,6 +104,7 @@ struct Args {
     int32_t r, pad;
     float* up;                // f16: the power of two by which row p was scaled down; null: 1 (written with V, read with it)
     const void* scales;       // rows: factors of the groups' results (of the accumulators' type) beside alpha, or null
+    uint32_t grid_x;          // the launch's blocks along x; the launcher sets it (a dimension has less than 2^32 threads)
 };
 
 enum Mode { ROWS = 0, OUTER = 1, SHARED = 2, PAIR = 3 };   // PAIR: outer with a pair of V's form for B (ragged_fast.hpp)
@@ -199,6 +200,7 @@ struct Tile {
     int group;   // n_groups: the rows behind the last group
     int first, rows, tile_m, tile_n;
 };
+__device__ __forceinline__ uint32_t block_of(const Args& a) { return blockIdx.y * a.grid_x + blockIdx.x; }
 // Tiles are dealt group by group; inside a group as tile_of() walks a matrix.  Every wave does this for itself: the
 // lanes take 64 groups at a time.  Returns false when the block has none.
 __device__ __forceinline__ bool find_tile(const Args& a, int tm, int tiles_n, uint32_t block, Tile& t) {
@@ -242,6 +244,17 @@ __device__ __forceinline__ bool find_tile(const Args& a, int tm, int tiles_n, ui
         want -= here;
     }
     return false;
+}
+// Shared: the rows' tiles, of whatever groups.
+__device__ __forceinline__ bool shared_tile(const Args& a, int tm, int tiles_n, uint32_t block, Tile& t) {
+    const int tiles_m = (int)((a.n_rows + tm - 1) / tm);
+    const uint32_t total = (uint32_t)tiles_m * (uint32_t)tiles_n;
+    if (block >= total) return false;
+    gemm::tile_of((uint32_t)gemm::logical_block(block, total), tiles_m, tiles_n, t.tile_m, t.tile_n);
+    t.group = 0;
+    t.first = t.tile_m * tm;
+    t.rows = a.n_rows - t.first < tm ? (int)(a.n_rows - t.first) : tm;
+    return true;
 }
 // Outer products: every group has as many tiles, but each takes as long as the group has rows.  They are dealt to the XCDs in
 // patches of up to 4 x 4, which share operands in an XCD's L2, the longest group's first (of up to 64 groups; of more, one
@@ -434,15 +447,11 @@ __global__ __launch_bounds__(GENERAL_THREADS * KW, KW == 1 ? 2 : 4) void ragged_
     const int tiles_n = (a.N + TN - 1) / TN;
     Tile t;
     if constexpr (MODE == ROWS) {
-        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+        if (!find_tile(a, TM, tiles_n, block_of(a), t)) return;
     } else if constexpr (MODE == OUTER) {
-        if (!outer_tile(a, TM, TN, blockIdx.x, t)) return;
+        if (!outer_tile(a, TM, TN, block_of(a), t)) return;
     } else {
-        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
-        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.group = 0;
-        t.first = t.tile_m * TM;
-        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
+        if (!shared_tile(a, TM, tiles_n, block_of(a), t)) return;
     }
     const bool real = MODE != ROWS || t.group < a.n_groups;   // the rows behind the last group have nothing to multiply
     const int n0 = t.tile_n * TN, m0 = t.tile_m * TM;

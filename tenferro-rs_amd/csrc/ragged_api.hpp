@@ -8,6 +8,16 @@
 namespace tfh {
 namespace ragged {
 
+// `blocks` blocks as a grid of x times y, each dimension of which has less than 2^32 threads and x a multiple of the XCDs: block
+// y * grid x + x, those from `blocks` on with nothing to do.  More than 2^31 are refused.
+inline int32_t launch_grid(int64_t blocks, int threads, uint32_t* x, uint32_t* y) {
+    if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the call needs %lld blocks, more than a launch has", (long long)blocks);
+    const int64_t most = ((int64_t)1 << 31) / threads / 8 * 8;
+    *x = (uint32_t)(blocks < most ? blocks : most);
+    *y = (uint32_t)((blocks + *x - 1) / *x);
+    return TFH_OK;
+}
+
 // Rows by group (k_row_groups.hip).
 struct GroupArgs {
     const void* ids;          // element of row i: (i / inner) * s_outer + (i % inner) * s_inner

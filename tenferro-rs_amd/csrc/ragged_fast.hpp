@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
     const int tiles_n = (a.N + TN - 1) / TN;
     Tile t;
     if constexpr (MODE == ROWS) {
-        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+        if (!find_tile(a, TM, tiles_n, block_of(a), t)) return;
         if constexpr (TM == 256) {
             // a group's last tile is seldom full: half or a quarter of the rows in half or 0.4 of the time
             typedef Shape<1, 4, 2, S::YT / 2, S::KB, S::SA, S::SB> Quarter;
@@ -548,13 +548,9 @@ __global__ __launch_bounds__(256, S::BLOCKS) void ragged_fast_kernel(const Args 
             }
         }
     } else if constexpr (MODE == OUTER || MODE == PAIR) {
-        if (!outer_tile(a, TM, TN, blockIdx.x, t)) return;
+        if (!outer_tile(a, TM, TN, block_of(a), t)) return;
     } else {
-        const int tiles_m = (int)((a.n_rows + TM - 1) / TM);
-        gemm::tile_of((uint32_t)gemm::logical_block(blockIdx.x, gridDim.x), tiles_m, tiles_n, t.tile_m, t.tile_n);
-        t.group = 0;
-        t.first = t.tile_m * TM;
-        t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
+        if (!shared_tile(a, TM, tiles_n, block_of(a), t)) return;
     }
     fast_tile<T, MODE, BKFAST, S>(a, t, lds);
 }

@@ -33,11 +33,13 @@ __global__ __launch_bounds__((few_threads<MODE>()), 1) void ragged_few_kernel(co
     const int tiles_n = (a.N + 15) / 16;
     Tile t;
     if constexpr (MODE == ROWS) {
-        if (!find_tile(a, TM, tiles_n, blockIdx.x, t)) return;
+        if (!find_tile(a, TM, tiles_n, block_of(a), t)) return;
     } else {
+        const uint32_t block = block_of(a);
+        if (block >= (uint32_t)((a.n_rows + TM - 1) / TM) * (uint32_t)tiles_n) return;
         t.group = 0;
-        t.tile_n = blockIdx.x % tiles_n;
-        t.first = (blockIdx.x / tiles_n) * TM;
+        t.tile_n = block % tiles_n;
+        t.first = (block / tiles_n) * TM;
         t.rows = a.n_rows - t.first < TM ? (int)(a.n_rows - t.first) : TM;
     }
     const bool real = MODE != ROWS || t.group < a.n_groups;

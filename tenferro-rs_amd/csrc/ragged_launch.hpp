@@ -13,6 +13,12 @@ namespace tfh {
 namespace ragged {
 
 inline int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
+// The grid of a launch (launch_grid), and Args that know it.
+inline int32_t grid_of(int64_t blocks, int threads, Args& a, dim3& grid) {
+    if (int32_t e = launch_grid(blocks, threads, &a.grid_x, &grid.y)) return e;
+    grid.x = a.grid_x;
+    return TFH_OK;
+}
 // Blocks of a launch over the groups' rows: no more tiles than the rows fill and one more, partly filled, for each group.
 inline int64_t row_tiles(const Args& a, int tm) {
     const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
@@ -34,11 +40,13 @@ int32_t launch_general_tiles(const Args& a, void* stream) {
     const int64_t blocks = MODE == ROWS ? row_tiles(a, 32 * XT) * tn
                            : MODE == OUTER ? Patches(a, 32 * XT, 32 * YT).blocks(a.n_groups) : tiles(a.n_rows, 32 * XT) * tn;
     if (blocks <= 0) return TFH_OK;
-    if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
+    Args args = a;
+    dim3 grid;
+    if (int32_t e = grid_of(blocks, GENERAL_THREADS * KW, args, grid)) return e;
     static const std::string label = std::string("(ragged_general_kernel<") + type_name<TA>() + ", " + type_name<TB>() + ", " + type_name<C>() + ", " +
                                      type_name<TO>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") + (UNIT ? "unit, " : "any, ") +
                                      std::to_string(32 * XT) + "x" + std::to_string(32 * YT) + (KW > 1 ? ", " + std::to_string(KW) : std::string()) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, UNIT, XT, YT, KW>), dim3((unsigned)blocks), dim3(GENERAL_THREADS * KW), 0, (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_general_kernel<TA, TB, C, TO, MODE, BKFAST, UNIT, XT, YT, KW>), grid, dim3(GENERAL_THREADS * KW), 0, (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 // Whether both operands are contiguous in the direction in which the kernel reads them, and long enough for a chunk.
@@ -86,7 +94,9 @@ int32_t launch_fast(const Args& a, void* stream) {
     const int64_t blocks = MODE == ROWS ? row_tiles(a, S::TM) * tn
                            : MODE == OUTER || MODE == PAIR ? Patches(a, S::TM, S::TN).blocks(a.n_groups) : tiles(a.n_rows, S::TM) * tn;
     if (blocks <= 0) return TFH_OK;
-    if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
+    Args args = a;
+    dim3 grid;
+    if (int32_t e = grid_of(blocks, 256, args, grid)) return e;
     static const bool once = [] {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_fast_kernel<T, MODE, BKFAST, S>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
         return true;
@@ -94,7 +104,7 @@ int32_t launch_fast(const Args& a, void* stream) {
     (void)once;
     static const std::string label = std::string("(ragged_fast_kernel<") + type_name<T>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") +
                                      std::to_string(S::TM) + "x" + std::to_string(S::TN) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_fast_kernel<T, MODE, BKFAST, S>), dim3((unsigned)blocks), dim3(256), S::LDS, (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_fast_kernel<T, MODE, BKFAST, S>), grid, dim3(256), S::LDS, (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 typedef Shape<2, 2, 4, 4, 128, 3, 2> Large;     // 256 x 256
@@ -126,27 +136,32 @@ template <class T, int MODE, int TR>
 int32_t launch_few(const Args& a, void* stream) {
     const int64_t blocks = (MODE == ROWS ? row_tiles(a, 16 * TR) : tiles(a.n_rows, 16 * TR)) * tiles(a.N, 16);
     if (blocks <= 0) return TFH_OK;
-    if (blocks > 0x7fffffff) return set_error(TFH_ERR_INVALID_ARGUMENT, "the product needs %lld blocks, more than one launch has", (long long)blocks);
+    Args args = a;
+    dim3 grid;
+    if (int32_t e = grid_of(blocks, few_threads<MODE>(), args, grid)) return e;
     static const bool once = [] {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_few_kernel<T, MODE, TR>), hipFuncAttributeMaxDynamicSharedMemorySize, few_lds<TR>());
         return true;
     }();
     (void)once;
     static const std::string label = std::string("(ragged_few_kernel<") + type_name<T>() + ", " + mode_name(MODE) + ", " + std::to_string(16 * TR) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR>), dim3((unsigned)blocks), dim3(few_threads<MODE>()), few_lds<TR>(), (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR>), grid, dim3(few_threads<MODE>()), few_lds<TR>(), (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 template <class T, bool BKFAST, int YT, int WAVES>
 int32_t launch_thin_waves(const Args& a, void* stream) {
     const int64_t blocks = row_tiles(a, THIN_ROWS);
     if (blocks <= 0) return TFH_OK;
+    Args args = a;
+    dim3 grid;
+    if (int32_t e = grid_of(blocks, 64 * WAVES, args, grid)) return e;
     static const bool once = [] {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (thin_lds<YT, WAVES>()));
         return true;
     }();
     (void)once;
     static const std::string label = std::string("(ragged_thin_kernel<") + type_name<T>() + (BKFAST ? ", k, " : ", n, ") + std::to_string(32 * YT) + ">)";
-    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), (thin_lds<YT, WAVES>()), (hipStream_t)stream, a);
+    TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT, WAVES>), grid, dim3(64 * WAVES), (thin_lds<YT, WAVES>()), (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
 }
 

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void ragged_thin_kernel(const Args a
     char* const lds = (char*)smem_raw;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Tile t;
-    if (!find_tile(a, THIN_ROWS, 1, blockIdx.x, t)) return;
+    if (!find_tile(a, THIN_ROWS, 1, block_of(a), t)) return;
     const int row = lane & 31, half = lane >> 5;
     const u32x4 A = buffer_of(a.A, (uint32_t)((a.a_rows - 1) * a.a_row * 2 + a.K * 2));
     const u32x4 B = buffer_of((const char*)a.B + t.group * a.b_group * 2, (uint32_t)(BKFAST ? (a.N - 1) * a.b_n * 2 + a.K * 2 : (a.K - 1) * a.b_k * 2 + a.N * 2));

@@ -1151,3 +1151,44 @@ def test_calls_on_a_side_stream_inside_a_capture_are_refused(tf, torch):
         z = tf.ragged_gemm(x, up, made_here, gather=True, stream=st)            # and outside, on the side stream
         torch.cuda.synchronize()
         assert torch.equal(z, h)
+
+
+# ------------------------------------------------------------------------------------------------------ launches of many blocks
+@pytest.mark.gpu
+def test_joined_rows_of_more_tokens_than_one_grid_dimension_holds(tf, torch):
+    # 2^26 tokens in blocks of four waves are 2^32 threads
+    n, N = (1 << 26) + 5, 8
+    x = torch.arange(n * N, dtype=torch.int32, device="cuda").remainder_(509).to(torch.bfloat16).view(n, N)      # exact, and others in every row
+    positions = torch.arange(n, dtype=torch.int32, device="cuda")
+    g = tf.RowGroups(torch.tensor([0, 7, n - 3], dtype=torch.int32, device="cuda"), positions, torch.where(positions < n - 3, positions, -1))
+    y = tf.combine_rows(x, g)
+    assert torch.equal(y[:n - 3], x[:n - 3]) and not y[n - 3:].any()
+    weights = torch.full((n, 1), 2.0, device="cuda")
+    dx, dw = tf.combine_rows_backward(x, weights, y, g)
+    assert torch.equal(dx, y * 2) and bool((dw[n - 3:] == 0).all())
+    some = torch.tensor([0, 1, 12345, (1 << 26) - 1, 1 << 26, n - 4], device="cuda")
+    assert torch.equal(dw[some, 0].double(), (x[some].double() ** 2).sum(1))      # eight squares below 2^18: exact
+
+
+@pytest.mark.gpu
+def test_products_of_more_tiles_than_one_grid_dimension_holds(tf, torch):
+    n = (1 << 30) + 333                                                           # 2^24 tiles of 64 rows, 256 threads each
+    a = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(251).to(torch.bfloat16).view(n, 1)
+    cut = 1000
+    g = tf.RowGroups(torch.tensor([0, cut, n - 2], dtype=torch.int32, device="cuda"), n_rows=n)
+    b = torch.tensor([2.0, -1.0], device="cuda").to(torch.bfloat16).view(2, 1, 1)
+    c = tf.ragged_gemm(a, b, g)
+    assert torch.equal(c[:cut], a[:cut] * 2) and torch.equal(c[cut:n - 2], -a[cut:n - 2]) and not c[n - 2:].any()
+    del c
+    groups = (1 << 24) + 77                                                       # and as many groups of a gradient
+    x, d = a[:groups], a[100:100 + groups]
+    g = tf.RowGroups(torch.arange(groups + 1, dtype=torch.int32, device="cuda"), n_rows=groups)
+    out = torch.full((groups, 1, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
+    tf.ragged_gemm_grad_into(x, d, g, 1.0, 0.0, out)
+    assert torch.equal(out.view(-1), (x.float() * d.float()).to(torch.bfloat16).view(-1))
+
+
+def test_more_blocks_than_a_launch_has_are_refused(tf):
+    L, V = tf.lib(), lambda *d: view(tf, d)
+    for dt in (tf.BF16, tf.F64):
+        refused(tf, L.tfh_ragged_gemm_grad(dt, row_groups(tf, n_rows=8, n_groups=1 << 30), 0, 1.0, V(8, 129), V(8, 129), 0.0, V(1 << 30, 129, 129), None), tf.InvalidArgument)
