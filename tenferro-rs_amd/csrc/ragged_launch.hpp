@@ -22,6 +22,7 @@ inline int32_t grid_of(int64_t blocks, int threads, Args& a, dim3& grid) {
 // Blocks of a launch over the groups' rows: no more tiles than the rows fill and one more, partly filled, for each group.
 inline int64_t row_tiles(const Args& a, int tm) {
     const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
+    if (a.n_groups > MANY_GROUPS) return many_tiles(a.n_rows, groups, tm);
     return a.n_rows / tm + (groups < a.n_rows ? groups : a.n_rows);
 }
 

@@ -1192,3 +1192,56 @@ def test_more_blocks_than_a_launch_has_are_refused(tf):
     L, V = tf.lib(), lambda *d: view(tf, d)
     for dt in (tf.BF16, tf.F64):
         refused(tf, L.tfh_ragged_gemm_grad(dt, row_groups(tf, n_rows=8, n_groups=1 << 30), 0, 1.0, V(8, 129), V(8, 129), 0.0, V(1 << 30, 129, 129), None), tf.InvalidArgument)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float32"])
+@pytest.mark.parametrize("groups,each,K,N", [(2049, 3, 64, 72), (3000, 40, 35, 17), (5000, 0.01, 40, 24), (2500, 60, 72, 136), (100000, 2, 8, 8)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_products_of_many_groups(tf, torch, name, groups, each, K, N, how):
+    # more groups than grouping by an index makes, some empty, with rows of none behind them; fewer rows than groups
+    rng = np.random.default_rng(groups)
+    counts = rng.integers(0, int(2 * each) + 1, groups) if each >= 1 else (rng.random(groups) < each).astype(int)
+    counts[[0, -1]] = [0, 3]
+    offsets = np.cumsum(np.concatenate([[0], counts]))
+    n = int(offsets[-1]) + 5
+    ids = torch.from_numpy(np.repeat(np.arange(groups), counts))
+    g = tf.RowGroups(torch.from_numpy(offsets.astype(np.int32)).cuda(), n_rows=n)
+    a, b, dc = tensor(torch, rng, (n, K), name), tensor(torch, rng, (groups, K, N), name, K ** -0.5), tensor(torch, rng, (n, N), name)
+    A, B, D = (t.cuda().double() for t in (a, b, dc))
+    on_b, p = layout(torch, b, how), slice(0, len(ids))
+    chosen = ids.cuda()
+    part = lambda x, m: torch.cat([torch.bmm(x[i:i + 4096, None], m[chosen[i:i + 4096]].contiguous())[:, 0] for i in range(0, len(ids), 4096)])
+    got = tf.ragged_gemm(a.cuda(), on_b, g)
+    close(got[p], part(A[p], B), part(A[p].abs(), B.abs()), K, name)
+    assert not got[len(ids):].any()
+    da, db = tf.ragged_gemm_backward(a.cuda(), on_b, dc.cuda(), g)
+    Bt = B.transpose(1, 2).contiguous()
+    close(da[p], part(D[p], Bt), part(D[p].abs(), Bt.abs()), N, name)
+    assert not da[len(ids):].any()
+    want, size = torch.zeros_like(B), torch.zeros_like(B)
+    for i in range(0, len(ids), 4096):
+        r = slice(i, min(i + 4096, len(ids)))
+        outer = A[r, :, None] * D[r, None, :]
+        want.index_add_(0, chosen[r], outer)
+        size.index_add_(0, chosen[r], outer.abs())
+    close(db, want, size, int(counts.max()), name)
+    if groups < 10000:
+        kept = torch.full((n, N), 7.0, dtype=a.dtype, device="cuda")                 # without zeros for the rows of none
+        tf.ragged_gemm_into(a.cuda(), on_b, g, 1.0, 0.0, kept)
+        assert torch.equal(kept[p], got[p]) and bool((kept[len(ids):] == 7).all())
+
+
+@pytest.mark.gpu
+def test_many_groups_that_do_not_ascend_stay_inside_the_views(tf, torch):
+    # offsets of any order and size: results as they may be, accesses inside the rows
+    rng = np.random.default_rng(5)
+    for n in (40, 30000):
+        offsets = rng.integers(-100, n + 100, 3001).astype(np.int32)
+        g = tf.RowGroups(torch.from_numpy(offsets).cuda(), n_rows=n)
+        a, b = torch.ones(n, 16, dtype=torch.bfloat16, device="cuda"), torch.ones(3000, 16, 8, dtype=torch.bfloat16, device="cuda")
+        c = torch.zeros(n, 8, dtype=torch.bfloat16, device="cuda")
+        tf.ragged_gemm_into(a, b, g, 1.0, 0.0, c)
+        assert set(c.unique().tolist()) <= {0.0, 16.0}
+        tf.ragged_gemm_backward(a, b, c, g)
+    torch.cuda.synchronize()
