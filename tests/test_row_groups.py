@@ -1245,3 +1245,85 @@ def test_many_groups_that_do_not_ascend_stay_inside_the_views(tf, torch):
         assert set(c.unique().tolist()) <= {0.0, 16.0}
         tf.ragged_gemm_backward(a, b, c, g)
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------------ long sums of the 16-bit kernels
+def device_products(torch, pairs):
+    """[(x, y)] -> (sums, sums of absolute values) in 64 bits on the GPU."""
+    return [(x @ y, x.abs() @ y.abs()) for x, y in ((x.cuda().double().contiguous(), y.cuda().double().contiguous()) for x, y in pairs)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16"])
+@pytest.mark.parametrize("K,N", [(1032, 1544), (2568, 1288)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+@pytest.mark.parametrize("counts,tiles", [([6149], "256x256"), ([1100, 0, 700, 1], "256x128"), ([130, 190, 0, 61] * 5, "128x128"), ([40] * 40, "32x128")])
+def test_long_sums_in_tiles_of_every_size(tf, torch, name, K, N, how, counts, tiles):
+    # every slot of LDS is used many times over
+    rng = np.random.default_rng(K + len(counts))
+    offsets, rows = np.cumsum([0] + counts), sum(counts)
+    a, b = tensor(torch, rng, (rows, K), name), tensor(torch, rng, (len(counts), K, N), name, K ** -0.5)
+    g = tf.RowGroups(torch.tensor(offsets, dtype=torch.int32, device="cuda"), n_rows=rows)
+    got = tf.ragged_gemm(a.cuda(), layout(torch, b, how), g)
+    assert tiles in tf.last_kernel() and "fast" in tf.last_kernel(), tf.last_kernel()
+    cut = [slice(offsets[i], offsets[i + 1]) for i in range(len(counts))]
+    for s, (want, size) in zip(cut, device_products(torch, [(a[s], b[i]) for i, s in enumerate(cut)])):
+        close(got[s], want, size, K, name)
+    if len(counts) < 40:
+        dc = tensor(torch, rng, (rows, N), name)
+        da, db = tf.ragged_gemm_backward(a.cuda(), layout(torch, b, how), dc.cuda(), g)
+        for s, (want, size) in zip(cut, device_products(torch, [(dc[s], b[i].t()) for i, s in enumerate(cut)])):
+            close(da[s], want, size, N, name)
+        for i, (want, size) in enumerate(device_products(torch, [(a[s].t(), dc[s]) for s in cut])):
+            close(db[i], want, size, max(counts), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16"])
+@pytest.mark.parametrize("K", [2056, 4104])
+@pytest.mark.parametrize("counts", [[4, 0, 3, 1], [20, 17], [50, 49, 0], [1]], ids=str)
+def test_long_sums_of_few_rows(tf, torch, name, K, counts):
+    rng = np.random.default_rng(K + sum(counts))
+    N, offsets, rows = 264, np.cumsum([0] + counts), sum(counts)
+    a, b = tensor(torch, rng, (rows, K), name), tensor(torch, rng, (len(counts), K, N), name, K ** -0.5)
+    g = tf.RowGroups(torch.tensor(offsets, dtype=torch.int32, device="cuda"), n_rows=rows)
+    got = tf.ragged_gemm(a.cuda(), layout(torch, b, "rows"), g)
+    assert "few" in tf.last_kernel(), tf.last_kernel()
+    cut = [slice(offsets[i], offsets[i + 1]) for i in range(len(counts))]
+    for s, (want, size) in zip(cut, device_products(torch, [(a[s], b[i]) for i, s in enumerate(cut)])):
+        close(got[s], want, size, K, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens,groups,K,N,R", [(8, 2, 4104, 520, 16), (20, 3, 4104, 1032, 64), (64, 5, 4104, 4104, 128), (500, 3, 4104, 1032, 16), (500, 3, 1032, 4104, 64), (500, 2, 4104, 1032, 128), (4480, 64, 1032, 1032, 32), (9000, 16, 1096, 520, 24)])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_long_sums_of_adapters(tf, torch, name, tokens, groups, K, N, R, how):
+    rng = np.random.default_rng(tokens + K + R)
+    ids = rng.integers(-1, groups, tokens)
+    x, dy, w = tensor(torch, rng, (tokens, K), name), tensor(torch, rng, (tokens, N), name), tensor(torch, rng, (K, N), name, K ** -0.5)
+    a, b = tensor(torch, rng, (groups, K, R), name, K ** -0.5), tensor(torch, rng, (groups, R, N), name, R ** -0.5)
+    scales = torch.from_numpy(0.2 + rng.random(groups)).float()
+    g = made(tf, torch, ids, groups)
+    on = [layout(torch, t, how) for t in (w, a, b)]
+    y = tf.adapter_gemm(x.cuda(), *on, g, scales.cuda())
+    dx, da, db = tf.adapter_gemm_backward(x.cuda(), *on, dy.cuda(), g, scales.cuda())
+    X, D, W, A, B, S = (t.cuda().double() for t in (x, dy, w, a, b, scales))
+    wt = W.t().contiguous()
+    want_y, size_y, want_x, size_x = X @ W, X.abs() @ W.abs(), D @ wt, D.abs() @ wt.abs()
+    low_y, low_x = torch.zeros_like(want_y), torch.zeros_like(want_x)
+    for i in range(groups):
+        t = torch.from_numpy(np.nonzero(ids == i)[0]).cuda()
+        x_, d_, at, bt = X[t], D[t], A[i].t().contiguous(), B[i].t().contiguous()
+        v, u, va, ua = x_ @ A[i], d_ @ bt, x_.abs() @ A[i].abs(), d_.abs() @ bt.abs()
+        want_y[t] += S[i] * (v @ B[i])
+        low_y[t] = S[i] * (va @ B[i].abs())
+        want_x[t] += S[i] * (u @ at)
+        low_x[t] = S[i] * (ua @ at.abs())
+        xt, vt = x_.t().contiguous(), v.t().contiguous()
+        size = S[i] * (xt.abs() @ ua)
+        close(da[i], S[i] * (xt @ u), size, len(t) + N, name, MIDDLE[name] * size.cpu())
+        size = S[i] * (va.t().contiguous() @ d_.abs())
+        close(db[i], S[i] * (vt @ d_), size, len(t) + K, name, MIDDLE[name] * size.cpu())
+    close(y, want_y, size_y + low_y, K + R, name, MIDDLE[name] * low_y.cpu())
+    close(dx, want_x, size_x + low_x, N + R, name, MIDDLE[name] * low_x.cpu())
