@@ -17,7 +17,8 @@ template <int YT> constexpr int thin_ahead() { return YT == 2 ? 3 : 2; }
 template <int YT, int WAVES> constexpr int thin_lds() { return WAVES * thin_ahead<YT>() * (THIN_ROWS + 32 * YT) * 128; }
 
 // V's row p as a pair of numbers of the operands' type, v = up (hi + lo): 16 bits of it in bf16, 22 in f16, so that it is
-// no rounding of its own beside the result's.  f16 alone has a short exponent: its rows are brought to [2^7, 2^8) first.
+// no rounding of its own beside the result's.  f16 alone has a short exponent: its rows' largest elements are brought to [2^14, 2^15)
+// first, the top of it, so that the others have their 22 bits down to 2^-18 of that, and half of them, as many as a result, to 2^-29.
 // `v`: this lane's columns lane, lane + 64.
 template <class T>
 __device__ __forceinline__ void store_pair(const Args& a, int64_t p, const float (&v)[2], int lane) {
@@ -34,7 +35,7 @@ __device__ __forceinline__ void store_pair(const Args& a, int64_t p, const float
         int e = 0;
         if (most > 0) {
             (void)frexpf(most, &e);
-            e = 8 - e;
+            e = 15 - e;
             e = e > 120 ? 120 : e < -120 ? -120 : e;
         }
         down = ldexpf(1.0f, e);

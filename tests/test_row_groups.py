@@ -1327,3 +1327,32 @@ def test_long_sums_of_adapters(tf, torch, name, tokens, groups, K, N, R, how):
         close(db[i], S[i] * (vt @ d_), size, len(t) + K, name, MIDDLE[name] * size.cpu())
     close(y, want_y, size_y + low_y, K + R, name, MIDDLE[name] * low_y.cpu())
     close(dx, want_x, size_x + low_x, N + R, name, MIDDLE[name] * low_x.cpu())
+
+
+# ------------------------------------------------------------------------------------------------------ the middle product of f16 adapters
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K,N,R", [(30, 64, 48, 8), (60, 520, 264, 16), (700, 192, 264, 64), (300, 1032, 520, 128)])
+@pytest.mark.parametrize("apart", [0, 12, 24])
+@pytest.mark.parametrize("how", ["columns", "rows"])
+def test_the_middle_of_f16_adapters_keeps_22_bits(tf, torch, rows, K, N, R, apart, how):
+    # Its elements are kept to half of 2^-21 of their own size, and to half of f16's smallest step, 2^-24, where the row's largest is at
+    # least 2^14 of these: 2^-39 of it.  Every second column of a is 2^-apart as large as the others, whose rows of b do the same: each
+    # contributes as much.  With w = 0 nothing covers for it.
+    rng = np.random.default_rng(rows + apart)
+    ids = rng.integers(-1, 3, rows)
+    x, w = tensor(torch, rng, (rows, K), "float16"), torch.zeros(K, N, dtype=torch.float16)
+    up, down = 2.0 ** min(apart, 10), 2.0 ** -max(0, apart - 10)
+    big = torch.where(torch.arange(R) % 2 == 0, up, down)
+    a = (torch.from_numpy(rng.standard_normal((3, K, R))) * K ** -0.5 * big).to(torch.float16)
+    b = (torch.from_numpy(rng.standard_normal((3, R, N))) / big[:, None] * up * 2.0 ** -min(apart, 10)).clamp(-6e4, 6e4).to(torch.float16)      # in range
+    if apart == 24:
+        b[:, ::2] = 0                                        # the small ones alone
+    on = [layout(torch, t, how) for t in (w, a, b)]
+    got = tf.adapter_gemm(x.cuda(), *on, made(tf, torch, ids, 3))
+    want, size, low = adapter_reference(torch, x, w, a, b, None, ids)
+    extra = 2.0 ** -22 * low
+    for i in range(3):
+        t = torch.from_numpy(np.nonzero(ids == i)[0])
+        v = x[t].double() @ a[i].double()
+        extra[t] += 2.0 ** -39 * v.abs().max(1, keepdim=True).values * b[i].double().abs().sum(0)
+    close(got, want, size, K + R, "float16", extra)
