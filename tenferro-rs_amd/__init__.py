@@ -731,6 +731,8 @@ class Tensor:
         """Zero-copy wrap of a torch CUDA tensor (any strides)."""
         if not t.is_cuda:
             raise InvalidArgument("invalid argument: from_torch takes a CUDA tensor")
+        if t.is_neg():
+            raise InvalidArgument("invalid argument: a tensor with torch's negative bit holds its values with the other sign: resolve_neg() it first")
         return cls(t, list(t.shape), [t.stride(d) for d in range(t.dim())], 0, GpuMemory(t.device.index or 0),
                    dtype_code(t.dtype))
 

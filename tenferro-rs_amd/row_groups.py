@@ -66,6 +66,8 @@ def _device(t):
         return t.logical_memory_space_.space_id
     if not t.is_cuda:
         raise NoCompatibleComputeDevice("no compatible compute device for this operation on MainMemory")
+    if t.is_neg():
+        raise InvalidArgument("invalid argument: a tensor with torch's negative bit holds its values with the other sign: resolve_neg() it first")
     return t.get_device()
 
 

@@ -1356,3 +1356,22 @@ def test_the_middle_of_f16_adapters_keeps_22_bits(tf, torch, rows, K, N, R, apar
         v = x[t].double() @ a[i].double()
         extra[t] += 2.0 ** -39 * v.abs().max(1, keepdim=True).values * b[i].double().abs().sum(0)
     close(got, want, size, K + R, "float16", extra)
+
+
+# ------------------------------------------------------------------------------------------------------ what a torch tensor may carry beside its values
+@pytest.mark.gpu
+def test_tensors_with_the_negative_bit_are_refused(tf, torch):
+    # .conj().imag is a real tensor whose memory holds the values with the other sign
+    z = torch.randn(8, 16, dtype=torch.complex64, device="cuda")
+    neg = z.conj().imag
+    assert neg.is_neg()
+    x, w = torch.randn(8, 16, device="cuda"), torch.randn(2, 16, 4, device="cuda")
+    g = tf.RowGroups(torch.tensor([0, 3, 8], dtype=torch.int32, device="cuda"), n_rows=8)
+    placed = tf.RowGroups.from_ids(torch.zeros(8, dtype=torch.int64, device="cuda"), 2)
+    for call in (lambda: tf.ragged_gemm(neg, w, g), lambda: tf.ragged_gemm(x, neg.unflatten(1, (4, 4)).permute(1, 0, 2)[:2], g), lambda: tf.combine_rows(neg, placed),
+                 lambda: tf.combine_rows(x, placed, neg[:, :1]), lambda: tf.adapter_gemm(neg, w[0], w[:, :, :2], w[:, :2], placed),
+                 lambda: tf.ragged_gemm_into(x, w, g, 1.0, 0.0, neg[:, :4]), lambda: tf.Tensor.from_torch(neg)):
+        with pytest.raises(tf.InvalidArgument, match="negative bit"):
+            call()
+    same = tf.ragged_gemm(neg.resolve_neg(), w, g)
+    assert torch.equal(same, tf.ragged_gemm((-z.imag).contiguous(), w, g))
