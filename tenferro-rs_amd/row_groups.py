@@ -11,6 +11,10 @@ first operand's kind.  Work is enqueued on `stream` (default: torch's current st
 waited for, and allocates through torch only, so the calls can be captured into a graph: on the current stream, and behind
 no event from before the capture (when the graph runs is the caller's to order).  On a stream other than the current one the
 caller orders the operands' earlier and the results' later use, as with any torch tensor.
+
+The calls record nothing for torch's autograd: gradients are calls of their own (*_backward), for a torch.autograd.Function to
+make.  So that none goes missing, an operand that requires grad is taken under torch.no_grad() (or in such a Function) only, and a
+forward-mode dual is not taken.
 """
 import ctypes as C
 import struct
@@ -28,12 +32,15 @@ class tfh_row_groups(C.Structure):
 
 _CODES, _TYPES = {}, {}
 _stream_of = None       # device index -> the handle of torch's current stream
+_torch = None
 
 
 def _codes():
-    global _stream_of
+    global _stream_of, _torch
     if not _CODES:
         import torch
+        import torch.autograd.forward_ad
+        _torch = torch
         # (the call behind torch.cuda.current_stream, without the object: 1 us of the 10 that a call takes)
         _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
         _CODES.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.float64: F64})
@@ -72,7 +79,14 @@ def _device(t):
 
 
 def _code(t):
-    dt = t.dtype if isinstance(t, Tensor) else _codes().get(t.dtype, -1)
+    if isinstance(t, Tensor):
+        dt = t.dtype
+    else:
+        dt = _codes().get(t.dtype, -1)
+        if t.requires_grad and _torch.is_grad_enabled():
+            raise InvalidArgument("invalid argument: an operand requires grad, which the call records nothing for: detach() it, or call under torch.no_grad()")
+        if _torch.autograd.forward_ad._current_level >= 0 and _torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise InvalidArgument("invalid argument: an operand is a forward-mode dual, whose tangent the call knows nothing of")
     if dt not in (BF16, F16, F32, F64):
         raise InvalidArgument(f"invalid argument: operations on rows in groups take bf16, f16, f32 and f64; got {t.dtype}")
     return dt

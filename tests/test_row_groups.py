@@ -1375,3 +1375,43 @@ def test_tensors_with_the_negative_bit_are_refused(tf, torch):
             call()
     same = tf.ragged_gemm(neg.resolve_neg(), w, g)
     assert torch.equal(same, tf.ragged_gemm((-z.imag).contiguous(), w, g))
+
+
+@pytest.mark.gpu
+def test_operands_of_autograd_are_refused_where_a_gradient_would_go_missing(tf, torch):
+    x, w = torch.randn(8, 16, device="cuda"), torch.randn(2, 16, 4, device="cuda")
+    g = tf.RowGroups(torch.tensor([0, 3, 8], dtype=torch.int32, device="cuda"), n_rows=8)
+    placed = tf.RowGroups.from_ids(torch.zeros(8, 1, dtype=torch.int64, device="cuda"), 2)
+    gates = torch.ones(8, 1, device="cuda")
+    want = tf.ragged_gemm(x, w, g)
+    leaf = torch.nn.Parameter(w.clone())
+    for call in (lambda: tf.ragged_gemm(x, leaf, g), lambda: tf.ragged_gemm(x.clone().requires_grad_(), w, g), lambda: tf.combine_rows(x, placed, gates.clone().requires_grad_()),
+                 lambda: tf.adapter_gemm(x, leaf[0], w[:, :, :2], w[:, :2], placed)):
+        with pytest.raises(tf.InvalidArgument, match="requires grad"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.inference_mode():
+        assert torch.equal(tf.ragged_gemm(x, leaf, g), want)
+
+    class Ragged(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a, b):
+            ctx.save_for_backward(a, b)
+            return tf.ragged_gemm(a, b, g)
+
+        @staticmethod
+        def backward(ctx, dc):
+            return tf.ragged_gemm_backward(*ctx.saved_tensors, dc, g)
+
+    a = x.clone().requires_grad_()
+    y = Ragged.apply(a, leaf)
+    dy = torch.randn_like(y)
+    da, db = torch.autograd.grad(y, (a, leaf), dy)
+    wa, wb = tf.ragged_gemm_backward(x, w, dy, g)
+    assert torch.equal(y.detach(), want) and torch.equal(da, wa) and torch.equal(db, wb)
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        assert torch.equal(tf.ragged_gemm(x, w, g), want)
+        with pytest.raises(tf.InvalidArgument, match="dual"):
+            tf.ragged_gemm(fw.make_dual(x, torch.ones_like(x)), w, g)
