@@ -272,7 +272,7 @@ int32_t tfh_ragged_gemm_grad_a(int32_t dtype, const tfh_row_groups* groups, int3
  * Y [n_rows / fan, N].  groups->positions is needed. */
 int32_t tfh_combine_rows(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* weights,
                          const tfh_view* y, tfh_stream stream);
-/* Its gradients: dX[p, :] = weights[t, j] * dY[t, :] (zeros for rows of no group) and dweights[t, j] = <X[p, :], dY[t, :]>
+/* Its gradients: dX[p, :] = weights[t, j] * dY[t, :] (zeros for rows of no group, and for those whose position was taken out) and dweights[t, j] = <X[p, :], dY[t, :]>
  * (0 for a choice of no group).  dx or dweights may be NULL: not wanted; x is read for dweights only. */
 int32_t tfh_combine_rows_grad(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* weights,
                               const tfh_view* dy, const tfh_view* dx, const tfh_view* dweights, tfh_stream stream);

@@ -99,12 +99,21 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineArgs a, 
     constexpr int E = Num<T>::E, STEP = 64 * E;
     const int lane = threadIdx.x & 63, block = (int)(blockIdx.z * gridDim.x + blockIdx.x);
     if (block >= token_blocks) {
-        // the rows behind the last group get zeros
+        // the rows behind the last group get zeros, and those before whose row's position is not theirs: no token writes them.  A
+        // lane looks at a row, its wave clears those found.
         if (!a.dx || block >= token_blocks + rest_blocks) return;
         const T zero[E] = {};
-        const int from = clamp_row(a.offsets[a.n_groups], a.n_rows);
-        for (int64_t p = from + (block - token_blocks) * 4 + (threadIdx.x >> 6); p < a.n_rows; p += rest_blocks * 4)
-            for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT, E>((T*)a.dx + p * a.dx_row, a.dx_n, n, a.n, zero);
+        const int end = clamp_row(a.offsets[a.n_groups], a.n_rows);
+        for (int64_t p0 = ((block - token_blocks) * 4 + (threadIdx.x >> 6)) * (int64_t)64; p0 < a.n_rows; p0 += rest_blocks * 256) {
+            const int64_t p = p0 + lane;
+            bool left = p < a.n_rows;
+            if (left && p < end) {
+                const int64_t i = a.order ? a.order[p] : p;
+                left = i < 0 || i >= a.n_rows || a.positions[i] != p;
+            }
+            for (uint64_t found = __ballot(left); found; found &= found - 1)
+                for (int n = lane * E; n < a.n; n += STEP) put_piece<T, UNIT, E>((T*)a.dx + (p0 + __builtin_ctzll(found)) * a.dx_row, a.dx_n, n, a.n, zero);
+        }
         return;
     }
     const int64_t t = (int64_t)block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -173,7 +182,7 @@ template <class T, class X, int F, bool UNIT> int32_t combine_as(const CombineAr
     return hip_check(hipGetLastError(), "combine launch");
 }
 template <class T, int F, bool UNIT> int32_t combine_grad_as(const CombineArgs& a, hipStream_t st) {
-    const int64_t blocks = (a.tokens + 3) / 4, rest = a.n_rows < 256 ? (a.n_rows + 3) / 4 : 64;
+    const int64_t blocks = (a.tokens + 3) / 4, rest = a.n_rows < 64 * 256 ? (a.n_rows + 255) / 256 : 64;
     uint32_t x, z;
     if (int32_t e = launch_grid(blocks + rest, 256, &x, &z)) return e;
     TFH_LAUNCH_NAMED(name_of<T>("(combine_grad_kernel<bf16>)", "(combine_grad_kernel<f16>)", "(combine_grad_kernel<float>)", "(combine_grad_kernel<double>)"),

@@ -234,7 +234,7 @@ int32_t combine(int32_t dtype, const tfh_row_groups* g, const tfh_view* x, const
     c.y = view_ptr(*y, dtype), c.y_row = y->strides[0], c.y_n = y->strides[1];
     if (dx) c.dx = view_ptr(*dx, dtype), c.dx_row = dx->strides[0], c.dx_n = dx->strides[1];
     if (dw) c.dw = view_ptr(*dw, sums), c.dw_token = dw->strides[0], c.dw_fan = dw->strides[1];
-    c.positions = g->positions, c.offsets = g->offsets;
+    c.positions = g->positions, c.offsets = g->offsets, c.order = g->order;
     c.n_rows = g->n_rows, c.tokens = tokens;
     c.n_groups = g->n_groups, c.fan = g->fan, c.n = (int32_t)N;
     const int prof = prof_begin(PROF_REDUCE, stream);

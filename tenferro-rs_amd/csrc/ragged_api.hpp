@@ -48,6 +48,7 @@ struct CombineArgs {
     int64_t dw_token, dw_fan;
     const int32_t* positions;
     const int32_t* offsets;
+    const int32_t* order;     // the gradient's, may be null
     int64_t n_rows, tokens;
     int32_t n_groups, fan, n;
 };

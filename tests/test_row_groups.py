@@ -1415,3 +1415,37 @@ def test_operands_of_autograd_are_refused_where_a_gradient_would_go_missing(tf, 
         assert torch.equal(tf.ragged_gemm(x, w, g), want)
         with pytest.raises(tf.InvalidArgument, match="dual"):
             tf.ragged_gemm(fw.make_dual(x, torch.ones_like(x)), w, g)
+
+
+# ------------------------------------------------------------------------------------------------------ choices taken out after grouping
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bfloat16", "float32"])
+@pytest.mark.parametrize("tokens,fan,groups,N", [(1, 1, 1, 3), (40, 2, 5, 64), (700, 4, 8, 24), (9000, 2, 6, 40)])
+@pytest.mark.parametrize("listed", [True, False])
+def test_choices_whose_position_was_taken_out_get_no_gradient(tf, torch, name, tokens, fan, groups, N, listed):
+    # a capacity limit applied to the positions: the rows still stand in their groups, and no token reads them
+    rng = np.random.default_rng(tokens)
+    ids = choices(rng, tokens, fan, groups)
+    if not listed:
+        ids = np.where((ids < 0) | (ids >= groups), groups, ids)
+        ids = np.sort(ids.reshape(-1)).reshape(tokens, fan)          # rows that lie in order: no order is given
+    offsets, order, positions = grouping(ids.reshape(-1), groups)
+    assert listed or order == list(range(tokens * fan))
+    positions, n = np.asarray(positions), tokens * fan
+    positions[rng.random(n) < 0.4] = -1
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")
+    g = tf.RowGroups(i32(offsets), i32(order) if listed else None, i32(positions), n_rows=n, fan=fan)
+    x, dy = tensor(torch, rng, (n, N), name), tensor(torch, rng, (tokens, N), name)
+    w = torch.from_numpy(rng.standard_normal((tokens, fan))).float()
+    junk = torch.full((n, N), float("nan"), dtype=x.dtype, device="cuda")
+    del junk                                                         # what the next buffer of that size finds there
+    dx, dw = tf.combine_rows_backward(x.cuda(), w.cuda(), dy.cuda(), g)
+    want, size = torch.zeros(n, N, dtype=torch.float64), torch.zeros(tokens * fan, dtype=torch.float64)
+    want_w = torch.zeros(tokens * fan, dtype=torch.float64)
+    kept = torch.from_numpy(np.nonzero(positions >= 0)[0])
+    p = torch.from_numpy(positions[positions >= 0])
+    want[p] = w.reshape(-1)[kept, None].double() * dy[kept // fan].double()
+    want_w[kept] = (x[p].double() * dy[kept // fan].double()).sum(1)
+    size[kept] = (x[p].double() * dy[kept // fan].double()).abs().sum(1)
+    close(dx, want, want.abs(), 1, name)
+    close(dw.reshape(-1), want_w, size, N, "float32")
