@@ -395,7 +395,7 @@ __device__ __forceinline__ void fast_tile(const Args& a, const Tile& t, char* ld
     // Results leave through LDS, so that a wave stores whole runs of a row: 16-byte chunks, the chunk index XORed with the
     // row because the 32 rows of a register would meet in one bank otherwise.  (Straight from the registers a store would
     // touch 32 rows with 16 bytes each.)
-    const float alpha = (float)a.alpha * (MODE == ROWS && a.scales && real ? ((const float*)a.scales)[t.group] : 1.0f), beta = (float)a.beta;
+    const float alpha = !real ? 0.0f : (float)a.alpha * (MODE == ROWS && a.scales ? ((const float*)a.scales)[t.group] : 1.0f), beta = (float)a.beta;
     if constexpr (MODE == PAIR) {
         // B's columns are a pair, hi and lo `pad` apart: their sums are added here, in f32, unless an infinity of A's is in them (finite_only)
         static_assert(TM * TN * 4 <= S::LDS && TN % 64 == 0, "the sums fit the two stages");

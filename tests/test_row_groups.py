@@ -1449,3 +1449,16 @@ def test_choices_whose_position_was_taken_out_get_no_gradient(tf, torch, name, t
     size[kept] = (x[p].double() * dy[kept // fan].double()).abs().sum(1)
     close(dx, want, want.abs(), 1, name)
     close(dw.reshape(-1), want_w, size, N, "float32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,K,N,rows", [("bfloat16", 64, 64, 900), ("float16", 256, 520, 9000), ("bfloat16", 4104, 264, 30), ("float32", 33, 5, 40), ("bfloat16", 35, 17, 300)])
+def test_rows_of_no_group_are_zeros_whatever_the_factor(tf, torch, name, K, N, rows):
+    code = {"bfloat16": tf.BF16, "float16": tf.F16, "float32": tf.F32}[name]
+    dtype = getattr(torch, name)
+    a, b, c = torch.ones(rows, K, dtype=dtype, device="cuda"), torch.ones(2, N, K, dtype=dtype, device="cuda").transpose(1, 2), torch.ones(rows, N, dtype=dtype, device="cuda")
+    g = tf.RowGroups(torch.tensor([0, 3, rows // 2], dtype=torch.int32, device="cuda"), n_rows=rows)
+    at = lambda t: view(tf, list(t.shape), list(t.stride()), t.data_ptr())
+    for alpha in (float("inf"), float("nan")):
+        tf._check(tf.lib().tfh_ragged_gemm(code, C.byref(g._c), 4, alpha, at(a), at(b), 0.0, at(c), torch.cuda.current_stream().cuda_stream))
+        assert not c[rows // 2:].any() and not c[:rows // 2].isfinite().any()
