@@ -26,6 +26,7 @@ BF16, F16 = 4, 5        # taken by the operations on rows in groups only
 _NP_DTYPES = {np.dtype(np.float32): F32, np.dtype(np.float64): F64, np.dtype(np.complex64): C64, np.dtype(np.complex128): C128,
               np.dtype(np.float16): F16}
 _DT_NP = {v: k for k, v in _NP_DTYPES.items()}
+_NO_BF16 = "invalid argument: tensors in main memory are numpy arrays, which have no bf16 (to_numpy() gives it as float32)"
 
 
 # ---------------------------------------------------------------------------------------------- C structs
@@ -690,6 +691,8 @@ class Tensor:
         n = int(np.prod(dims)) if dims else 1
         dt = dtype_code(dtype)
         if space.kind == 0:
+            if dt == BF16:
+                raise InvalidArgument(_NO_BF16)
             buf = np.zeros(n, _DT_NP[dt]) if fill is None else np.full(n, fill, _DT_NP[dt])
             return cls(buf, dims, _contig_strides(dims, order), 0, space, dt)
         import torch
@@ -923,6 +926,8 @@ class Tensor:
             t._lib_alloc = True
             return t
         self.wait()
+        if self.dtype == BF16:
+            raise InvalidArgument(_NO_BF16)
         return Tensor(self._buf.cpu().numpy(), self._dims, self._strides, self._offset, target, self.dtype)
 
     def wait(self):

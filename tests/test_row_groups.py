@@ -1462,3 +1462,18 @@ def test_rows_of_no_group_are_zeros_whatever_the_factor(tf, torch, name, K, N, r
     for alpha in (float("inf"), float("nan")):
         tf._check(tf.lib().tfh_ragged_gemm(code, C.byref(g._c), 4, alpha, at(a), at(b), 0.0, at(c), torch.cuda.current_stream().cuda_stream))
         assert not c[rows // 2:].any() and not c[:rows // 2].isfinite().any()
+
+
+@pytest.mark.parametrize("make", ["zeros", "ones", "empty"])
+def test_main_memory_refuses_bf16_by_name(tf, make):
+    with pytest.raises(tf.InvalidArgument, match="bf16"):
+        getattr(tf.Tensor, make)([2, 3], tf.MainMemory, tf.MemoryOrder.RowMajor, tf.BF16)
+    assert getattr(tf.Tensor, make)([2, 3], tf.MainMemory, tf.MemoryOrder.RowMajor, tf.F16).to_numpy().dtype == np.float16
+
+
+@pytest.mark.gpu
+def test_bf16_does_not_move_to_main_memory(tf, torch):
+    t = tf.Tensor.from_torch(torch.ones(2, 3, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(tf.InvalidArgument, match="bf16"):
+        t.to_memory_space_async(tf.MainMemory)
+    assert t.to_numpy().tolist() == [[1.0] * 3] * 2
