@@ -23,6 +23,7 @@ from . import (BF16, F16, F32, F64, CompletionEvent, CrossMemorySpaceOperation, 
                NoCompatibleComputeDevice, RankMismatch, ShapeMismatch, Tensor, _check, _in_flight, lib, tfh_view)
 
 GATHER_A, SCATTER_C, ZERO_REST = 1, 2, 4      # TFH_ROWS_*
+_MOST = 0x7fffffff      # what the C structure's 32-bit fields hold (ctypes would cut off the rest without a word)
 
 
 class tfh_row_groups(C.Structure):
@@ -234,6 +235,8 @@ class RowGroups:
         self.offsets, self.order, self.positions, self.n_rows, self.fan = offsets, order, positions, int(n_rows), int(fan)
         self.n_groups = offsets.numel() - 1
         self.event = None
+        if max(self.n_rows, self.n_groups, self.fan) > _MOST:
+            raise InvalidArgument(f"invalid argument: {self.n_groups} groups of {self.n_rows} rows with a fan of {self.fan} are out of range")
         self._c = tfh_row_groups(offsets.data_ptr(), order.data_ptr() if order is not None else None,
                                  positions.data_ptr() if positions is not None else None, self.n_rows, self.n_groups, self.fan)
         if self.n_groups < 1 or self.n_rows < 0 or self.fan < 1 or self.n_rows % self.fan:
@@ -251,8 +254,8 @@ class RowGroups:
         if ids.dim() not in (1, 2):
             raise RankMismatch(f"rank mismatch: expected 1, got {ids.dim()}", 1, ids.dim())
         n_groups, n = int(n_groups), ids.numel()
-        if n_groups < 1:
-            raise InvalidArgument(f"invalid argument: {n_groups} groups")
+        if n_groups < 1 or max(n, n_groups) > _MOST:
+            raise InvalidArgument(f"invalid argument: {n_groups} groups of {n} rows are out of range")
         fan = ids.shape[1] if ids.dim() == 2 else 1
         _CODES or _codes()
         current = _stream_of(device)

@@ -1477,3 +1477,15 @@ def test_bf16_does_not_move_to_main_memory(tf, torch):
     with pytest.raises(tf.InvalidArgument, match="bf16"):
         t.to_memory_space_async(tf.MainMemory)
     assert t.to_numpy().tolist() == [[1.0] * 3] * 2
+
+
+@pytest.mark.gpu
+def test_numbers_that_32_bit_fields_do_not_hold_are_refused(tf, torch):
+    ids = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for n in (0, -1, 2049, 1 << 31, (1 << 32) + 4):
+        with pytest.raises(tf.InvalidArgument):
+            tf.RowGroups.from_ids(ids, n)
+    offsets = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    for k in (dict(n_rows=0, fan=(1 << 32) + 1), dict(n_rows=1 << 40), dict(n_rows=(1 << 32), fan=1 << 32), dict(n_rows=-1), dict(n_rows=0, fan=0)):
+        with pytest.raises(tf.InvalidArgument):
+            tf.RowGroups(offsets, **k)
