@@ -176,7 +176,10 @@ class _Call:
             _check(lib().tfh_stream_wait_event(self.stream, CompletionEvent(self.current)._h))
             self.ordered = True
         dtype = self.dtype if dtype is None else dtype
-        if like is not None and not isinstance(like, Tensor):
+        if isinstance(like, Tensor):   # (torch has no negative strides)
+            ordered = min(like._strides, default=0) >= 0 and 0 not in like._dims
+            like = torch.as_strided(like._buf, like._dims, like._strides, like._buf.storage_offset() + like._offset) if ordered else None
+        if like is not None:
             t = torch.empty_like(like)
         else:
             tdt = dtype if isinstance(dtype, torch.dtype) else _TYPES[dtype]

@@ -1489,3 +1489,24 @@ def test_numbers_that_32_bit_fields_do_not_hold_are_refused(tf, torch):
     for k in (dict(n_rows=0, fan=(1 << 32) + 1), dict(n_rows=1 << 40), dict(n_rows=(1 << 32), fan=1 << 32), dict(n_rows=-1), dict(n_rows=0, fan=0)):
         with pytest.raises(tf.InvalidArgument):
             tf.RowGroups(offsets, **k)
+
+
+@pytest.mark.gpu
+def test_gradients_of_tensors_are_laid_out_like_them(tf, torch):
+    x, up, down, ids, gates, dy = layer_inputs(torch, 15)
+    T, flat = tf.Tensor.from_torch, tf.RowGroups.from_ids(ids[:, 0], up.shape[0])
+    dc = torch.randn(x.shape[0], up.shape[2], device="cuda")
+    want = tf.ragged_gemm_backward(x, up, dc, flat, gather=True)
+    columns = up.transpose(1, 2).contiguous().transpose(1, 2)
+    order = tf.Tensor(up.permute(2, 1, 0).contiguous().view(-1), list(up.shape), [1, up.shape[0], up.shape[0] * up.shape[1]], 0, tf.GpuMemory(0), tf.F32)   # column-major
+    big = torch.zeros(up.numel() + 7, device="cuda")
+    big[5:5 + up.numel()].copy_(up.reshape(-1))
+    shifted = tf.Tensor(big, list(up.shape), list(up.stride()), 5, tf.GpuMemory(0), tf.F32)
+    for b in (T(up), T(columns), order, shifted, T(up).permute([0, 2, 1]).permute([0, 2, 1])):
+        da, db = tf.ragged_gemm_backward(T(x), b, T(dc), flat, gather=True)
+        assert db.strides() == b.strides()
+        close(torch.from_numpy(db.to_numpy()), want[1], want[1].abs() + 10, 48, "float32")
+        assert np.abs(da.to_numpy() - want[0].cpu().numpy()).max() < 1e-4
+    wide = T(up[:1].expand(up.shape[0], -1, -1))                          # one matrix for all groups: nothing to be laid out like
+    _, db = tf.ragged_gemm_backward(T(x), wide, T(dc), flat, gather=True)
+    assert db.dims() == list(up.shape) and 0 not in db.strides()
