@@ -1,5 +1,6 @@
 // ragged_launch.hpp -- chooses and launches a kernel on rows in groups; one translation unit per operand type includes it.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "launch.hpp"
@@ -24,6 +25,16 @@ inline int64_t row_tiles(const Args& a, int tm) {
     const int64_t groups = a.n_groups + (a.zero_rest ? 1 : 0);
     if (a.n_groups > MANY_GROUPS) return many_tiles(a.n_rows, groups, tm);
     return a.n_rows / tm + (groups < a.n_rows ? groups : a.n_rows);
+}
+
+// A kernel's dynamic LDS beyond the default, once for each device: the attribute is of the device that is current.
+inline void allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
+    int device = 0;
+    (void)hipGetDevice(&device);
+    const uint64_t bit = (uint64_t)1 << (device & 63);
+    if (allowed.load(std::memory_order_relaxed) & bit) return;
+    (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    allowed.fetch_or(bit, std::memory_order_relaxed);
 }
 
 // "(kernel<arguments>)" as tfh_last_kernel spells them.
@@ -98,11 +109,8 @@ int32_t launch_fast(const Args& a, void* stream) {
     Args args = a;
     dim3 grid;
     if (int32_t e = grid_of(blocks, 256, args, grid)) return e;
-    static const bool once = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_fast_kernel<T, MODE, BKFAST, S>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
-        return true;
-    }();
-    (void)once;
+    static std::atomic<uint64_t> allowed{0};
+    allow_lds(reinterpret_cast<const void*>(&ragged_fast_kernel<T, MODE, BKFAST, S>), S::LDS, allowed);
     static const std::string label = std::string("(ragged_fast_kernel<") + type_name<T>() + ", " + mode_name(MODE) + (BKFAST ? ", k, " : ", n, ") +
                                      std::to_string(S::TM) + "x" + std::to_string(S::TN) + ">)";
     TFH_LAUNCH_NAMED(label.c_str(), (ragged_fast_kernel<T, MODE, BKFAST, S>), grid, dim3(256), S::LDS, (hipStream_t)stream, args);
@@ -140,11 +148,8 @@ int32_t launch_few(const Args& a, void* stream) {
     Args args = a;
     dim3 grid;
     if (int32_t e = grid_of(blocks, few_threads<MODE>(), args, grid)) return e;
-    static const bool once = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_few_kernel<T, MODE, TR>), hipFuncAttributeMaxDynamicSharedMemorySize, few_lds<TR>());
-        return true;
-    }();
-    (void)once;
+    static std::atomic<uint64_t> allowed{0};
+    allow_lds(reinterpret_cast<const void*>(&ragged_few_kernel<T, MODE, TR>), few_lds<TR>(), allowed);
     static const std::string label = std::string("(ragged_few_kernel<") + type_name<T>() + ", " + mode_name(MODE) + ", " + std::to_string(16 * TR) + ">)";
     TFH_LAUNCH_NAMED(label.c_str(), (ragged_few_kernel<T, MODE, TR>), grid, dim3(few_threads<MODE>()), few_lds<TR>(), (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
@@ -156,11 +161,8 @@ int32_t launch_thin_waves(const Args& a, void* stream) {
     Args args = a;
     dim3 grid;
     if (int32_t e = grid_of(blocks, 64 * WAVES, args, grid)) return e;
-    static const bool once = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (thin_lds<YT, WAVES>()));
-        return true;
-    }();
-    (void)once;
+    static std::atomic<uint64_t> allowed{0};
+    allow_lds(reinterpret_cast<const void*>(&ragged_thin_kernel<T, BKFAST, YT, WAVES>), (thin_lds<YT, WAVES>()), allowed);
     static const std::string label = std::string("(ragged_thin_kernel<") + type_name<T>() + (BKFAST ? ", k, " : ", n, ") + std::to_string(32 * YT) + ">)";
     TFH_LAUNCH_NAMED(label.c_str(), (ragged_thin_kernel<T, BKFAST, YT, WAVES>), grid, dim3(64 * WAVES), (thin_lds<YT, WAVES>()), (hipStream_t)stream, args);
     return hip_check(hipGetLastError(), "product over groups of rows");
