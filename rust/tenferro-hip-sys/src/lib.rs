@@ -186,7 +186,6 @@ extern "C" {
     pub fn tfh_conj(dtype: i32, input: *const tfh_view, out: *mut tfh_view, stream: tfh_stream) -> i32;
     pub fn tfh_fill(dtype: i32, value: *const c_void, out: *mut tfh_view, stream: tfh_stream) -> i32;
 
-    // ---- Subscripts and ContractionTree (tenferro-einsum/src/lib.rs:239-356)
     // ---- rows in groups
     pub fn tfh_group_rows_workspace(n_rows: i64, n_groups: i32) -> usize;
     pub fn tfh_group_rows(id_bits: i32, ids: *const tfh_view, n_groups: i32, offsets: *mut i32, order: *mut i32,
@@ -213,6 +212,7 @@ extern "C" {
         da: *const tfh_view, db: *const tfh_view, workspace: *mut c_void, workspace_bytes: usize,
         stream: tfh_stream) -> i32;
 
+    // ---- Subscripts and ContractionTree (tenferro-einsum/src/lib.rs:239-356)
     pub fn tfh_subscripts_new(labels: *const u32, ranks: *const i32, n_inputs: i32, output: *const u32,
         n_output: i32, out: *mut *mut tfh_subscripts) -> i32;
     pub fn tfh_subscripts_parse(notation: *const c_char, out: *mut *mut tfh_subscripts) -> i32;

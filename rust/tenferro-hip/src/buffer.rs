@@ -29,21 +29,13 @@ pub struct HipBuffer<T> {
 unsafe impl<T: Send> Send for HipBuffer<T> {}
 unsafe impl<T: Sync> Sync for HipBuffer<T> {}
 
-impl<T: ScalarBase> HipBuffer<T> {
+impl<T> HipBuffer<T> {
     /// Uninitialised device memory for `len` elements on the current device.
     pub fn new(len: usize, device_id: usize) -> Result<Self> {
         crate::set_device(device_id)?;
         let mut raw: *mut c_void = std::ptr::null_mut();
         check(unsafe { sys::tfh_malloc(len * std::mem::size_of::<T>(), &mut raw) })?;
         Ok(Self { ptr: raw as *mut T, len, device_id })
-    }
-
-    /// `Tensor::zeros` / `ones` (tenferro-tensor/src/lib.rs:336-347) on device memory: every element = `value`.
-    pub fn filled(len: usize, value: T, device_id: usize, stream: &Stream) -> Result<Self> {
-        let buf = Self::new(len, device_id)?;
-        let mut v = HipViewMut::dense(&buf, &[len]).raw();
-        check(unsafe { sys::tfh_fill(dtype_tag::<T>()?, &value as *const T as *const c_void, &mut v, stream.raw()) })?;
-        Ok(buf)
     }
 
     /// Host -> device (`Tensor::to_memory_space_async`, tenferro-tensor/src/lib.rs:660-671).  Pageable host memory is
@@ -109,6 +101,16 @@ impl<T: ScalarBase> HipBuffer<T> {
     /// As for `as_device_slice`.
     pub unsafe fn as_device_slice_mut(&mut self) -> &mut [T] {
         std::slice::from_raw_parts_mut(self.ptr, self.len)
+    }
+}
+
+impl<T: ScalarBase> HipBuffer<T> {
+    /// `Tensor::zeros` / `ones` (tenferro-tensor/src/lib.rs:336-347) on device memory: every element = `value`.
+    pub fn filled(len: usize, value: T, device_id: usize, stream: &Stream) -> Result<Self> {
+        let buf = Self::new(len, device_id)?;
+        let mut v = HipViewMut::dense(&buf, &[len]).raw();
+        check(unsafe { sys::tfh_fill(dtype_tag::<T>()?, &value as *const T as *const c_void, &mut v, stream.raw()) })?;
+        Ok(buf)
     }
 }
 
@@ -205,19 +207,6 @@ fn check_rank(rank: usize) -> Result<()> {
 }
 
 impl<'a, T: ScalarBase> HipView<'a, T> {
-    pub fn new(buffer: &'a HipBuffer<T>, dims: &[usize], strides: &[isize], offset: isize) -> Result<Self> {
-        check_rank(dims.len())?;
-        if dims.len() != strides.len() {
-            return Err(Error::RankMismatch { expected: dims.len(), got: strides.len() });
-        }
-        Ok(Self { base: buffer.as_device_ptr(), dims: dims.to_vec(), strides: strides.to_vec(), offset, conj: false, _buffer: PhantomData })
-    }
-
-    /// The whole buffer as a dense row-major tensor of shape `dims`.
-    pub fn dense(buffer: &'a HipBuffer<T>, dims: &[usize]) -> Self {
-        Self { base: buffer.as_device_ptr(), dims: dims.to_vec(), strides: row_major(dims), offset: 0, conj: false, _buffer: PhantomData }
-    }
-
     /// From the `StridedView` that `TensorPrims::execute` is handed: the slice under it is device memory
     /// ([`HipBuffer::as_device_slice`]); only its address, dims, strides and offset are read.
     pub fn from_strided<'v>(view: &'a StridedView<'v, T>) -> Result<Self>
@@ -233,6 +222,21 @@ impl<'a, T: ScalarBase> HipView<'a, T> {
             conj: false,
             _buffer: PhantomData,
         })
+    }
+}
+
+impl<'a, T: Copy> HipView<'a, T> {
+    pub fn new(buffer: &'a HipBuffer<T>, dims: &[usize], strides: &[isize], offset: isize) -> Result<Self> {
+        check_rank(dims.len())?;
+        if dims.len() != strides.len() {
+            return Err(Error::RankMismatch { expected: dims.len(), got: strides.len() });
+        }
+        Ok(Self { base: buffer.as_device_ptr(), dims: dims.to_vec(), strides: strides.to_vec(), offset, conj: false, _buffer: PhantomData })
+    }
+
+    /// The whole buffer as a dense row-major tensor of shape `dims`.
+    pub fn dense(buffer: &'a HipBuffer<T>, dims: &[usize]) -> Self {
+        Self { base: buffer.as_device_ptr(), dims: dims.to_vec(), strides: row_major(dims), offset: 0, conj: false, _buffer: PhantomData }
     }
 
     /// The same elements read as their complex conjugates (`TFH_VIEW_CONJ`): the lazy form of `Tensor::conj`
@@ -272,7 +276,7 @@ impl<'a, T: ScalarBase> HipView<'a, T> {
     }
 }
 
-impl<'a, T: ScalarBase> HipViewMut<'a, T> {
+impl<'a, T: Copy> HipViewMut<'a, T> {
     pub fn new(buffer: &'a mut HipBuffer<T>, dims: &[usize], strides: &[isize], offset: isize) -> Result<Self> {
         check_rank(dims.len())?;
         if dims.len() != strides.len() {
@@ -287,6 +291,18 @@ impl<'a, T: ScalarBase> HipViewMut<'a, T> {
         Self { base: buffer.as_device_ptr(), dims: dims.to_vec(), strides: row_major(dims), offset: 0, _buffer: PhantomData }
     }
 
+    pub fn dims(&self) -> &[usize] {
+        &self.dims
+    }
+    pub fn strides(&self) -> &[isize] {
+        &self.strides
+    }
+    pub fn raw(&self) -> sys::tfh_view {
+        fill_raw(self.base as *mut c_void, &self.dims, &self.strides, self.offset, 0)
+    }
+}
+
+impl<'a, T: ScalarBase> HipViewMut<'a, T> {
     /// From the `StridedViewMut` that `TensorPrims::execute` is handed (device memory underneath).  The borrow of the
     /// view (`'a`) is separate from, and outlived by, the lifetime of the data it views (`'v`): `execute` passes
     /// `&mut StridedViewMut<T>` whose own lifetime parameter is invariant and unrelated to the borrow.
@@ -302,16 +318,6 @@ impl<'a, T: ScalarBase> HipViewMut<'a, T> {
             offset: view.offset(),
             _buffer: PhantomData,
         })
-    }
-
-    pub fn dims(&self) -> &[usize] {
-        &self.dims
-    }
-    pub fn strides(&self) -> &[isize] {
-        &self.strides
-    }
-    pub fn raw(&self) -> sys::tfh_view {
-        fill_raw(self.base as *mut c_void, &self.dims, &self.strides, self.offset, 0)
     }
 
     /// `Tensor::into_conj` (tenferro-tensor/src/lib.rs:653-658): conjugate in place.

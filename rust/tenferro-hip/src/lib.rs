@@ -27,7 +27,7 @@ pub use backend::{HipBackend, HipGroupedPlan, HipPlan};
 pub use buffer::{HipBuffer, HipView, HipViewMut, PinnedBuffer};
 pub use einsum::{einsum_with_plan_into, ContractionTree, Subscripts};
 pub use event::{CompletionEvent, Stream};
-pub use rows::{AdapterFactors, RowGroups};
+pub use rows::{AdapterFactors, Bf16, F16, RowGroups, RowIndex, RowScalar};
 
 use std::any::TypeId;
 use std::ffi::CStr;

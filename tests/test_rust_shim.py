@@ -178,3 +178,18 @@ def test_the_safe_crate_uses_every_symbol_it_binds_and_implements_the_trait():
     assert "impl<T> Drop for HipPlan<T>" in backend and "sys::tfh_plan_destroy" in backend
     event = open(os.path.join(SAFE_DIR, "event.rs")).read()
     assert "pub struct CompletionEvent" in event and "impl Drop for CompletionEvent" in event
+
+
+def test_rows_in_groups_take_every_type_of_the_c_interface():
+    # 16-bit elements, weights and scales of the sums' type, indices of 32 and 64 bits
+    rows = open(os.path.join(SAFE_DIR, "rows.rs")).read()
+    tags = dict(re.findall(r"impl RowScalar for (\w+) \{\s*type Sum = \w+;\s*const TAG: i32 = sys::(\w+);", rows))
+    assert tags == {"Bf16": "TFH_BF16", "F16": "TFH_F16", "f32": "TFH_F32", "f64": "TFH_F64"}
+    assert dict(re.findall(r"impl RowScalar for (\w+) \{\s*type Sum = (\w+);", rows)) == {"Bf16": "f32", "F16": "f32", "f32": "f32", "f64": "f64"}
+    assert dict(re.findall(r"impl RowIndex for (\w+) \{\s*const BITS: i32 = (\d+);", rows)) == {"i32": "32", "i64": "64"}
+    assert "dtype_tag" not in rows and "HipView<T>>, y" not in rows
+    for name in ("weights: Option<&HipView<T::Sum>>", "dweights: Option<&mut HipViewMut<T::Sum>>", "scales: Option<&'a HipView<'a, T::Sum>>"):
+        assert name in rows, name
+    buffer = open(os.path.join(SAFE_DIR, "buffer.rs")).read()                # memory and views of any element; the Standard set where a tag is asked for
+    for item in ("impl<T> HipBuffer<T> {", "impl<T: ScalarBase> HipBuffer<T> {", "impl<'a, T: Copy> HipView<'a, T> {", "impl<'a, T: Copy> HipViewMut<'a, T> {"):
+        assert item in buffer, item
