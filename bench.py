@@ -619,6 +619,22 @@ HAS_LAYOUTS = ("c0", "c1", "c3", "c4", "b64", "b128")   # configurations that ar
 HEADLINE = "c3"   # the largest configuration that fits one GPU
 
 
+def rows_in_groups(h, passes=12):
+    """The operators on rows in groups over the cases of perf/operators.py, `passes` of each over two sets of inputs in turn (a
+    kernel's statistics under rocprofv3; the printed time a pass is the median's, each waited for)."""
+    from perf import operators
+    operators.own = True
+    for case in operators.listed():
+        states, times = [operators.prepare(case, seed) for seed in (0, 1)], []
+        h.torch.cuda.synchronize()
+        for i in range(passes):
+            start = time.perf_counter()
+            operators.run(states[i % 2])
+            h.torch.cuda.synchronize()
+            times.append(time.perf_counter() - start)
+        print("%-20s %10.1f us" % (case["name"], 1e6 * sorted(times)[passes // 2]), flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -634,6 +650,8 @@ def main():
                     help="permutes and reductions of seeded random tensors (rank 3..7, >= 128 MB, extents that are no powers of two)")
     ap.add_argument("--host-overhead", action="store_true",
                     help="print the host cost of tfh_execute per call (first against repeated) instead of running the benchmark")
+    ap.add_argument("--rows-in-groups", action="store_true",
+                    help="run the operators on rows in groups over the cases of perf/operators.py instead of the benchmark")
     ap.add_argument("--pmc-calibration", action="store_true",
                     help="also launch three plain 1 GiB device-to-device copies (torch's elementwise copy kernel): under "
                          "rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE their readings give the counter's scale for known traffic")
@@ -641,12 +659,15 @@ def main():
     if args.gpus != 1:
         sys.stderr.write("bench.py: this build runs on ONE GPU (no collectives, no sharding); --gpus %d is not supported\n" % args.gpus)
         sys.exit(2)
-    h = Harness(args.steps, args.warmup, not args.no_cpu and not args.host_overhead and not args.shape_sweep)
+    h = Harness(args.steps, args.warmup, not args.no_cpu and not args.host_overhead and not args.shape_sweep and not args.rows_in_groups)
     if args.shape_sweep:
         shape_sweep(h, min_bytes=args.sweep_mb << 20, ops=tuple(args.sweep_ops.split(",")), dtypes=tuple(args.sweep_dtypes.split(",")))
         return
     if args.host_overhead:
         host_overhead(h)
+        return
+    if args.rows_in_groups:
+        rows_in_groups(h)
         return
     if args.pmc_calibration:
         src = h.torch.ones(1 << 28, dtype=h.torch.float32, device="cuda")
