@@ -215,13 +215,15 @@ int32_t tfh_fill(int32_t dtype, const void* value, tfh_view* out, tfh_stream str
  * sector of a block-sparse tensor's row), so the sizes never reach the host.  All calls enqueue on `stream`, wait for
  * nothing and allocate nothing; what scratch they need is the caller's (`workspace`), so a captured call keeps to memory
  * of its own graph.  Scalar types: TFH_BF16, TFH_F16, TFH_F32, TFH_F64.  Sums are held in f32 (f64 for TFH_F64) and
- * rounded once.  Views may have any strides, negative and zero ones included for inputs; an output may not overlap an
+ * rounded once.  Views may have any strides, negative and zero ones included for inputs (scales alone have to lie next to
+ * each other, or TFH_ERR_STRIDED); an output may not overlap an
  * input or itself.  The work runs on the device that is current, on which the memory has to be.
  *
  * tfh_row_groups: n_rows rows listed group by group.
  *   offsets    [n_groups + 1], ascending from 0: group g is p = offsets[g] .. offsets[g + 1]; the rows behind
  *              offsets[n_groups] belong to no group
- *   order      [n_rows] or NULL (the rows lie in that order already): place p holds row order[p], no row twice
+ *   order      [n_rows] or NULL (the rows lie in that order already): place p holds row order[p], no row twice; what is
+ *              written by row is left as it is for a row that the order names nowhere
  *   positions  [n_rows] or NULL: where row i stands, -1 for a row of no group
  *   fan        rows per source row (a token's choices): row i = t * fan + j is choice j of token t
  * Entries out of range are treated as absent (offsets are clamped to [0, n_rows]); they never lead out of the views.
@@ -279,7 +281,7 @@ int32_t tfh_combine_rows_grad(int32_t dtype, const tfh_row_groups* groups, const
 
 /* Y[t, :] = X[t, :] . W + scales[g] * (X[t, :] . A[g]) . B[g] for a row t of group g, X[t, :] . W for a row of none: one
  * matrix for all rows and a low-rank correction of it by group.  X [n_rows, K], W [K, N], A [n_groups, K, R],
- * B [n_groups, R, N], scales [n_groups] of the sums' type or NULL (ones), Y [n_rows, N]; rows of X and Y in their own
+ * B [n_groups, R, N], scales [n_groups] of the sums' type, next to each other, or NULL (ones), Y [n_rows, N]; rows of X and Y in their own
  * order, not the groups'.  fan must be 1.  workspace: tfh_adapter_workspace(dtype, n_rows, R, 0) bytes, 16-byte aligned. */
 size_t tfh_adapter_workspace(int32_t dtype, int64_t n_rows, int64_t rank, int32_t gradient);
 int32_t tfh_adapter_gemm(int32_t dtype, const tfh_row_groups* groups, const tfh_view* x, const tfh_view* w, const tfh_view* a,

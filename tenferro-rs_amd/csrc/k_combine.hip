@@ -5,7 +5,7 @@
 // with p = pos[t fan + j]; a choice without a place (p < 0) adds nothing, whatever its weight holds.  One wave a token:
 // its row of y (dy) is made (read) once, in 16-byte pieces, with the places and weights in scalar registers and two pieces of every
 // choice in flight.  HBM bound: 16 384 tokens of four choices, 2048 bf16 columns: 74 us, 4.5 TB/s of reads and writes (a copy: 5.1);
-// the gradients of 8192: 64 us, 4.7 TB/s.
+// the gradients of 8192: 66 us, 4.6 TB/s; 8192 tokens of f32 parts into bf16: 57 us, 5.3 TB/s, some of it from L2.
 #include <hip/hip_runtime.h>
 
 #include "launch.hpp"

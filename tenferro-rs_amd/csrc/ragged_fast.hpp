@@ -11,10 +11,10 @@
 // so a fragment has 16 k's products to arrive in, a load those of all slots but one, and there is one barrier per stage.
 //
 // Bound by the matrix cores, and by their power with random numbers.  Reached, bf16: one group of 16 384 rows, 8192 x 4096: 1250
-// TFLOP/s (a library product: 1490); 65 536 gathered rows of 64 uneven groups, 2048 x 2048: 590 us, 930 TFLOP/s, the matrix cores 46 %
+// TFLOP/s (a library product: 1490); 65 536 gathered rows of 64 uneven groups, 2048 x 2048: 590 us, 930 TFLOP/s, the matrix cores 45 %
 // busy at 1.8 GHz -- a tile of 32 stages starts and ends with a tenth of its time, the groups' last tiles and the last round cost as
-// much, and LDS is read and written three quarters of the time; gradients of 32 768 rows of 32 uneven groups, 2048 x 1024: 201 us, 684, with their rows
-// looked up (163 us, 843 without); adapters' shared product, 16 384 x 4096 x 4096: 530 us, 1040.
+// much, and LDS is read and written three quarters of the time; gradients of 32 768 rows of 32 uneven groups, 2048 x 1024: 186 us, 740, with their rows
+// looked up; the rows' gradients there, kept in f32: 203 us (178 in bf16); adapters' shared product, 16 384 x 4096 x 4096: 530 us, 1040.
 #pragma once
 #include <utility>
 
@@ -101,7 +101,8 @@ __device__ __forceinline__ u32x4 fragment32(const char* tile, int row, int h, in
 //
 // A k-fast tile wants KB = 128: its loads then ask for whole lines, and 64-byte pieces cost L2 as much each (256 x 256 tiles
 // need 13 TB/s of it).  That leaves room in LDS for five tiles, three of one operand and two of the other; the other's loads
-// go first after the barrier.  Row-fast tiles ask for whole rows of columns anyway and take KB = 64, five stages of both.
+// go first after the barrier.  256 x 128 tiles, two to a compute unit, take KB = 64, three stages of both; outer products, whose
+// tiles are row-fast and ask for whole rows of columns anyway, lose nothing by that.
 template <int WM_, int WN_, int XT_, int YT_, int KB_ = 128, int SA_ = 2, int SB_ = 2> struct Shape {
     static_assert(WM_ * WN_ == 4, "four waves");
     static_assert(SB_ >= 2 && (SA_ == SB_ || SA_ == SB_ + 1), "the waits below count on it");

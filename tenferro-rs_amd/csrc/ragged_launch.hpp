@@ -198,7 +198,8 @@ template <class T> int32_t launch_product(int kind, const Args& a, void* stream)
         if (kind == PRODUCT_SHARED && a.pad > 0 && !columns && few_takes<SHARED>(a) && tiles(a.n_rows, 64) * tiles(a.N, 16) <= 1024)
             return a.n_rows <= 16 ? launch_few<T, SHARED, 1>(a, stream) : a.n_rows <= 32 ? launch_few<T, SHARED, 2>(a, stream) : launch_few<T, SHARED, 4>(a, stream);
         // Tiles of 128 x 128 that span the groups: larger ones of one group each leave more of the rows' tiles half empty (8192 rows
-        // of 16 groups, 4096 x 4096: 285 us against 345; 16 384 of 8: 530 and 580; 4096 of 8, 2048 x 4096: 92 and 112).
+        // of 16 groups, 4096 x 4096, on the same inputs again: 285 us against 345, 298 with others each time; 16 384 of 8: 530 and 580; 4096 of
+        // 8, 2048 x 4096: 92 and 112).
         if (kind == PRODUCT_SHARED && a.pad > 0) return columns ? launch_fast<T, SHARED, false, Middle>(a, stream) : launch_fast<T, SHARED, true, Middle>(a, stream);
         // (eight groups of 4096 rows, 4096 and 2048 x 64: 26 us in tiles of 64 rows, three stages on their way, 34 in those of 128)
         if (kind == PRODUCT_OUTER_V && a.pad > 0)

@@ -6,7 +6,7 @@ reference; beside HipBackend.plan_grouped, whose groups' extents are fixed when 
     h = ragged_gemm(x, w_up, groups, gather=True)                  # [tokens * fan, N], group by group
     y = combine_rows(ragged_gemm(act(h), w_down, groups), groups, gates)      # [tokens, K]
 
-Operands are torch CUDA tensors or GpuMemory Tensors of bf16, f16, f32 or f64, with any strides; a result is of the
+Operands are torch CUDA tensors or GpuMemory Tensors of bf16, f16, f32 or f64, with any strides (scales: contiguous); a result is of the
 first operand's kind.  Work is enqueued on `stream` (default: torch's current stream of the operands' device), never
 waited for, and allocates through torch only, so the calls can be captured into a graph: on the current stream, and behind
 no event from before the capture (when the graph runs is the caller's to order).  On a stream other than the current one the
@@ -426,7 +426,7 @@ def adapter_gemm_into(x, w, a, b, groups, y, scales=None, stream=None):
 def adapter_gemm(x, w, a, b, groups, scales=None, stream=None):
     """x @ w + scales[g] * (x @ a[g]) @ b[g], row by row with the row's group g; x @ w alone for a row of none.
     x [n_rows, K] in its own order, w [K, N], a [n_groups, K, R], b [n_groups, R, N], scales f32 (f64 beside f64)
-    [n_groups] or None: ones.  groups with fan 1."""
+    [n_groups], contiguous, or None: ones.  groups with fan 1."""
     _groups(groups)
     _rank("w", w, 2), _rank("a", a, 3)
     with _Call(x, (x, w, a, b), groups, stream, (scales,)) as k:
