@@ -226,7 +226,8 @@ int32_t tfh_fill(int32_t dtype, const void* value, tfh_view* out, tfh_stream str
  *              written by row is left as it is for a row that the order names nowhere
  *   positions  [n_rows] or NULL: where row i stands, -1 for a row of no group
  *   fan        rows per source row (a token's choices): row i = t * fan + j is choice j of token t
- * Entries out of range are treated as absent (offsets are clamped to [0, n_rows]); they never lead out of the views.
+ * Entries out of range are treated as absent (offsets are clamped to [0, n_rows], and a place whose order leads nowhere reads a row
+ * of zeros); they never lead out of the views.
  * Rows, groups and the operands' extents are at most 2^31 - 2^20, and a call takes no more than 2^31 blocks of a result, of 32 by 32
  * elements at least (a group's last ones may be partly filled); strides and offsets have 64 bits. */
 typedef struct tfh_row_groups {

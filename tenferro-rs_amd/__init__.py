@@ -402,6 +402,18 @@ def view_of(t):
 _in_flight = []     # (event, buffers): device buffers that kernels on a stream other than torch's current one may still use
 
 
+def _hold(event, buffers):
+    """Keeps buffers until the event has completed, and lets go of those whose event has, one by one: another thread may be adding
+    to the list meanwhile (asking an event releases the interpreter)."""
+    for entry in list(_in_flight):
+        if entry[0].ready():
+            try:
+                _in_flight.remove(entry)
+            except ValueError:      # another thread has let go of it
+                pass
+    _in_flight.append((event, buffers))
+
+
 def _enqueue_on(tensors, st):
     """Stream-side prologue of a call that enqueues on stream `st`: pending completion events of the tensors become
     stream dependencies (tenferro-einsum/src/lib.rs:146-177), never host waits."""
@@ -422,8 +434,7 @@ def _completed_on(outputs, st, used=()):
         if isinstance(t, Tensor):
             t.event = ev
     if st and st != torch.cuda.current_stream().cuda_stream:
-        _in_flight[:] = [(e, bufs) for e, bufs in _in_flight if not e.ready()]
-        _in_flight.append((ev, [t._buf for t in list(used) + list(outputs) if isinstance(t, Tensor)]))
+        _hold(ev, [t._buf for t in list(used) + list(outputs) if isinstance(t, Tensor)])
 
 
 class HipPlan:

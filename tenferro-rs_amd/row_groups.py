@@ -20,7 +20,7 @@ import ctypes as C
 import struct
 
 from . import (BF16, F16, F32, F64, CompletionEvent, CrossMemorySpaceOperation, GpuMemory, InvalidArgument,
-               NoCompatibleComputeDevice, RankMismatch, ShapeMismatch, Tensor, _check, _in_flight, lib, tfh_view)
+               NoCompatibleComputeDevice, RankMismatch, ShapeMismatch, Tensor, _check, _hold, lib, tfh_view)
 
 GATHER_A, SCATTER_C, ZERO_REST = 1, 2, 4      # TFH_ROWS_*
 _MOST = 0x7fffffff      # what the C structure's 32-bit fields hold (ctypes would cut off the rest without a word)
@@ -110,10 +110,8 @@ def _stream(stream, current):
     return stream
 
 
-def _hold(event, tensors):
-    """Keeps the tensors' buffers until the event is done, and lets go of those whose event is."""
-    _in_flight[:] = [(e, held) for e, held in _in_flight if not e.ready()]
-    _in_flight.append((event, [getattr(t, "_buf", t) for t in tensors]))
+def _hold_all(event, tensors):
+    _hold(event, [getattr(t, "_buf", t) for t in tensors])
 
 
 class _Call:
@@ -163,7 +161,7 @@ class _Call:
     def __exit__(self, *error):
         try:
             if error[0] is not None and self.stream != self.current:
-                _hold(CompletionEvent(self.stream), self.used)   # an earlier launch of the call may be using them
+                _hold_all(CompletionEvent(self.stream), self.used)   # an earlier launch of the call may be using them
         finally:
             if self.guard is not None:
                 self.guard.__exit__(*error)
@@ -204,7 +202,7 @@ class _Call:
             for t in tensors:
                 t.event = ev
             if other:
-                _hold(ev, self.used + list(outputs))
+                _hold_all(ev, self.used + list(outputs))
 
 
 class RowGroups:

@@ -1510,3 +1510,23 @@ def test_gradients_of_tensors_are_laid_out_like_them(tf, torch):
     wide = T(up[:1].expand(up.shape[0], -1, -1))                          # one matrix for all groups: nothing to be laid out like
     _, db = tf.ragged_gemm_backward(T(x), wide, T(dc), flat, gather=True)
     assert db.dims() == list(up.shape) and 0 not in db.strides()
+
+
+def test_buffers_held_by_another_thread_meanwhile_stay_held(tf, monkeypatch):
+    # asking an event lets other threads run: what they add to the list of buffers in use stays in it
+    class Event:
+        def __init__(self, done, then=None):
+            self.done, self.then = done, then
+
+        def ready(self):
+            if self.then:
+                self.then()
+            return self.done
+
+    kept = []
+    monkeypatch.setattr(tf, "_in_flight", kept)
+    meanwhile = lambda: kept.append((Event(False), ["theirs"])) if not any(e[1] == ["theirs"] for e in kept) else None
+    gone = (Event(True), ["taken out by the other"])
+    kept += [(Event(True, meanwhile), ["done"]), (Event(False, lambda: kept.remove(gone) if gone in kept else None), ["running"]), gone]
+    tf._hold(Event(False), ["ours"])
+    assert [e[1] for e in kept] == [["running"], ["theirs"], ["ours"]]
