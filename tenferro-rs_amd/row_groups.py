@@ -86,7 +86,7 @@ def _code(t):
         dt = _codes().get(t.dtype, -1)
         if t.requires_grad and _torch.is_grad_enabled():
             raise InvalidArgument("invalid argument: an operand requires grad, which the call records nothing for: detach() it, or call under torch.no_grad()")
-        if _torch.autograd.forward_ad._current_level >= 0 and _torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        if getattr(_torch.autograd.forward_ad, "_current_level", 0) >= 0 and _torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
             raise InvalidArgument("invalid argument: an operand is a forward-mode dual, whose tangent the call knows nothing of")
     if dt not in (BF16, F16, F32, F64):
         raise InvalidArgument(f"invalid argument: operations on rows in groups take bf16, f16, f32 and f64; got {t.dtype}")
